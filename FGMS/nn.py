@@ -110,3 +110,104 @@ class SparseConv(torch.nn.Module):
     def forward(self, feats, kmap):
         out = sparse_conv(feats, self.weight, kmap, self.allow_tf32)
         return out if self.bias is None else out + self.bias
+
+
+# ------------------------------------------------------------------------------- attention
+def rotary_freqs(sections, base=100.0, device=None):
+    """Radians a step for each rotated pair of channels: ``base ** (-i / count)`` for the pairs i of every section."""
+    return torch.cat([torch.empty(0)] + [base ** (-torch.arange(c, dtype=torch.float32) / c) for c in sections if c]).to(device)
+
+
+def norm_rotary(q, k, q_scale, k_scale, coords, freqs, sections, eps=1e-6, interleaved=False):
+    """Root-mean-square norms of queries and keys for each head and their rotation by the rows' coordinates, in one pass;
+    differentiable in q, k and the scales.
+
+    q ``[N, heads, D]``, k ``[N, key heads, D]`` (slices of one projection are read as they lie), scales ``[D]`` or None,
+    coords int32 ``[N, axes]``.  The first ``sections[0]`` pairs of channels turn by ``coords[:, 0] * freqs[pair]``, the next
+    ``sections[1]`` with the second axis, ...; pairs behind the last section stay.  Pair p is channels (p, p + D / 2), with
+    ``interleaved`` (2p, 2p + 1)."""
+    return backend.norm_rotary(q, k, q_scale, k_scale, coords, freqs, list(sections), float(eps), bool(interleaved))
+
+
+def segment_attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=None, k_lengths=None):
+    """Softmax attention inside ragged segments; differentiable in q, k and v.
+
+    q ``[Nq, heads, D]``, k and v ``[Nk, key heads, D]``, heads a multiple of key heads.  Segment s is rows
+    ``q_offsets[s]`` to ``q_offsets[s + 1]`` of q and likewise of k and v (``k_offsets``; None: the same): int32 tensors on
+    the device, from which no size has to come back.  ``causal``: ends of queries and keys aligned, keys behind a query not
+    seen.  A row that sees no key comes out as zeros.  ``k_lengths`` (int32, one a segment; no gradients): how much of each
+    segment of k and v is in use, for caches with room left.  ``scale`` is positive, None: ``1 / sqrt(D)``."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    return backend.segment_attention(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, k_lengths, bool(causal), float(scale))
+
+
+def window_segments(coords, size):
+    """Voxels by window: (order, offsets) so that rows ``order[offsets[s]:offsets[s + 1]]`` are the voxels of window s, cells of
+    ``size`` voxels (a number, or one for each axis).  Waits for the number of windows."""
+    cells = torch.div(coords, torch.as_tensor(size, device=coords.device), rounding_mode="floor")
+    _, window, counts = torch.unique(cells, dim=0, return_inverse=True, return_counts=True)
+    offsets = torch.zeros(counts.numel() + 1, dtype=torch.int32, device=coords.device)
+    offsets[1:] = torch.cumsum(counts, 0)
+    return torch.argsort(window, stable=True), offsets
+
+
+class VoxelCache:
+    """Keys and values of ``segments`` scans with room for ``capacity`` rows each, filled row by row."""
+
+    def __init__(self, segments, capacity, kv_heads, dim, dtype=None, device=None):
+        self.capacity = capacity
+        self.k = torch.zeros(segments * capacity, kv_heads, dim, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.offsets = torch.arange(segments + 1, dtype=torch.int32, device=device) * capacity
+        self.lengths = torch.zeros(segments, dtype=torch.int32, device=device)
+
+    def append(self, k, v):
+        """One new row for every scan; a full scan keeps its last row replaced."""
+        rows = (self.offsets[:-1] + self.lengths.clamp(max=self.capacity - 1)).long()
+        self.k.index_copy_(0, rows, k)
+        self.v.index_copy_(0, rows, v)
+        self.lengths.add_(1).clamp_(max=self.capacity)
+
+
+class VoxelAttention(torch.nn.Module):
+    """Attention among the voxels of each segment, positions by rotation: ``y = layer(feats, coords, offsets)`` with the rows
+    of a segment next to each other (:func:`window_segments`), or row by row over a :class:`VoxelCache`:
+    ``y = layer.step(feats, coords, cache)``.
+
+    ``sections`` shares the ``channels / heads / 2`` pairs of a head out among the coordinates' axes."""
+
+    def __init__(self, channels, heads, kv_heads=None, sections=None, base=100.0, causal=False, dtype=None, device=None):
+        super().__init__()
+        self.heads, self.kv_heads, self.causal = heads, kv_heads or heads, causal
+        if channels % heads or heads % self.kv_heads:
+            raise ValueError("channels must be a multiple of heads, and heads of kv_heads")
+        self.dim = channels // heads
+        pairs = self.dim // 2
+        self.sections = tuple(sections) if sections is not None else (pairs - 2 * (pairs // 3), pairs // 3, pairs // 3)
+        self.qkv = torch.nn.Linear(channels, (heads + 2 * self.kv_heads) * self.dim, bias=False, dtype=dtype, device=device)
+        self.q_scale = torch.nn.Parameter(torch.ones(self.dim, dtype=dtype, device=device))
+        self.k_scale = torch.nn.Parameter(torch.ones(self.dim, dtype=dtype, device=device))
+        self.out = torch.nn.Linear(channels, channels, bias=False, dtype=dtype, device=device)
+        # (angles stay fp32 whatever the layer is cast to)
+        self._freqs = rotary_freqs(self.sections, base)
+
+    def _heads(self, feats, coords):
+        h, hk, d = self.heads, self.kv_heads, self.dim
+        q, k, v = (t.unflatten(-1, (-1, d)) for t in self.qkv(feats).split((h * d, hk * d, hk * d), -1))
+        if self._freqs.device != feats.device:
+            self._freqs = self._freqs.to(feats.device)
+        q, k = norm_rotary(q, k, self.q_scale, self.k_scale, coords, self._freqs, self.sections)
+        return q, k, v
+
+    def forward(self, feats, coords, offsets):
+        q, k, v = self._heads(feats, coords)
+        return self.out(segment_attention(q, k, v, offsets, causal=self.causal).flatten(1))
+
+    def step(self, feats, coords, cache):
+        """One new row of every scan: its keys and values join the cache, its query sees all of them."""
+        q, k, v = self._heads(feats, coords)
+        cache.append(k, v)
+        ones = torch.arange(feats.shape[0] + 1, dtype=torch.int32, device=feats.device)
+        y = segment_attention(q, cache.k, cache.v, ones, cache.offsets, k_lengths=cache.lengths)
+        return self.out(y.flatten(1))

@@ -20,7 +20,10 @@ LIB_PATH = os.path.join(LIB_DIR, "libfgms_hip.so")
 OBJ_DIR = os.path.join(ROOT, "build", "obj")
 
 HIP_SOURCES = ["fgms_api.hip", "fgms_generic.hip", "fgms_plan.hip", "fgms_mfma.hip", "fgms_small.hip", "fgms_narrow.hip", "fgms_wgrad.hip",
-               "fgms_probe.hip", "fgms_kmap.hip", "fgms_wide.hip", "fgms_pad.hip", "fgms_brief.hip"]
+               "fgms_probe.hip", "fgms_kmap.hip", "fgms_wide.hip", "fgms_pad.hip", "fgms_brief.hip",
+               "fgms_norm_rotary.hip", "fgms_attention.hip", "fgms_attention_f16.hip", "fgms_attention_bf16.hip", "fgms_attention_f32.hip"]
+
+TORCH_SOURCES = ["fgms_torch.cpp", "fgms_torch_attention.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
@@ -75,12 +78,23 @@ def build_torch_ext(verbose=False):
                                    os.path.join(ROOT, "include")]:
         inc += ["-I", p]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    # host-only translation unit: no device code, so the plain C++ driver does
-    cmd = [CXX, "-O2", "-fPIC", "-std=c++17", "-shared",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=backend",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi,
-           "-Wno-deprecated-declarations", "-I", "/opt/rocm/include"] + inc + [
-           os.path.join(CSRC, "fgms_torch.cpp"), "-o", out,
+    # host-only translation units: no device code, so the plain C++ driver does
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    flags = ["-O2", "-fPIC", "-std=c++17",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=backend",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi,
+             "-Wno-deprecated-declarations", "-I", "/opt/rocm/include"] + inc
+
+    def compile_one(src):
+        obj = os.path.join(OBJ_DIR, src.replace(".cpp", ".o"))
+        o = _run([CXX] + flags + ["-c", os.path.join(CSRC, src), "-o", obj])
+        if verbose and o.strip():
+            print(o)
+        return obj
+
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        objs = list(ex.map(compile_one, TORCH_SOURCES))
+    cmd = [CXX, "-shared", "-o", out] + objs + [
            "-L", tlib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
            "-L", LIB_DIR, "-lfgms_hip",
            "-Wl,-rpath,$ORIGIN/../fgms_amd/lib", "-Wl,-rpath," + tlib]

@@ -12,13 +12,14 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libfgms_hip.so")
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 SYMBOLS = [
     "fgms_version", "fgms_last_error", "fgms_plan_create", "fgms_plan_check", "fgms_plan_transposed", "fgms_plan_destroy",
     "fgms_plan_usable", "fgms_plan_stats", "fgms_conv_fwd", "fgms_conv_bwd", "fgms_fusion_fwd", "fgms_fwd", "fgms_bwd", "fgms_dgrad",
     "fgms_wgrad", "fgms_wgrad_static", "fgms_set_kernel_policy", "fgms_profile_enable", "fgms_profile_read",
     "fgms_profile_reset", "fgms_probe_gather", "fgms_build_kernel_map", "fgms_build_map_begin", "fgms_build_map_end", "fgms_allocation_count",
     "fgms_weights_pin", "fgms_weights_unpin", "fgms_relaid_weights_hits",
+    "fgms_norm_rotary_fwd", "fgms_norm_rotary_bwd", "fgms_segment_attention_fwd", "fgms_segment_attention_bwd",
 ]
 
 _lib = None
@@ -78,6 +79,12 @@ def lib():
     L.fgms_weights_pin.restype = i32
     L.fgms_weights_unpin.argtypes = [vp]
     L.fgms_weights_unpin.restype = i32
+    f32, turn, rows = ctypes.c_float, [i32, vp, i32, ctypes.c_float, i32, vp], [i64] * 4
+    L.fgms_norm_rotary_fwd.argtypes = [vp] * 8 + [i64, i32, i32, i32] + rows + turn
+    L.fgms_norm_rotary_bwd.argtypes = [vp] * 12 + [i64, i32, i32, i32] + rows + turn
+    attention = [i64, i64, i32, i32, i32, i32] + [i64] * 6 + [i32, f32, i32, vp]
+    L.fgms_segment_attention_fwd.argtypes = [vp] * 8 + attention
+    L.fgms_segment_attention_bwd.argtypes = [vp] * 11 + attention
     L.fgms_profile_enable.argtypes = [i32]
     L.fgms_profile_enable.restype = None
     L.fgms_profile_reset.restype = None
@@ -364,3 +371,82 @@ def wgrad_static(in_feats, out_grad, kernel_grad, kpos, in_map, out_map, plan=No
         _p(in_feats), _p(out_grad), _p(kernel_grad), _p(kpos), _p(in_map), _p(out_map),
         in_feats.shape[0], out_grad.shape[0], kernel_grad.shape[1], kernel_grad.shape[2],
         kernel_grad.shape[0], in_map.numel(), _dtype(in_feats), _ph(plan), _stream()))
+
+
+_ATTENTION_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _attention_dtype(t):
+    if t.dtype not in _ATTENTION_DTYPES:
+        raise ValueError("FGMS attention handles float32, float16 and bfloat16 tensors")
+    return _ATTENTION_DTYPES[t.dtype]
+
+
+def _need_rows(t, name, like):
+    if not t.is_cuda or t.dim() != 3 or t.stride(2) != 1 or t.dtype != like.dtype:
+        raise ValueError("%s must be [rows, heads, channels] of q's dtype on the GPU, channels side by side" % name)
+
+
+def _turn(q, k, coords, freqs, sections, interleaved, eps):
+    _need_rows(q, "q", q)
+    _need_rows(k, "k", q)
+    _need(coords, "coords", torch.int32)
+    _need(freqs, "freqs", torch.float32)
+    if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or tuple(coords.shape) != (q.shape[0], len(sections)) \
+            or freqs.numel() != sum(sections):
+        raise ValueError("q, k, coords, freqs and sections do not go together")
+    return (q.shape[0], q.shape[1], k.shape[1], q.shape[2], q.stride(0), q.stride(1), k.stride(0), k.stride(1), len(sections),
+            (ctypes.c_int * len(sections))(*sections), int(interleaved), float(eps), _attention_dtype(q), _stream())
+
+
+def norm_rotary_fwd(q, k, q_scale, k_scale, coords, freqs, sections, q_out, k_out, eps=1e-6, interleaved=False):
+    """``fgms_norm_rotary_fwd``; scales may be None."""
+    for t, n in ((q_scale, "q_scale"), (k_scale, "k_scale"), (q_out, "q_out"), (k_out, "k_out")):
+        if t is not None:
+            _need(t, n, q.dtype)
+    rest = _turn(q, k, coords, freqs, sections, interleaved, eps)
+    _check(lib().fgms_norm_rotary_fwd(_p(q), _p(k), _p(q_scale), _p(k_scale), _p(coords), _p(freqs), _p(q_out), _p(k_out), *rest))
+
+
+def norm_rotary_bwd(q_out_grad, k_out_grad, q, k, q_scale, k_scale, coords, freqs, sections, q_grad, k_grad, q_scale_grad=None,
+                    k_scale_grad=None, eps=1e-6, interleaved=False):
+    """``fgms_norm_rotary_bwd``: gradients are written; None: not wanted."""
+    for t, n in ((q_out_grad, "q_out_grad"), (k_out_grad, "k_out_grad"), (q_scale, "q_scale"), (k_scale, "k_scale"), (q_grad, "q_grad"),
+                 (k_grad, "k_grad"), (q_scale_grad, "q_scale_grad"), (k_scale_grad, "k_scale_grad")):
+        if t is not None:
+            _need(t, n, q.dtype)
+    rest = _turn(q, k, coords, freqs, sections, interleaved, eps)
+    _check(lib().fgms_norm_rotary_bwd(_p(q_out_grad), _p(k_out_grad), _p(q), _p(k), _p(q_scale), _p(k_scale), _p(coords), _p(freqs),
+                                      _p(q_grad), _p(k_grad), _p(q_scale_grad), _p(k_scale_grad), *rest))
+
+
+def _segments(q, k, v, q_offsets, k_offsets, causal, scale):
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        _need_rows(t, n, q)
+    _need(q_offsets, "q_offsets", torch.int32)
+    _need(k_offsets, "k_offsets", torch.int32)
+    if k.shape != v.shape or q.shape[2] != k.shape[2] or q_offsets.numel() != k_offsets.numel() or q_offsets.numel() < 1:
+        raise ValueError("q, k, v and the offsets do not go together")
+    return (q.shape[0], k.shape[0], q_offsets.numel() - 1, q.shape[1], k.shape[1], q.shape[2], q.stride(0), q.stride(1), k.stride(0),
+            k.stride(1), v.stride(0), v.stride(1), int(causal), float(scale), _attention_dtype(q), _stream())
+
+
+def segment_attention_fwd(q, k, v, out, lse, q_offsets, k_offsets, k_lengths=None, causal=False, scale=1.0):
+    """``fgms_segment_attention_fwd``; lse (fp32 [rows, heads]) may be None."""
+    _need(out, "out", q.dtype)
+    for t, n, d in ((lse, "lse", torch.float32), (k_lengths, "k_lengths", torch.int32)):
+        if t is not None:
+            _need(t, n, d)
+    rest = _segments(q, k, v, q_offsets, k_offsets, causal, scale)
+    _check(lib().fgms_segment_attention_fwd(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(q_offsets), _p(k_offsets), _p(k_lengths), *rest))
+
+
+def segment_attention_bwd(out_grad, q, k, v, out, lse, q_grad, k_grad, v_grad, q_offsets, k_offsets, causal=False, scale=1.0):
+    """``fgms_segment_attention_bwd``: gradients are written; None: not wanted."""
+    for t, n in ((out_grad, "out_grad"), (out, "out"), (q_grad, "q_grad"), (k_grad, "k_grad"), (v_grad, "v_grad")):
+        if t is not None:
+            _need(t, n, q.dtype)
+    _need(lse, "lse", torch.float32)
+    rest = _segments(q, k, v, q_offsets, k_offsets, causal, scale)
+    _check(lib().fgms_segment_attention_bwd(_p(out_grad), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(q_grad), _p(k_grad), _p(v_grad),
+                                            _p(q_offsets), _p(k_offsets), *rest))

@@ -1,0 +1,216 @@
+// Attention over ragged segments: arguments, and the pieces its kernels share.
+//
+// A segment is a range of rows of q and a range of rows of k and v (a window of a cloud, a scan, a cache);
+// where they begin is read on the device, so that no size comes back to the host.  Query heads come in
+// groups of `group` that share a key head.  For one segment and key head the queries of a group are
+// group * Lq rows of one matrix, row r being head r % group of token r / group: the keys are then read once
+// for the whole group, and a single new token still fills several rows of a tile.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "fgms_internal.h"
+#include "fgms_mma.h"
+
+namespace fgms {
+
+struct AttentionArgs {
+  const void *q, *k, *v;
+  const int32_t *q_offsets, *k_offsets, *k_lengths;      // [segments + 1], [segments + 1], [segments] or nullptr
+  int64_t n_q, n_k;
+  int segments, heads, kv_heads, dim;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
+  float scale;
+  int causal;
+  int dtype;
+  hipStream_t stream;
+  // forward: written; backward: read
+  void *out;             // [n_q, heads, dim]
+  float *lse;            // [n_q, heads]: log of the row's sum of exponentials, -inf for a row without keys
+  // backward
+  const void *g_out;     // [n_q, heads, dim]
+  float *delta;          // [n_q, heads]: g_out . out
+  void *gq, *gk, *gv;    // contiguous, any of them may be nullptr
+  // a long axis cut into `parts` pieces, joined by a second launch
+  int parts;
+  float *part_sum;       // [slot][kv head][part][tile row][dim]
+  float *part_lse;       // [slot][kv head][part][tile row]
+};
+
+int launch_attention_fwd(AttentionArgs a);
+int launch_attention_bwd(AttentionArgs a);
+// For one type (fgms_attention_f16.hip, _bf16.hip, _f32.hip).
+template <typename T> int attention_fwd(const AttentionArgs &a);
+template <typename T> int attention_bwd(const AttentionArgs &a);
+
+// Tiles of `rows` rows, numbered segment by segment without their lengths being known: segment s begins at slot
+// offset[s] / rows + s, which leaves it ceil(length / rows) slots at least; a slot behind its segment's last row has
+// nothing to do.  Rows behind the last segment are a segment of their own (number `segments`), without partners.
+__host__ __device__ inline int64_t attention_slots(int64_t n, int64_t segments, int64_t rows) { return n / rows + segments + 1; }
+
+#ifdef __HIPCC__
+
+// Row at which segment s begins, whatever stands in the offsets.
+__device__ __forceinline__ int64_t segment_begin(const int32_t *__restrict__ offsets, int s, int segments, int64_t n) {
+  if (s <= 0) return 0;
+  if (s > segments) return n;
+  const int64_t at = offsets[s];
+  return at < 0 ? 0 : at > n ? n : at;
+}
+
+struct Slot {
+  int segment;
+  int64_t begin, length;      // the segment's rows (times `group`: length in rows of the tile's matrix)
+  int64_t first;              // the tile's first row, in the segment
+};
+
+// The slot's segment, by a search that asks 64 of them at a time.  `group`: rows of the matrix to a row of the tensor.
+__device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, int segments, int64_t n, int group, int rows,
+                                          int64_t slot) {
+  const int lane = threadIdx.x % 64;
+  int64_t lo = 0, hi = (int64_t)segments + 1;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+    const bool before = at < hi && segment_begin(offsets, (int)at, segments, n) * group / rows + at <= slot;
+    const unsigned long long after = ~__builtin_amdgcn_ballot_w64(before);
+    lo += (after ? __builtin_ctzll(after) : 64) * step;      // (an entry that did begin before, in whatever order the others are)
+    hi = hi < lo + step ? hi : lo + step;
+  }
+  Slot r;
+  r.segment = __builtin_amdgcn_readfirstlane((int)lo);
+  r.begin = segment_begin(offsets, r.segment, segments, n);
+  const int64_t end = segment_begin(offsets, r.segment + 1, segments, n);
+  r.length = end > r.begin ? (end - r.begin) * group : 0;
+  r.first = (slot - (r.begin * group / rows + r.segment)) * rows;
+  return r;
+}
+
+// The rows of the other side that go with segment s.
+__device__ __forceinline__ void partner_rows(const int32_t *__restrict__ offsets, const int32_t *__restrict__ lengths, int s,
+                                             int segments, int64_t n, int64_t &begin, int64_t &length) {
+  begin = segment_begin(offsets, s, segments, n);
+  const int64_t end = segment_begin(offsets, s + 1, segments, n);
+  length = s < segments && end > begin ? end - begin : 0;
+  if (lengths && s < segments) {
+    const int64_t used = lengths[s];
+    length = used < 0 ? 0 : used < length ? used : length;
+  }
+}
+
+// acc += a x b, 16 bytes of the contracted axis a lane: 16 deep for 16-bit types, 8 for float.
+template <typename T>
+__device__ __forceinline__ void multiply(float16v &acc, const int4v &a, const int4v &b) {
+  if constexpr (__is_same(T, _Float16)) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), acc, 0, 0, 0);
+  } else if constexpr (__is_same(T, __bf16)) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+    const float4v fa = __builtin_bit_cast(float4v, a), fb = __builtin_bit_cast(float4v, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[e], fb[e], acc, 0, 0, 0);
+  }
+}
+
+// A tile of rows in LDS, DP channels each, in 16-byte chunks.  A fragment of rows is read by 32 lanes that ask 32 rows
+// for the same chunk, one of columns (16-bit types: the transposing read) by 16 lanes that ask four rows for four chunks,
+// two rows' worth beside it.  Chunk c of a row lies at c ^ swizzle(row): both kinds then cover all banks, the first over 16 rows,
+// the second over its four (rows of 256 bytes: the row's lowest two bits move groups of four chunks, the next two the chunks
+// in them; of 128: bit 1 moves groups, as two rows share 256 bytes; of 64: four rows do).
+template <typename T, int DP>
+struct RowTile {
+  static constexpr int E = 16 / (int)sizeof(T), CH = DP / E;
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (CH % 16 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (CH % 8 == 0) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+  }
+  static __device__ __forceinline__ int at(int row, int c) { return row * CH + (c ^ swizzle(row)); }
+  // operand with the tile's rows as its outer index: lane l has row row0 + l % 32, chunk 2 * step + l / 32
+  static __device__ __forceinline__ int4v rows(const int4v *tile, int row0, int step, int lane) {
+    return tile[at(row0 + lane % 32, 2 * step + lane / 32)];
+  }
+  // 16-bit types: operand with the tile's columns as its outer index, contracted over its rows: lane l has column
+  // col0 + l % 32 of rows row0 + 4 * (l / 32) + {0 .. 3} and, 8 further down, four more -- the rows whose products the
+  // accumulator registers 8 i .. 8 i + 7 of that lane hold, so that these are the other operand as they are
+  static __device__ __forceinline__ int4v columns(const int4v *tile, int row0, int col0, int lane) {
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    typedef short short8v __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) short4v lds_v4;
+    const int i = lane & 15, row = row0 + 4 * (lane >> 5) + (i >> 2), c = col0 / 8 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+    const short *base = reinterpret_cast<const short *>(tile);
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4 *)(base + at(row, c) * 8 + (i & 1) * 4));
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4 *)(base + at(row + 8, c) * 8 + (i & 1) * 4));
+    const short8v v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(int4v, v);
+  }
+  static __device__ __forceinline__ float element(const int4v *tile, int row, int col) {
+    return reinterpret_cast<const float *>(tile)[at(row, col / 4) * 4 + col % 4];
+  }
+};
+
+// out[channel][lane's row] += sum over 32 rows of the tile from row0 on of tile[row][channel] * w[row][lane's row]; w as an
+// accumulator holds it (register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32), rounded to T.
+template <typename T, int DP>
+__device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], const int4v *tile, int row0, const float16v &w, int lane) {
+  using Rows = RowTile<T, DP>;
+  if constexpr (sizeof(T) == 2) {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    typedef float float8v __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float8v part = {w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3], w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]};
+      const int4v b = __builtin_bit_cast(int4v, __builtin_convertvector(part, T8));
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) multiply<T>(out[db], Rows::columns(tile, row0 + 16 * i, db * 32, lane), b);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+        out[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(Rows::element(tile, row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4, db * 32 + lane % 32),
+                                                       w[r], out[db], 0, 0, 0);
+  }
+}
+
+// The larger of / the sum over lanes l and l ^ 32.
+__device__ __forceinline__ float both_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return __builtin_fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+
+// Row `row` (or nullptr) of `dim` channels into fragments, zeros where there is nothing.
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(int4v (&to)[DP / (32 / (int)sizeof(T))], const T *row, int dim, int lane) {
+  constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int s = 0; s < DP / (2 * E); ++s) {
+    const int c = (2 * s + lane / 32) * E;
+    to[s] = row && c < dim ? *reinterpret_cast<const int4v *>(row + c) : int4v{0, 0, 0, 0};
+  }
+}
+
+// A lane's row of a result, from accumulators that hold it as columns, times `by`.
+template <typename To, int DP>
+__device__ __forceinline__ void store_row(To *row, const float16v (&acc)[DP / 32], float by, int dim, int lane) {
+  typedef To To4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int c = db * 32 + 8 * p + 4 * (lane / 32);
+      const float4v v = {acc[db][4 * p] * by, acc[db][4 * p + 1] * by, acc[db][4 * p + 2] * by, acc[db][4 * p + 3] * by};
+      if (c < dim) *reinterpret_cast<To4 *>(row + c) = __builtin_convertvector(v, To4);
+    }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+#endif
+
+}  // namespace fgms

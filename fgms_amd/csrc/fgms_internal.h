@@ -227,7 +227,10 @@ bool is_capturing(hipStream_t stream);   // into a HIP graph
 // all-zero between calls), slot 2: the generic kernel's accumulator, slot 3: the gather probe's sink,
 // slots 4 .. 7: padded copies of input rows, output rows, weights and a result (fgms_pad.hip), slot 8: the
 // workgroups' sums of a narrow layer's weight gradient (fgms_narrow.hip).
+// slot 9: parts of a long axis on their way to their join, slot 10: g_out . out of attention's rows (fgms_attention_bodies.h),
+// slot 11: the workgroups' sums of the norms' scales' gradients (fgms_norm_rotary.hip).
 // *fresh (optional) is set when the buffer was (re)allocated by this call.
+constexpr int kSlotAttention = 9, kSlotAttentionDelta = 10, kSlotScaleSums = 11;
 int workspace_get(hipStream_t stream, int slot, size_t bytes, void **ptr, bool *fresh = nullptr);
 // Buffer for a re-laid copy of a.w in `layout` (any number that tells the layouts of one weight
 // tensor apart): the stream's workspace, to be filled (*fill = true), or -- for weights under

@@ -43,6 +43,7 @@
 
 #include "fgms.h"
 #include "fgms_diag.h"
+#include "fgms_torch_attention.h"
 
 namespace {
 
@@ -542,6 +543,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
            pybind11::call_guard<pybind11::gil_scoped_release>())
       .def("finish", &MapOnItsWay::finish, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("sparse_conv", &sparse_conv);
+  m.def("norm_rotary", &norm_rotary);
+  m.def("segment_attention", &segment_attention);
   m.def("fgms_fusion_fwd_cuda", &ConvolutionForwardFused);
   m.def("fgms_fwd_cuda", &ConvolutionForward);
   m.def("fgms_bwd_cuda", &ConvolutionBackward);

@@ -48,6 +48,7 @@ extern "C" {
 
 #define FGMS_F32 0
 #define FGMS_F16 1
+#define FGMS_BF16 2      /* attention and the norms in front of it only */
 
 #define FGMS_OK 0
 #define FGMS_E_INVALID (-1)   /* bad argument (shape, dtype, null pointer)   */
@@ -271,6 +272,74 @@ int fgms_build_map_begin(fgms_map_build_t **build, const int32_t *in_coords, int
                          int32_t *in_map, int32_t *out_map, int64_t capacity,
                          int32_t *kernel_nnz, int32_t *kpos, int32_t *qkpos, int want_plan, void *stream);
 int fgms_build_map_end(fgms_map_build_t *build, int32_t *host_nnz, int64_t *n_pairs, fgms_plan_t **plan);
+
+/*
+ * Attention over voxel clouds: what goes between sparse convolutions where rows are to exchange
+ * information by content.  No counterpart in the reference.  Types: FGMS_F32, FGMS_F16, FGMS_BF16;
+ * heads of 8, 16, ... 128 channels.  Inputs are [rows, heads, head_dim] with the channels of a head next
+ * to each other and row and head strides given in ELEMENTS (slices of one projection do), every row of a
+ * head on 16 bytes; results and their gradients are contiguous and begin on 16 bytes.  Sums, softmax
+ * statistics and norms are fp32.
+ */
+
+/*
+ * Norms of queries and keys for each head and their rotation by the rows' coordinates, in one pass:
+ *   z = x * scale / sqrt(mean(x^2) + eps)                                (over a head's channels)
+ *   pair p of channels (a, b): y_a = z_a cos f - z_b sin f, y_b = z_a sin f + z_b cos f,
+ *   f = coords[row][axis] * freqs[p]
+ * Pair p is (p, p + head_dim / 2), with interleaved != 0 (2p, 2p + 1).  The first sections[0] pairs turn
+ * with axis 0, the next sections[1] with axis 1, ...; pairs behind the last section stay as they are.
+ *   - q [n, q_heads, head_dim], k [n, k_heads, head_dim] (k_heads = 0: none); q_scale, k_scale [head_dim] of
+ *     the same type, NULL: ones; q_out, k_out: contiguous
+ *   - coords: int32 [n, axes], device; freqs: fp32 [sum of sections], device; sections: HOST int [axes],
+ *     1 to 4 axes.  Any 32-bit coordinate: the angle is reduced in 64 bits.
+ * The backward call writes the gradients of q, k and the scales; NULL: not wanted.  The scales' gradients
+ * are summed in a fixed order.
+ */
+int fgms_norm_rotary_fwd(const void *q, const void *k, const void *q_scale, const void *k_scale,
+                         const int32_t *coords, const float *freqs, void *q_out, void *k_out,
+                         int64_t n, int q_heads, int k_heads, int head_dim,
+                         int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                         int axes, const int *sections, int interleaved, float eps, int dtype, void *stream);
+int fgms_norm_rotary_bwd(const void *q_out_grad, const void *k_out_grad,
+                         const void *q, const void *k, const void *q_scale, const void *k_scale,
+                         const int32_t *coords, const float *freqs,
+                         void *q_grad, void *k_grad, void *q_scale_grad, void *k_scale_grad,
+                         int64_t n, int q_heads, int k_heads, int head_dim,
+                         int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                         int axes, const int *sections, int interleaved, float eps, int dtype, void *stream);
+
+/*
+ * Softmax attention inside segments:  out_i = sum_j p_ij v_j,  p_i = softmax_j(scale * q_i . k_j)  over the
+ * keys j of i's segment.
+ *   - q [n_q, heads, head_dim], k and v [n_k, kv_heads, head_dim]; heads a multiple of kv_heads, head h reads
+ *     key head h / (heads / kv_heads)
+ *   - segment s: rows [q_offsets[s], q_offsets[s + 1]) of q and [k_offsets[s], k_offsets[s + 1]) of k and v;
+ *     int32 [segments + 1], device, not decreasing, the first taken as 0.  Lengths may be 0 on either side, and no
+ *     length is needed on the host.  Rows of q behind the last offset see nothing.
+ *   - k_lengths: NULL, or int32 [segments], device: only the first k_lengths[s] rows of segment s are keys
+ *     (caches with room left; what lies behind is not read)
+ *   - causal != 0: the last query of a segment sees all of its keys, the one before it one less, ...
+ *   - a row that sees no key: out 0 (and lse -infinity, gradients 0)
+ *   - lse: fp32 [n_q, heads], the log of each row's sum of exponentials, for the backward call; may be NULL
+ *   - scale: positive
+ * Few queries over many keys (a new row and its cache) are cut along the keys, in a workspace of the stream.
+ * The backward call forms the probabilities again from q, k and lse; it writes the gradients whose pointers
+ * are not NULL, sums over the heads of a group included.  No atomics: the same bits every time.
+ * Values of v that are infinite or NaN reach rows that see them, and with `causal` may turn other rows of the
+ * same segment into NaN.
+ */
+int fgms_segment_attention_fwd(const void *q, const void *k, const void *v, void *out, float *lse,
+                               const int32_t *q_offsets, const int32_t *k_offsets, const int32_t *k_lengths,
+                               int64_t n_q, int64_t n_k, int segments, int heads, int kv_heads, int head_dim,
+                               int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                               int64_t v_row, int64_t v_head, int causal, float scale, int dtype, void *stream);
+int fgms_segment_attention_bwd(const void *out_grad, const void *q, const void *k, const void *v,
+                               const void *out, const float *lse, void *q_grad, void *k_grad, void *v_grad,
+                               const int32_t *q_offsets, const int32_t *k_offsets,
+                               int64_t n_q, int64_t n_k, int segments, int heads, int kv_heads, int head_dim,
+                               int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                               int64_t v_row, int64_t v_head, int causal, float scale, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

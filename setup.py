@@ -41,7 +41,7 @@ setup(
     version="1.3+gfx950",
     packages=["FGMS", "fgms_amd"],
     # the sources are listed for sdists; BuildNative compiles them itself
-    ext_modules=[Extension("FGMS.backend", sources=["fgms_amd/csrc/fgms_torch.cpp"])],
+    ext_modules=[Extension("FGMS.backend", sources=["fgms_amd/csrc/fgms_torch.cpp", "fgms_amd/csrc/fgms_torch_attention.cpp"])],
     cmdclass={"build_ext": BuildNative},
     zip_safe=False,
 )
