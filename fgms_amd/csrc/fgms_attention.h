@@ -18,7 +18,7 @@ namespace fgms {
 struct AttentionArgs {
   const void *q, *k, *v;
   const int32_t *q_offsets, *k_offsets, *k_lengths;      // [segments + 1], [segments + 1], [segments] or nullptr
-  int64_t n_q, n_k;
+  int n_q, n_k;
   int segments, heads, kv_heads, dim;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
   float scale;
@@ -32,6 +32,7 @@ struct AttentionArgs {
   const void *g_out;     // [n_q, heads, dim]
   float *delta;          // [n_q, heads]: g_out . out
   void *gq, *gk, *gv;    // contiguous, any of them may be nullptr
+  int order, slots;      // of the workgroups (place_of), and the tiles of each key head
   // a long axis cut into `parts` pieces, joined by a second launch
   int parts;
   float *part_sum;       // [slot][kv head][part][tile row][dim]
@@ -47,40 +48,42 @@ template <typename T> int attention_bwd(const AttentionArgs &a);
 // Tiles of `rows` rows, numbered segment by segment without their lengths being known: segment s begins at slot
 // offset[s] / rows + s, which leaves it ceil(length / rows) slots at least; a slot behind its segment's last row has
 // nothing to do.  Rows behind the last segment are a segment of their own (number `segments`), without partners.
-__host__ __device__ inline int64_t attention_slots(int64_t n, int64_t segments, int64_t rows) { return n / rows + segments + 1; }
+__host__ __device__ inline int64_t attention_slots(int64_t n, int64_t segments, int rows) { return n / rows + segments + 1; }
 
 #ifdef __HIPCC__
 
-// Row at which segment s begins, whatever stands in the offsets.
-__device__ __forceinline__ int64_t segment_begin(const int32_t *__restrict__ offsets, int s, int segments, int64_t n) {
-  if (s <= 0) return 0;
-  if (s > segments) return n;
-  const int64_t at = offsets[s];
-  return at < 0 ? 0 : at > n ? n : at;
+// Row at which segment s begins, whatever stands in the offsets.  (One load for any s, and no branch around it.)
+__device__ __forceinline__ int segment_begin(const int32_t *__restrict__ offsets, int s, int segments, int n) {
+  const int at = offsets[min(max(s, 0), segments)];
+  return s <= 0 ? 0 : s > segments ? n : min(max(at, 0), n);
 }
 
 struct Slot {
   int segment;
-  int64_t begin, length;      // the segment's rows (times `group`: length in rows of the tile's matrix)
-  int64_t first;              // the tile's first row, in the segment
+  int begin, length;      // the segment's rows (times `group`: length in rows of the tile's matrix)
+  int first;              // the tile's first row, in the segment
 };
 
-// The slot's segment, by a search that asks 64 of them at a time.  `group`: rows of the matrix to a row of the tensor.
-__device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, int segments, int64_t n, int group, int rows,
-                                          int64_t slot) {
+// x / by for 0 <= x < 2^22, from by's reciprocal: (x + 1/2) / by is at least 1 / (2 by) from a whole number, and the product off by
+// less than (x + 1/2) 2^-23 / by.
+__device__ __forceinline__ int divide(int x, float reciprocal) { return (int)(((float)x + 0.5f) * reciprocal); }
+
+// The slot's segment, by a search that asks 64 of them at a time.  `group`: rows of the matrix to a row of the tensor; all rows of
+// the tensor times `group` are less than 2^31.
+__device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, int segments, int n, int group, int rows, int slot) {
   const int lane = threadIdx.x % 64;
-  int64_t lo = 0, hi = (int64_t)segments + 1;
+  int lo = 0, hi = segments + 1;
   while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
-    const bool before = at < hi && segment_begin(offsets, (int)at, segments, n) * group / rows + at <= slot;
+    const int step = (int)(((unsigned)(hi - lo) + 63u) / 64u), at = (int)min((unsigned)lo + (lane + 1u) * (unsigned)step, (unsigned)hi);
+    const bool before = at < hi && segment_begin(offsets, at, segments, n) * group / rows + at <= slot;
     const unsigned long long after = ~__builtin_amdgcn_ballot_w64(before);
     lo += (after ? __builtin_ctzll(after) : 64) * step;      // (an entry that did begin before, in whatever order the others are)
-    hi = hi < lo + step ? hi : lo + step;
+    hi = min(hi, lo + step);
   }
   Slot r;
-  r.segment = __builtin_amdgcn_readfirstlane((int)lo);
+  r.segment = __builtin_amdgcn_readfirstlane(lo);
   r.begin = segment_begin(offsets, r.segment, segments, n);
-  const int64_t end = segment_begin(offsets, r.segment + 1, segments, n);
+  const int end = segment_begin(offsets, r.segment + 1, segments, n);
   r.length = end > r.begin ? (end - r.begin) * group : 0;
   r.first = (slot - (r.begin * group / rows + r.segment)) * rows;
   return r;
@@ -88,14 +91,11 @@ __device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, i
 
 // The rows of the other side that go with segment s.
 __device__ __forceinline__ void partner_rows(const int32_t *__restrict__ offsets, const int32_t *__restrict__ lengths, int s,
-                                             int segments, int64_t n, int64_t &begin, int64_t &length) {
+                                             int segments, int n, int &begin, int &length) {
   begin = segment_begin(offsets, s, segments, n);
-  const int64_t end = segment_begin(offsets, s + 1, segments, n);
+  const int end = segment_begin(offsets, s + 1, segments, n);
   length = s < segments && end > begin ? end - begin : 0;
-  if (lengths && s < segments) {
-    const int64_t used = lengths[s];
-    length = used < 0 ? 0 : used < length ? used : length;
-  }
+  if (lengths && s < segments) length = min(max(lengths[s], 0), length);
 }
 
 // acc += a x b, 16 bytes of the contracted axis a lane: 16 deep for 16-bit types, 8 for float.
@@ -144,13 +144,24 @@ struct RowTile {
     const short8v v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(int4v, v);
   }
-  static __device__ __forceinline__ float element(const int4v *tile, int row, int col) {
-    return reinterpret_cast<const float *>(tile)[at(row, col / 4) * 4 + col % 4];
+  // float: channels (DP / 32) * (l % 32) + {0 .. DP / 32 - 1} of a row, one for each block of 32
+  static __device__ __forceinline__ void channels(float (&to)[DP / 32], const int4v *tile, int row, int lane) {
+    typedef float V __attribute__((ext_vector_type(DP / 32)));
+    const int col = DP / 32 * (lane % 32);
+    const float *const from = reinterpret_cast<const float *>(tile) + at(row, col / 4) * 4 + col % 4;
+    if constexpr (DP == 32) {
+      to[0] = *from;
+    } else {
+      const V v = *reinterpret_cast<const V *>(from);
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) to[b] = v[b];
+    }
   }
 };
 
 // out[channel][lane's row] += sum over 32 rows of the tile from row0 on of tile[row][channel] * w[row][lane's row]; w as an
-// accumulator holds it (register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32), rounded to T.
+// accumulator holds it (register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32), rounded to T.  Which channels the rows
+// of out[b] are is free: 32 b + {0 .. 31} with the transposing read; float takes DP / 32 neighbouring ones a lane in one read.
 template <typename T, int DP>
 __device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], const int4v *tile, int row0, const float16v &w, int lane) {
   using Rows = RowTile<T, DP>;
@@ -166,11 +177,12 @@ __device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], cons
     }
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int r = 0; r < 16; ++r) {
+      float rows[DP / 32];
+      Rows::channels(rows, tile, row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4, lane);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
-        out[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(Rows::element(tile, row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4, db * 32 + lane % 32),
-                                                       w[r], out[db], 0, 0, 0);
+      for (int db = 0; db < DP / 32; ++db) out[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(rows[db], w[r], out[db], 0, 0, 0);
+    }
   }
 }
 
@@ -195,19 +207,35 @@ __device__ __forceinline__ void load_row(int4v (&to)[DP / (32 / (int)sizeof(T))]
   }
 }
 
-// A lane's row of a result, from accumulators that hold it as columns, times `by`.
-template <typename To, int DP>
+// A lane's row of a result, from accumulators of T's products that hold it as columns, times `by`.
+template <typename T, typename To, int DP>
 __device__ __forceinline__ void store_row(To *row, const float16v (&acc)[DP / 32], float by, int dim, int lane) {
-  typedef To To4 __attribute__((ext_vector_type(4)));
+  if constexpr (sizeof(T) == 2) {
+    typedef To To4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int c = db * 32 + 8 * p + 4 * (lane / 32);
-      const float4v v = {acc[db][4 * p] * by, acc[db][4 * p + 1] * by, acc[db][4 * p + 2] * by, acc[db][4 * p + 3] * by};
-      if (c < dim) *reinterpret_cast<To4 *>(row + c) = __builtin_convertvector(v, To4);
-    }
+      for (int p = 0; p < 4; ++p) {
+        const int c = db * 32 + 8 * p + 4 * (lane / 32);
+        const float4v v = {acc[db][4 * p] * by, acc[db][4 * p + 1] * by, acc[db][4 * p + 2] * by, acc[db][4 * p + 3] * by};
+        if (c < dim) *reinterpret_cast<To4 *>(row + c) = __builtin_convertvector(v, To4);
+      }
+  } else {
+    // four rows of all blocks: 4 * DP / 32 neighbouring channels, of which dim, a multiple of 8, may end inside
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e) {
+        const int first = 4 * e, c = DP / 32 * (8 * p + 4 * (lane / 32)) + first;
+        float4v v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = acc[(first + i) % (DP / 32)][4 * p + (first + i) / (DP / 32)] * by;
+        if (c < dim) *reinterpret_cast<float4v *>(row + c) = v;
+      }
+  }
 }
+
+template <int N> struct Blocks { static constexpr int value = N; };
 
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -17,6 +17,9 @@ int refuse(const char *what, const char *why) {
   return FGMS_E_INVALID;
 }
 
+constexpr int64_t kMostRowBytes = 16 << 20;      // 128 rows of a tile below 2^31
+constexpr int64_t kMostRows = INT32_MAX - (1 << 18);
+
 bool aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // A strided [rows, heads, dim] tensor that the kernels read 16 bytes at a time (`there`: it has elements).
@@ -26,6 +29,8 @@ int check_rows(const char *what, const void *p, bool there, int64_t row, int64_t
   const int64_t bytes = element_bytes(dtype);
   if (!aligned(p) || row < 0 || head < 0 || row * bytes % 16 || head * bytes % 16)
     return refuse(what, "rows and heads have to begin on 16 bytes");
+  // (a tile's rows are reached by 32-bit offsets)
+  if (row * bytes > kMostRowBytes || head > kMostRowBytes) return refuse(what, "rows lie too far apart");
   return FGMS_OK;
 }
 
@@ -56,17 +61,23 @@ int check_norm_rotary(const char *what, const NormRotaryArgs &a) {
   return FGMS_OK;
 }
 
-int check_attention(const char *what, const AttentionArgs &a) {
+int check_attention(const char *what, const AttentionArgs &a, int64_t n_q, int64_t n_k) {
   int rc = check_shape(what, a.heads, a.kv_heads, a.dim, a.dtype);
   if (rc != FGMS_OK) return rc;
   if (a.kv_heads < 1 || a.heads % a.kv_heads) return refuse(what, "the query heads must be a multiple of the key heads");
-  if (a.n_q < 0 || a.n_k < 0 || a.n_q > INT32_MAX || a.n_k > INT32_MAX) return refuse(what, "between 0 and 2^31 - 1 rows");
-  if (a.segments < 0 || a.segments > INT32_MAX - 2) return refuse(what, "the number of segments is out of range");
-  if (a.segments > 0 && (!a.q_offsets || !a.k_offsets)) return refuse(what, "null offsets");
+  if (n_q < 0 || n_k < 0 || n_k > kMostRows || n_q > kMostRows / (a.heads / a.kv_heads))
+    return refuse(what, "the rows, times the heads of a group, must be fewer than 2^31 - 2^18");
+  if (a.segments < 0 || a.segments > kMostRows) return refuse(what, "the number of segments is out of range");
+  if (!a.q_offsets || !a.k_offsets) return refuse(what, "null offsets");
   if (!(a.scale > 0.f) || !(a.scale < 1e30f)) return refuse(what, "scale must be positive and finite");
-  if ((rc = check_rows(what, a.q, a.n_q > 0, a.q_row, a.q_head, a.dtype))) return rc;
-  if ((rc = check_rows(what, a.k, a.n_k > 0, a.k_row, a.k_head, a.dtype))) return rc;
-  return check_rows(what, a.v, a.n_k > 0, a.v_row, a.v_head, a.dtype);
+  if ((rc = check_rows(what, a.q, n_q > 0, a.q_row, a.q_head, a.dtype))) return rc;
+  if ((rc = check_rows(what, a.k, n_k > 0, a.k_row, a.k_head, a.dtype))) return rc;
+  if ((rc = check_rows(what, a.v, n_k > 0, a.v_row, a.v_head, a.dtype))) return rc;
+  // (a tile's rows end where the buffer over them does)
+  if ((n_k > 1 && (a.k_row < a.dim || a.v_row < a.dim))) return refuse(what, "rows of k and v overlap");
+  if ((int64_t)a.heads * (a.q_head > a.dim ? a.q_head : a.dim) * element_bytes(a.dtype) > (int64_t)512 << 20)
+    return refuse(what, "the heads of a row lie too far apart");
+  return FGMS_OK;
 }
 
 AttentionArgs attention_args(const void *q, const void *k, const void *v, const int32_t *q_offsets, const int32_t *k_offsets,
@@ -76,7 +87,7 @@ AttentionArgs attention_args(const void *q, const void *k, const void *v, const 
   AttentionArgs a{};
   a.q = q, a.k = k, a.v = v;
   a.q_offsets = q_offsets, a.k_offsets = k_offsets, a.k_lengths = k_lengths;
-  a.n_q = n_q, a.n_k = n_k, a.segments = segments, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
+  a.n_q = (int)n_q, a.n_k = (int)n_k, a.segments = segments, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
   a.causal = causal, a.scale = scale, a.dtype = dtype, a.stream = (hipStream_t)stream, a.parts = 1;
   return a;
@@ -150,7 +161,7 @@ extern "C" int fgms_segment_attention_fwd(const void *q, const void *k, const vo
   static const char what[] = "fgms_segment_attention_fwd";
   AttentionArgs a = attention_args(q, k, v, q_offsets, k_offsets, k_lengths, n_q, n_k, segments, heads, kv_heads, head_dim, q_row, q_head,
                                    k_row, k_head, v_row, v_head, causal, scale, dtype, stream);
-  const int rc = check_attention(what, a);
+  const int rc = check_attention(what, a, n_q, n_k);
   if (rc != FGMS_OK || n_q == 0) return rc;
   if (!out || !aligned(out)) return refuse(what, "the result has to begin on 16 bytes");
   a.out = out, a.lse = lse;
@@ -165,7 +176,7 @@ extern "C" int fgms_segment_attention_bwd(const void *out_grad, const void *q, c
   static const char what[] = "fgms_segment_attention_bwd";
   AttentionArgs a = attention_args(q, k, v, q_offsets, k_offsets, nullptr, n_q, n_k, segments, heads, kv_heads, head_dim, q_row, q_head,
                                    k_row, k_head, v_row, v_head, causal, scale, dtype, stream);
-  const int rc = check_attention(what, a);
+  const int rc = check_attention(what, a, n_q, n_k);
   if (rc != FGMS_OK) return rc;
   if (n_q > 0 && (!out_grad || !out || !lse)) return refuse(what, "null pointer");
   if (!aligned(out_grad) || !aligned(out) || !aligned(q_grad) || !aligned(k_grad) || !aligned(v_grad))

@@ -2,138 +2,210 @@
 #pragma once
 
 #include "fgms_attention.h"
+#include "fgms_device.h"
 
 namespace fgms {
 namespace {
 
-// Keys (queries in the keys' gradients) to a tile.
+// Keys (queries in the keys' gradients) to a tile: 16 KB each.
 template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) * DP > 256 ? 32 : 64; }
 
-// Rows [first, first + ROWS) of a strided tensor to LDS, zeros from row `end` on and behind the channels.
-template <typename T, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void stage_rows(int4v *tile, const T *base, int64_t stride, int64_t first, int64_t end, int dim) {
-  using Rows = RowTile<T, DP>;
-  constexpr int PER = ROWS * Rows::CH / THREADS;
-  int4v v[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = threadIdx.x + i * THREADS, row = e / Rows::CH, c = e % Rows::CH;
-    v[i] = first + row < end && c * Rows::E < dim ? *reinterpret_cast<const int4v *>(base + (first + row) * stride + c * Rows::E)
-                                                  : int4v{0, 0, 0, 0};
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = threadIdx.x + i * THREADS;
-    tile[Rows::at(e / Rows::CH, e % Rows::CH)] = v[i];
-  }
+// Waves to a SIMD that the registers are to leave room for.
+template <typename T, int DP> constexpr int waves_of_queries() { return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
+template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
+
+// 16 bytes a lane from a buffer to LDS, one lane's behind the other's from `to` on (the same for all lanes).
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *to, unsigned offset) {
+  typedef __attribute__((address_space(3))) void lds_any;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_any *)to, 16, offset, 0, 0, 0);
 }
 
-// Where a launch's workgroup stands.
-struct Place {
-  int64_t slot;
-  int kv_head, part;
+// Rows of a strided tensor on their way to a tile in LDS, past the registers: every lane asks for the chunk that belongs where
+// its 16 bytes land.  Chunks behind the channels, and rows behind the last, are out of the buffer's range and arrive as zeros.
+template <typename T, int DP, int ROWS, int NW>
+struct Stager {
+  using Rows = RowTile<T, DP>;
+  static constexpr int PER = ROWS * Rows::CH / (64 * NW);
+  const char *base;
+  int64_t stride;              // bytes
+  unsigned offset[PER];
+  __device__ __forceinline__ void open(const T *from, int64_t row_stride, int dim, int wave, int lane) {
+    base = (const char *)from;
+    stride = row_stride * (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (wave + i * NW) * 64 + lane, row = e / Rows::CH, c = (e % Rows::CH) ^ Rows::swizzle(row);
+      offset[i] = c * Rows::E < dim ? (unsigned)row * (unsigned)stride + c * 16 : kAbsentRow;
+    }
+  }
+  // rows [first, first + ROWS) of `count`
+  __device__ __forceinline__ void load(int4v *tile, int first, int count, int wave) const {
+    const int there = min(max(count - first, 0), ROWS);
+    const __amdgpu_buffer_rsrc_t rows = rows_resource(base + first * stride, (unsigned)there * (unsigned)stride);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      load_to_lds(rows, tile + (wave + i * NW) * 64, offset[i]);
+  }
 };
-__device__ __forceinline__ Place place_of(int64_t block, int kv_heads, int parts) {
+
+// Everything asked for has landed, for all waves.
+__device__ __forceinline__ void tiles_ready() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0)
+  __syncthreads();
+}
+
+// Where a launch's workgroup stands.  Long segments: head by head, so that the keys and values of few heads are in use at a time, and the
+// last tiles, which see most keys where the order is causal, first.  Short ones: the heads of a tile share lines of memory
+// (a row's heads lie side by side), so they and three neighbouring tiles go to one XCD (workgroup b runs on XCD b mod 8) one after the other;
+// launches too small for that take their tiles as they come.
+struct Place {
+  int slot, kv_head, part;
+};
+enum { kPlaceByHead = 1, kPlaceByXcd = 2 };
+constexpr int kPlaceTiles = 4;
+__device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int parts, int order, int slots) {
   Place p;
   p.part = (int)(block % parts);
-  p.kv_head = (int)(block / parts % kv_heads);
-  p.slot = block / parts / kv_heads;
+  block /= parts;
+  if (order == kPlaceByHead) {
+    p.kv_head = (int)(block / slots);
+    p.slot = slots - 1 - (int)(block % slots);
+  } else {
+    if (order == kPlaceByXcd) {
+      const unsigned per = kPlaceTiles * kv_heads, i = block / 8;
+      block = (i / per * 8 + block % 8) * per + i % per;
+    }
+    p.kv_head = (int)(block % kv_heads);
+    p.slot = (int)(block / kv_heads);
+  }
   return p;
 }
 
 // --- forward --------------------------------------------------------------------------------------------------
 // A wave holds 32 query rows as columns: scores come out of the matrix unit transposed (keys down the registers, a query a
 // lane and its partner 32 lanes on), so that a row's maximum and sum are taken inside two lanes, and the exponentials are
-// the right operand of the second product as they stand, with no exchange between lanes.
+// the right operand of the second product as they stand, with no exchange between lanes.  Tiles of keys and values pass through
+// two pairs of buffers: the next one is on its way while this one is worked on.
 template <typename T, int DP, int NW, bool PARTS>
-__global__ __launch_bounds__(NW * 64) void segment_attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_attention_kernel(const AttentionArgs a) {
   constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
-  __shared__ int4v k_tile[NK * RowTile<T, DP>::CH], v_tile[NK * RowTile<T, DP>::CH];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, group = a.heads / a.kv_heads;
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1);
+  using Rows = RowTile<T, DP>;
+  __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot);
   if (slot.first >= slot.length) return;
-  int64_t k_begin, k_count;
+  int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
-  const int64_t ahead = k_count - slot.length / group;      // the last query sees the last key
+  const int ahead = k_count - slot.length / group;      // the last query sees the last key
 
-  const int64_t row = slot.first + wave * 32 + lane % 32;
-  const bool mine = row < slot.length;
-  const int64_t token = row / group;
-  const int head = at.kv_head * group + (int)(row % group);
-  int4v q[STEPS];
-  load_row<T, DP>(q, mine ? (const T *)a.q + (slot.begin + token) * a.q_row + head * a.q_head : nullptr, a.dim, lane);
-
-  // keys this lane's row sees: those below `seen`; of a workgroup's rows the last sees most, of a wave's the first least
-  const int64_t seen = a.causal ? min(k_count, token + ahead + 1) : k_count;
-  const int64_t last_row = min(slot.first + T_ROWS, slot.length) - 1;
-  int64_t begin = 0, end = a.causal ? min(k_count, last_row / group + ahead + 1) : k_count;
-  const int64_t whole = a.causal ? min(k_count, (slot.first + wave * 32) / group + ahead + 1) : k_count;
+  // keys that the rows see: those below `seen` for this lane's, of the workgroup's rows the last sees most, of a wave's the first least
+  const int token0 = slot.first / group, head0 = slot.first - token0 * group;      // the tile's first row
+  const float per_group = 1.f / group;
+  const auto token_of = [&](int local) { return token0 + divide(head0 + local, per_group); };
+  const int local = wave * 32 + lane % 32, token = token_of(local), head = at.kv_head * group + head0 + local - (token - token0) * group;
+  const bool mine = slot.first + local < slot.length;
+  const bool awake = slot.first + wave * 32 < slot.length;
+  const int last = min(T_ROWS, slot.length - slot.first) - 1, wave_last = min(wave * 32 + 31, last);
+  int begin = 0, end = a.causal ? min(k_count, token_of(last) + ahead + 1) : k_count;
   if constexpr (PARTS) {
-    const int64_t piece = ((k_count + a.parts - 1) / a.parts + NK - 1) / NK * NK;
+    const int piece = ((k_count + a.parts - 1) / a.parts + NK - 1) / NK * NK;
     begin = at.part * piece;
     end = min(end, begin + piece);
   }
+  const int seen = a.causal ? min(k_count, token + ahead + 1) : k_count;
+  const int whole = min(end, a.causal ? token_of(wave * 32) + ahead + 1 : k_count);
+  const int wave_end = __builtin_amdgcn_readfirstlane(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
 
-  const T *const k = (const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head;
-  const T *const v = (const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head;
+  Stager<T, DP, NK, NW> k;
+  k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
+  Stager<T, DP, NK, NW> v;
+  v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
+  if (begin < end) {
+    k.load(k_tile0, begin, k_count, wave);
+    v.load(v_tile0, begin, k_count, wave);
+  }
+  int4v q[STEPS];
+  load_row<T, DP>(q, mine ? (const T *)a.q + (slot.begin + token) * a.q_row + head * a.q_head : nullptr, a.dim, lane);
+
   const float by = a.scale * kLog2e;
   const float inf = __builtin_inff();
-  float most = -inf, sum = 0.f;      // of the scores so far, times `by`; this lane's part of the sum
+  // of the scores so far, times `by`: a number that none exceeds by more than kSlack, -inf before the first (and what is subtracted from them)
+  constexpr float kSlack = 8.f;
+  float most = -inf, base = 0.f, sum = 0.f;
   float16v o[DP / 32] = {};
-  for (int64_t j = begin; j < end; j += NK) {
-    __syncthreads();
-    stage_rows<T, DP, NK, NW * 64>(k_tile, k, a.k_row, j, k_count, a.dim);
-    stage_rows<T, DP, NK, NW * 64>(v_tile, v, a.v_row, j, k_count, a.dim);
-    __syncthreads();
-    float16v s[NK / 32] = {};
+  // KB blocks of 32 keys
+  const auto take = [&](auto blocks, const int4v *k_tile, const int4v *v_tile, int j) __attribute__((always_inline)) {
+    constexpr int KB = decltype(blocks)::value;
+    float16v s[KB] = {};
 #pragma unroll
-    for (int kb = 0; kb < NK / 32; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) multiply<T>(s[kb], RowTile<T, DP>::rows(k_tile, kb * 32, i, lane), q[i]);
-    if (j + NK > whole) {
-      const int left = (int)max((int64_t)-1, min((int64_t)NK, seen - j));
+      for (int i = 0; i < STEPS; ++i)
+        if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s[kb], Rows::rows(k_tile, kb * 32, i, lane), q[i]);
+    if (j + KB * 32 > whole) {
+      const int left = seen - j;
 #pragma unroll
-      for (int kb = 0; kb < NK / 32; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (kb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 >= left) s[kb][r] = -inf;
     }
-    float top = -inf;
+    float top = s[0][0];
 #pragma unroll
-    for (int kb = 0; kb < NK / 32; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[kb][r]);
-    top = __builtin_fmaxf(most, both_max(top) * by);
-    const float from = top == -inf ? 0.f : top;      // (a row that has met no key yet)
-    const float keep = __builtin_amdgcn_exp2f(most - from);
-    most = top;
-    float add = 0.f;
+    top = both_max(top) * by;
+    // a new maximum is taken only where the old one is left behind by 2^8, which fp32 sums and 16-bit probabilities bear
+    if (__builtin_amdgcn_ballot_w64(top > most + kSlack)) {
+      const bool mine = top > most + kSlack;
+      const float keep = mine ? __builtin_amdgcn_exp2f(most - top) : 1.f;
+      most = mine ? top : most;
+      base = mine ? top : base;
+      sum *= keep;
 #pragma unroll
-    for (int kb = 0; kb < NK / 32; ++kb)
+      for (int db = 0; db < DP / 32; ++db) o[db] *= keep;
+    }
+    float add[2] = {0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], by, -from));
-        add += s[kb][r];
+        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], by, -base));
+        add[r % 2] += s[kb][r];
       }
-    sum = __builtin_fmaf(sum, keep, add);
+    sum += add[0] + add[1];
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) o[db] *= keep;
-#pragma unroll
-    for (int kb = 0; kb < NK / 32; ++kb) add_weighted_rows<T, DP>(o, v_tile, kb * 32, s[kb], lane);
+    for (int kb = 0; kb < KB; ++kb) add_weighted_rows<T, DP>(o, v_tile, kb * 32, s[kb], lane);
+  };
+  const auto step = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+    tiles_ready();
+    if (j + NK < end) {
+      k.load(k_next, j + NK, k_count, wave);
+      v.load(v_next, j + NK, k_count, wave);
+    }
+    if (NK == 64 && j + 32 < wave_end) take(Blocks<NK / 32>(), k_tile, v_tile, j);
+    else if (j < wave_end) take(Blocks<1>(), k_tile, v_tile, j);
+  };
+  for (int j = begin; j < end; j += 2 * NK) {
+    step(k_tile0, v_tile0, k_tile1, v_tile1, j);
+    if (j + NK >= end) break;
+    step(k_tile1, v_tile1, k_tile0, v_tile0, j + NK);
   }
 
   sum = both_sum(sum);
   const bool none = seen <= begin || end <= begin;      // no key for this row (here)
   const float inverse = none ? 0.f : 1.f / sum;
-  const float lse = none ? -inf : (most + __builtin_log2f(sum)) * (1.f / kLog2e);
+  const float lse = none ? -inf : (base + __builtin_log2f(sum)) * (1.f / kLog2e);
   if constexpr (PARTS) {
-    const int64_t tile = ((at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + wave * 32 + lane % 32;
-    if (mine && !none) store_row<float, DP>(a.part_sum + tile * a.dim, o, inverse, a.dim, lane);
+    const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
+    if (mine && !none) store_row<T, float, DP>(a.part_sum + tile * a.dim, o, inverse, a.dim, lane);
     if (mine && lane < 32) a.part_lse[tile] = lse;
   } else if (mine) {
-    const int64_t to = (slot.begin + token) * a.heads + head;
-    store_row<T, DP>((T *)a.out + to * a.dim, o, inverse, a.dim, lane);
+    const int64_t to = (int64_t)(slot.begin + token) * a.heads + head;
+    store_row<T, T, DP>((T *)a.out + to * a.dim, o, inverse, a.dim, lane);
     if (a.lse && lane < 32) a.lse[to] = lse;
   }
 }
@@ -142,19 +214,18 @@ __global__ __launch_bounds__(NW * 64) void segment_attention_kernel(const Attent
 // A thread four channels of a row; SUMS: the parts add up (gradients, times `by`), else they are averages over their keys, to be
 // weighted by their sums of exponentials.
 template <typename T, int NW, bool SUMS>
-__global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, const int32_t *__restrict__ offsets, int64_t n, int group,
+__global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, const int32_t *__restrict__ offsets, int n, int group,
                                                          const float *__restrict__ sums, T *__restrict__ out, float by) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   constexpr int T_ROWS = 32 * NW;
   const int per_row = a.dim / 4;
-  const Place at = place_of(blockIdx.x, a.kv_heads, 1);
+  const Place at = place_of(blockIdx.x, a.kv_heads, 1, 0, 0);
   const Slot slot = find_slot(offsets, a.segments, n, group, T_ROWS, at.slot);
-  const int64_t first = (at.slot * a.kv_heads + at.kv_head) * a.parts * T_ROWS;
+  const int64_t first = ((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts * T_ROWS;
   for (int e = threadIdx.x; e < T_ROWS * per_row; e += 256) {
-    const int local = e / per_row, c = e % per_row * 4;
-    const int64_t row = slot.first + local;
+    const int local = e / per_row, c = e % per_row * 4, row = slot.first + local;
     if (row >= slot.length) break;
-    const int64_t to = ((slot.begin + row / group) * a.kv_heads + at.kv_head) * group + row % group;
+    const int64_t to = ((int64_t)(slot.begin + row / group) * a.kv_heads + at.kv_head) * group + row % group;
     float4v total = {0.f, 0.f, 0.f, 0.f};
     if constexpr (SUMS) {
       for (int p = 0; p < a.parts; ++p) total += *reinterpret_cast<const float4v *>(sums + (first + (int64_t)p * T_ROWS + local) * a.dim + c);
@@ -179,7 +250,6 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, 
     *reinterpret_cast<T4 *>(out + to * a.dim + c) = __builtin_convertvector(total, T4);
   }
 }
-
 
 // --- backward -------------------------------------------------------------------------------------------------
 // ds = p (g_out . v - delta) is rounded to T for its two products, p for its one.  In fp16 a power of two goes with them, taken out
@@ -210,22 +280,45 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T *__restric
 // Queries' gradients.  As the forward kernel: a wave's 32 query rows are columns, so that a row's log-sum and delta are one value a lane,
 // and ds the right operand of dq^T = k^T ds as it stands.
 template <typename T, int DP, int NW, bool PARTS>
-__global__ __launch_bounds__(NW * 64) void attention_query_grad_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attention_query_grad_kernel(const AttentionArgs a) {
   constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
-  __shared__ int4v k_tile[NK * RowTile<T, DP>::CH], v_tile[NK * RowTile<T, DP>::CH];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, group = a.heads / a.kv_heads;
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1);
+  using Rows = RowTile<T, DP>;
+  __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot);
   if (slot.first >= slot.length) return;
-  int64_t k_begin, k_count;
+  int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
-  const int64_t ahead = k_count - slot.length / group;
+  const int ahead = k_count - slot.length / group;
 
-  const int64_t row = slot.first + wave * 32 + lane % 32;
-  const bool mine = row < slot.length;
-  const int64_t token = row / group;
-  const int head = at.kv_head * group + (int)(row % group);
-  const int64_t to = (slot.begin + token) * a.heads + head;
+  const int token0 = slot.first / group, head0 = slot.first - token0 * group;
+  const float per_group = 1.f / group;
+  const auto token_of = [&](int local) { return token0 + divide(head0 + local, per_group); };
+  const int local = wave * 32 + lane % 32, token = token_of(local), head = at.kv_head * group + head0 + local - (token - token0) * group;
+  const bool mine = slot.first + local < slot.length;
+  const bool awake = slot.first + wave * 32 < slot.length;
+  const int last = min(T_ROWS, slot.length - slot.first) - 1, wave_last = min(wave * 32 + 31, last);
+  int begin = 0, end = a.causal ? min(k_count, token_of(last) + ahead + 1) : k_count;
+  if constexpr (PARTS) {
+    const int piece = ((k_count + a.parts - 1) / a.parts + NK - 1) / NK * NK;
+    begin = at.part * piece;
+    end = min(end, begin + piece);
+  }
+  const int seen = a.causal ? min(k_count, token + ahead + 1) : k_count;
+  const int whole = min(end, a.causal ? token_of(wave * 32) + ahead + 1 : k_count);
+  const int wave_end = __builtin_amdgcn_readfirstlane(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
+
+  Stager<T, DP, NK, NW> k;
+  k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
+  Stager<T, DP, NK, NW> v;
+  v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
+  if (begin < end) {
+    k.load(k_tile0, begin, k_count, wave);
+    v.load(v_tile0, begin, k_count, wave);
+  }
+  const int64_t to = (int64_t)(slot.begin + token) * a.heads + head;
   int4v q[STEPS], g[STEPS];
   load_row<T, DP>(q, mine ? (const T *)a.q + (slot.begin + token) * a.q_row + head * a.q_head : nullptr, a.dim, lane);
   load_row<T, DP>(g, mine ? (const T *)a.g_out + to * a.dim : nullptr, a.dim, lane);
@@ -234,141 +327,183 @@ __global__ __launch_bounds__(NW * 64) void attention_query_grad_kernel(const Att
   lse = lse == -inf ? inf : lse * kLog2e - ds_shift<T>();      // (no keys: all probabilities 0)
   const float delta = mine ? a.delta[to] : 0.f;
 
-  const int64_t seen = a.causal ? min(k_count, token + ahead + 1) : k_count;
-  const int64_t last_row = min(slot.first + T_ROWS, slot.length) - 1;
-  int64_t begin = 0, end = a.causal ? min(k_count, last_row / group + ahead + 1) : k_count;
-  const int64_t whole = a.causal ? min(k_count, (slot.first + wave * 32) / group + ahead + 1) : k_count;
-  if constexpr (PARTS) {
-    const int64_t piece = ((k_count + a.parts - 1) / a.parts + NK - 1) / NK * NK;
-    begin = at.part * piece;
-    end = min(end, begin + piece);
-  }
-  const T *const k = (const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head;
-  const T *const v = (const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head;
   const float by = a.scale * kLog2e;
   float16v dq[DP / 32] = {};
-  for (int64_t j = begin; j < end; j += NK) {
-    __syncthreads();
-    stage_rows<T, DP, NK, NW * 64>(k_tile, k, a.k_row, j, k_count, a.dim);
-    stage_rows<T, DP, NK, NW * 64>(v_tile, v, a.v_row, j, k_count, a.dim);
-    __syncthreads();
-    const int left = j + NK > whole ? (int)max((int64_t)-1, min((int64_t)NK, seen - j)) : NK;
+  const auto take = [&](const int4v *k_tile, const int4v *v_tile, int kb, int j) __attribute__((always_inline)) {
+    float16v s = {}, dp = {};
 #pragma unroll
-    for (int kb = 0; kb < NK / 32; ++kb) {
-      float16v s = {}, dp = {};
+    for (int i = 0; i < STEPS; ++i)
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s, Rows::rows(k_tile, kb * 32, i, lane), q[i]);
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) multiply<T>(s, RowTile<T, DP>::rows(k_tile, kb * 32, i, lane), q[i]);
+    for (int i = 0; i < STEPS; ++i)
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(dp, Rows::rows(v_tile, kb * 32, i, lane), g[i]);
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) multiply<T>(dp, RowTile<T, DP>::rows(v_tile, kb * 32, i, lane), g[i]);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], by, -lse)) * (dp[r] - delta);
+    if (j + kb * 32 + 32 > whole) {
+      const int left = seen - j;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], by, -lse)) * (dp[r] - delta);
-        s[r] = kb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 < left ? ds : 0.f;
-      }
-      add_weighted_rows<T, DP>(dq, k_tile, kb * 32, s, lane);
+      for (int r = 0; r < 16; ++r)
+        if (kb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 >= left) s[r] = 0.f;
     }
+    add_weighted_rows<T, DP>(dq, k_tile, kb * 32, s, lane);
+  };
+  const auto step = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+    tiles_ready();
+    if (j + NK < end) {
+      k.load(k_next, j + NK, k_count, wave);
+      v.load(v_next, j + NK, k_count, wave);
+    }
+#pragma unroll
+    for (int kb = 0; kb < NK / 32; ++kb)
+      if (j + kb * 32 < wave_end) take(k_tile, v_tile, kb, j);
+  };
+  for (int j = begin; j < end; j += 2 * NK) {
+    step(k_tile0, v_tile0, k_tile1, v_tile1, j);
+    if (j + NK >= end) break;
+    step(k_tile1, v_tile1, k_tile0, v_tile0, j + NK);
   }
   const float scale = a.scale * pow2(-ds_shift<T>());
   if constexpr (PARTS) {
-    const int64_t tile = ((at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + wave * 32 + lane % 32;
-    if (mine) store_row<float, DP>(a.part_sum + tile * a.dim, dq, scale, a.dim, lane);
+    const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
+    if (mine) store_row<T, float, DP>(a.part_sum + tile * a.dim, dq, scale, a.dim, lane);
   } else if (mine) {
-    store_row<T, DP>((T *)a.gq + to * a.dim, dq, scale, a.dim, lane);
+    store_row<T, T, DP>((T *)a.gq + to * a.dim, dq, scale, a.dim, lane);
   }
 }
 
 // Keys' and values' gradients: a wave's 32 keys are columns, the queries of all heads of the group pass by as rows, and
 // dk^T = q^T ds, dv^T = g_out^T p take ds and p as they stand.
 template <typename T, int DP, int NW, bool PARTS>
-__global__ __launch_bounds__(NW * 64) void attention_key_grad_kernel(const AttentionArgs a) {
-  constexpr int NQ = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW, THREADS = NW * 64;
+__global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_key_grad_kernel(const AttentionArgs a) {
+  constexpr int NQ = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
-  __shared__ int4v q_tile[NQ * Rows::CH], g_tile[NQ * Rows::CH];
-  __shared__ float4v lse_tile[NQ / 4], delta_tile[NQ / 4];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, group = a.heads / a.kv_heads;
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1);
+  constexpr int PER = NQ * Rows::CH / (64 * NW);
+  __shared__ int4v q_tile0[NQ * Rows::CH], g_tile0[NQ * Rows::CH], q_tile1[NQ * Rows::CH], g_tile1[NQ * Rows::CH];
+  __shared__ float4v lse_tile0[NQ / 4], delta_tile0[NQ / 4], lse_tile1[NQ / 4], delta_tile1[NQ / 4];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.k_offsets, a.segments, a.n_k, 1, T_ROWS, at.slot);
   if (slot.first >= slot.length) return;
-  int64_t q_begin, q_count;
+  int q_begin, q_count;
   partner_rows(a.q_offsets, nullptr, slot.segment, a.segments, a.n_q, q_begin, q_count);
-  const int64_t ahead = slot.length - q_count, rows = q_count * group;
+  const int ahead = slot.length - q_count, rows = q_count * group;
 
-  const int64_t key = slot.first + wave * 32 + lane % 32;
+  const int local = wave * 32 + lane % 32, key = slot.first + local;
   const bool mine = key < slot.length;
-  int4v k[STEPS], v[STEPS];
-  load_row<T, DP>(k, mine ? (const T *)a.k + (slot.begin + key) * a.k_row + at.kv_head * a.k_head : nullptr, a.dim, lane);
-  load_row<T, DP>(v, mine ? (const T *)a.v + (slot.begin + key) * a.v_row + at.kv_head * a.v_head : nullptr, a.dim, lane);
+  const bool awake = slot.first + wave * 32 < slot.length;
 
-  // rows from which on this lane's key is seen, the workgroup's first key (first of all), the wave's last
-  int64_t begin = 0, end = rows;
-  const int64_t from = a.causal ? max((int64_t)0, key - ahead) * group : 0;
-  const int64_t whole = a.causal ? max((int64_t)0, slot.first + wave * 32 + 31 - ahead) * group : 0;
+  // rows from which on this lane's key is seen, the workgroup's first key (first of all), the wave's first and last
+  int begin = 0, end = rows;
+  const int from = a.causal ? max(0, key - ahead) * group : 0;
+  const int wave_from = awake ? a.causal ? max(0, slot.first + wave * 32 - ahead) * group : 0 : rows;
+  const int whole = a.causal ? max(0, slot.first + wave * 32 + 31 - ahead) * group : 0;
   if constexpr (PARTS) {
-    const int64_t piece = ((rows + a.parts - 1) / a.parts + NQ - 1) / NQ * NQ;
+    const int piece = ((rows + a.parts - 1) / a.parts + NQ - 1) / NQ * NQ;
     begin = at.part * piece;
     end = min(end, begin + piece);
   }
-  if (a.causal) {
-    const int64_t first = max((int64_t)0, slot.first - ahead) * group / NQ * NQ;
-    begin = max(begin, first);
+  if (a.causal) begin = max(begin, max(0, slot.first - ahead) * group / NQ * NQ);
+
+  // Rows on their way to LDS: row r is head r % group of token r / group, whose place in the tensors is found anew for every tile.
+  const int64_t q_row = a.q_row * (int)sizeof(T), q_head = a.q_head * (int)sizeof(T), g_row = (int64_t)a.heads * a.dim * (int)sizeof(T);
+  const char *const q_base = (const char *)a.q + q_begin * q_row + at.kv_head * group * q_head;
+  const char *const g_base = (const char *)a.g_out + q_begin * g_row + (int64_t)at.kv_head * group * a.dim * (int)sizeof(T);
+  const float *const lse_base = a.lse + (int64_t)q_begin * a.heads + at.kv_head * group;
+  const float *const delta_base = a.delta + (int64_t)q_begin * a.heads + at.kv_head * group;
+  const float per_group = 1.f / group, inf = __builtin_inff();
+  float next_lse, next_delta;
+  const auto load = [&](int4v *q_tile, int4v *g_tile, int first) __attribute__((always_inline)) {
+    const int token0 = first / group, head0 = first - token0 * group;
+    const __amdgpu_buffer_rsrc_t qs = rows_resource(q_base + token0 * q_row, kMaxBufferBytes), gs = rows_resource(g_base + token0 * g_row, kMaxBufferBytes);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = (wave + i * NW) * 64 + lane, row = e / Rows::CH, c = (e % Rows::CH) ^ Rows::swizzle(row);
+      const int token = divide(head0 + row, per_group), head = head0 + row - token * group;
+      const bool there = first + row < rows && c * Rows::E < a.dim;
+      load_to_lds(qs, q_tile + (wave + i * NW) * 64,
+                  there ? (unsigned)token * (unsigned)q_row + (unsigned)head * (unsigned)q_head + c * 16 : kAbsentRow);
+      load_to_lds(gs, g_tile + (wave + i * NW) * 64,
+                  there ? (unsigned)token * (unsigned)g_row + (unsigned)(head * a.dim * (int)sizeof(T)) + c * 16 : kAbsentRow);
+    }
+    if (wave == 0 && lane < NQ) {
+      const int token = divide(head0 + lane, per_group), head = head0 + lane - token * group;
+      const bool there = first + lane < rows;
+      const int64_t to = there ? (int64_t)(token0 + token) * a.heads + head : 0;
+      next_lse = lse_base[to], next_delta = delta_base[to];
+      next_lse = there ? next_lse : -inf;      // (no such row: all probabilities 0)
+      next_delta = there ? next_delta : 0.f;
+    }
+  };
+  const auto keep = [&](float4v *lse_tile, float4v *delta_tile) __attribute__((always_inline)) {
+    if (wave == 0 && lane < NQ) {
+      reinterpret_cast<float *>(lse_tile)[lane] = next_lse == -inf ? inf : next_lse * kLog2e - p_shift<T>();
+      reinterpret_cast<float *>(delta_tile)[lane] = next_delta;
+    }
+  };
+  if (begin < end) {
+    load(q_tile0, g_tile0, begin);
+    keep(lse_tile0, delta_tile0);
   }
-  const float by = a.scale * kLog2e, inf = __builtin_inff();
+  int4v k[STEPS], v[STEPS];
+  load_row<T, DP>(k, mine ? (const T *)a.k + (slot.begin + key) * a.k_row + at.kv_head * a.k_head : nullptr, a.dim, lane);
+  load_row<T, DP>(v, mine ? (const T *)a.v + (slot.begin + key) * a.v_row + at.kv_head * a.v_head : nullptr, a.dim, lane);
+  const float by = a.scale * kLog2e;
   float16v dk[DP / 32] = {}, dv[DP / 32] = {};
-  for (int64_t r0 = begin; r0 < end; r0 += NQ) {
-    __syncthreads();
+  const auto take = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
+                        int r0) __attribute__((always_inline)) {
+    float16v p = {}, ds = {};
 #pragma unroll
-    for (int i = 0; i < NQ * Rows::CH / THREADS; ++i) {
-      const int e = threadIdx.x + i * THREADS, c = e % Rows::CH;
-      const int64_t row = r0 + e / Rows::CH, token = q_begin + row / group;
-      const int head = at.kv_head * group + (int)(row % group);
-      int4v x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-      if (row < rows && c * Rows::E < a.dim) {
-        x = *reinterpret_cast<const int4v *>((const T *)a.q + token * a.q_row + head * a.q_head + c * Rows::E);
-        y = *reinterpret_cast<const int4v *>((const T *)a.g_out + (token * a.heads + head) * a.dim + c * Rows::E);
+    for (int i = 0; i < STEPS; ++i)
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(p, Rows::rows(q_tile, qb * 32, i, lane), k[i]);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(ds, Rows::rows(g_tile, qb * 32, i, lane), v[i]);
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const float4v lse = lse_tile[qb * 8 + 2 * r4 + lane / 32], delta = delta_tile[qb * 8 + 2 * r4 + lane / 32];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * r4 + e;
+        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], by, -lse[e]));
+        ds[r] = p[r] * ((ds[r] - delta[e]) * pow2(ds_shift<T>() - p_shift<T>()));
       }
-      q_tile[Rows::at(e / Rows::CH, c)] = x;
-      g_tile[Rows::at(e / Rows::CH, c)] = y;
     }
-    for (int e = threadIdx.x; e < NQ; e += THREADS) {
-      const int64_t row = r0 + e, to = (q_begin + row / group) * a.heads + at.kv_head * group + row % group;
-      const float lse = row < rows ? a.lse[to] : -inf;      // (no keys, no such row: all probabilities 0)
-      reinterpret_cast<float *>(lse_tile)[e] = lse == -inf ? inf : lse * kLog2e - p_shift<T>();
-      reinterpret_cast<float *>(delta_tile)[e] = row < rows ? a.delta[to] : 0.f;
+    if (r0 + qb * 32 < whole) {
+      const int hidden = from - r0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (qb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 < hidden) p[r] = ds[r] = 0.f;
     }
-    __syncthreads();
-    const int hidden = r0 < whole ? (int)min((int64_t)NQ, max((int64_t)0, from - r0)) : 0;
+    add_weighted_rows<T, DP>(dv, g_tile, qb * 32, p, lane);
+    add_weighted_rows<T, DP>(dk, q_tile, qb * 32, ds, lane);
+  };
+  const auto step = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
+                        float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
+    tiles_ready();
+    const bool more = r0 + NQ < end;
+    if (more) load(q_next, g_next, r0 + NQ);
 #pragma unroll
-    for (int qb = 0; qb < NQ / 32; ++qb) {
-      float16v p = {}, ds = {};
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) multiply<T>(p, Rows::rows(q_tile, qb * 32, i, lane), k[i]);
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) multiply<T>(ds, Rows::rows(g_tile, qb * 32, i, lane), v[i]);
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const float4v lse = lse_tile[qb * 8 + 2 * r4 + lane / 32], delta = delta_tile[qb * 8 + 2 * r4 + lane / 32];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * r4 + e;
-          p[r] = qb * 32 + 8 * r4 + 4 * (lane / 32) + e < hidden ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], by, -lse[e]));
-          ds[r] = qb * 32 + 8 * r4 + 4 * (lane / 32) + e < hidden ? 0.f : p[r] * ((ds[r] - delta[e]) * pow2(ds_shift<T>() - p_shift<T>()));
-        }
-      }
-      add_weighted_rows<T, DP>(dv, g_tile, qb * 32, p, lane);
-      add_weighted_rows<T, DP>(dk, q_tile, qb * 32, ds, lane);
-    }
+    for (int qb = 0; qb < NQ / 32; ++qb)
+      if (r0 + qb * 32 + 31 >= wave_from && r0 + qb * 32 < end) take(q_tile, g_tile, lse_tile, delta_tile, qb, r0);
+    if (more) keep(lse_next, delta_next);
+  };
+  for (int r0 = begin; r0 < end; r0 += 2 * NQ) {
+    step(q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
+    if (r0 + NQ >= end) break;
+    step(q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0 + NQ);
   }
   const float k_by = a.scale * pow2(-ds_shift<T>()), v_by = pow2(-p_shift<T>());
   if (!mine) return;
   if constexpr (PARTS) {
-    const int64_t tile = ((at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + wave * 32 + lane % 32;
-    const int64_t all = attention_slots(a.n_k, a.segments, T_ROWS) * a.kv_heads * a.parts * T_ROWS * a.dim;
-    store_row<float, DP>(a.part_sum + tile * a.dim, dk, k_by, a.dim, lane);
-    store_row<float, DP>(a.part_sum + all + tile * a.dim, dv, v_by, a.dim, lane);
+    const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
+    const int64_t all = (int64_t)a.slots * a.kv_heads * a.parts * T_ROWS * a.dim;
+    store_row<T, float, DP>(a.part_sum + tile * a.dim, dk, k_by, a.dim, lane);
+    store_row<T, float, DP>(a.part_sum + all + tile * a.dim, dv, v_by, a.dim, lane);
   } else {
-    const int64_t to = ((slot.begin + key) * a.kv_heads + at.kv_head) * a.dim;
-    if (a.gk) store_row<T, DP>((T *)a.gk + to, dk, k_by, a.dim, lane);
-    if (a.gv) store_row<T, DP>((T *)a.gv + to, dv, v_by, a.dim, lane);
+    const int64_t to = ((int64_t)(slot.begin + key) * a.kv_heads + at.kv_head) * a.dim;
+    if (a.gk) store_row<T, T, DP>((T *)a.gk + to, dk, k_by, a.dim, lane);
+    if (a.gv) store_row<T, T, DP>((T *)a.gv + to, dv, v_by, a.dim, lane);
   }
 }
 
@@ -400,13 +535,27 @@ inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments) {
   return parts < 2 ? 1 : parts > 1024 ? 1024 : (int)parts;
 }
 
+// Workgroups of a launch over tiles of `rows` rows: slots and order go into `a`.
+inline int plan_grid(AttentionArgs &a, int64_t rows, int tile, int64_t partners, unsigned *grid, int64_t *tiles) {
+  const int64_t slots = attention_slots(rows, a.segments, tile), segments = a.segments > 0 ? a.segments : 1;
+  a.parts = parts_for((rows / tile + a.segments) * a.kv_heads, partners, a.segments);
+  // (long: the partners of one segment and all heads are more than half of an XCD's L2)
+  const int64_t element = a.dtype == FGMS_F32 ? 4 : 2;
+  a.order = a.parts > 1 ? 0 : partners / segments * 2 * a.kv_heads * a.dim * element > (2 << 20) ? kPlaceByHead
+            : slots * a.kv_heads >= 64 * kPlaceTiles * a.kv_heads ? kPlaceByXcd : 0;
+  *tiles = slots * a.kv_heads;
+  const int64_t per = (int64_t)kPlaceTiles * a.kv_heads * 8;
+  const int rc = grid_of((a.order == kPlaceByXcd ? (*tiles + per - 1) / per * per : *tiles) * a.parts, grid);
+  a.slots = (int)slots;
+  return rc;
+}
+
 template <typename T, int DP, int NW>
 int forward(AttentionArgs a) {
   const int group = a.heads / a.kv_heads;
-  const int64_t tiles = attention_slots(a.n_q * group, a.segments, 32 * NW) * a.kv_heads;
-  a.parts = parts_for((a.n_q * group / (32 * NW) + a.segments) * a.kv_heads, a.n_k, a.segments);
   unsigned grid;
-  int rc = grid_of(tiles * a.parts, &grid);
+  int64_t tiles;
+  int rc = plan_grid(a, (int64_t)a.n_q * group, 32 * NW, a.n_k, &grid, &tiles);
   if (rc != FGMS_OK) return rc;
   if (a.parts == 1) {
     segment_attention_kernel<T, DP, NW, false><<<grid, NW * 64, 0, a.stream>>>(a);
@@ -424,10 +573,9 @@ int forward(AttentionArgs a) {
 template <typename T, int DP, int NW>
 int query_grad(AttentionArgs a) {
   const int group = a.heads / a.kv_heads;
-  const int64_t tiles = attention_slots(a.n_q * group, a.segments, 32 * NW) * a.kv_heads;
-  a.parts = parts_for((a.n_q * group / (32 * NW) + a.segments) * a.kv_heads, a.n_k, a.segments);
   unsigned grid;
-  int rc = grid_of(tiles * a.parts, &grid);
+  int64_t tiles;
+  int rc = plan_grid(a, (int64_t)a.n_q * group, 32 * NW, a.n_k, &grid, &tiles);
   if (rc != FGMS_OK) return rc;
   if (a.parts == 1) {
     attention_query_grad_kernel<T, DP, NW, false><<<grid, NW * 64, 0, a.stream>>>(a);
@@ -442,10 +590,9 @@ int query_grad(AttentionArgs a) {
 
 template <typename T, int DP, int NW>
 int key_grad(AttentionArgs a) {
-  const int64_t tiles = attention_slots(a.n_k, a.segments, 32 * NW) * a.kv_heads;
-  a.parts = parts_for((a.n_k / (32 * NW) + a.segments) * a.kv_heads, a.n_q * (a.heads / a.kv_heads), a.segments);
   unsigned grid;
-  int rc = grid_of(tiles * a.parts, &grid);
+  int64_t tiles;
+  int rc = plan_grid(a, a.n_k, 32 * NW, (int64_t)a.n_q * (a.heads / a.kv_heads), &grid, &tiles);
   if (rc != FGMS_OK) return rc;
   if (a.parts == 1) {
     attention_key_grad_kernel<T, DP, NW, false><<<grid, NW * 64, 0, a.stream>>>(a);
@@ -462,12 +609,12 @@ int key_grad(AttentionArgs a) {
 
 template <typename T, int DP>
 int forward_any(const AttentionArgs &a) {
-  return waves_for(a.n_q * (a.heads / a.kv_heads), a.segments) == 4 ? forward<T, DP, 4>(a) : forward<T, DP, 1>(a);
+  return waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments) == 4 ? forward<T, DP, 4>(a) : forward<T, DP, 1>(a);
 }
 
 template <typename T, int DP>
 int backward_any(const AttentionArgs &a) {
-  const int64_t rows = a.n_q * a.heads;
+  const int64_t rows = (int64_t)a.n_q * a.heads;
   unsigned grid;
   int rc = grid_of((rows + 31) / 32, &grid);
   if (rc == FGMS_OK && rows > 0) {
@@ -475,7 +622,7 @@ int backward_any(const AttentionArgs &a) {
     rc = launched("segment attention, backward");
   }
   if (rc == FGMS_OK && a.gq && a.n_q > 0)
-    rc = waves_for(a.n_q * (a.heads / a.kv_heads), a.segments) == 4 ? query_grad<T, DP, 4>(a) : query_grad<T, DP, 1>(a);
+    rc = waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments) == 4 ? query_grad<T, DP, 4>(a) : query_grad<T, DP, 1>(a);
   if (rc == FGMS_OK && (a.gk || a.gv) && a.n_k > 0)
     rc = waves_for(a.n_k, a.segments) == 4 ? key_grad<T, DP, 4>(a) : key_grad<T, DP, 1>(a);
   return rc;
