@@ -7,8 +7,8 @@
 namespace fgms {
 namespace {
 
-// Keys (queries in the keys' gradients) to a tile: 16 KB each.
-template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) * DP > 256 ? 32 : 64; }
+// Keys (queries in the keys' gradients) to a tile.
+template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) == 4 ? 32 : 64; }
 
 // Waves to a SIMD that the registers are to leave room for.
 template <typename T, int DP> constexpr int waves_of_queries() { return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
@@ -211,43 +211,68 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
 }
 
 // --- joining the parts -----------------------------------------------------------------------------------------
-// A thread four channels of a row; SUMS: the parts add up (gradients, times `by`), else they are averages over their keys, to be
-// weighted by their sums of exponentials.
+// SUMS: the parts add up (gradients); else they are averages over their keys, to be weighted by their sums of exponentials.  A workgroup
+// has eight rows of a tile: the parts' weights first, then a thread four channels of a row, eight parts under way at a time.
+constexpr int kMostParts = 256, kJoinRows = 8;
 template <typename T, int NW, bool SUMS>
 __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, const int32_t *__restrict__ offsets, int n, int group,
-                                                         const float *__restrict__ sums, T *__restrict__ out, float by) {
+                                                         const float *__restrict__ sums, T *__restrict__ out) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   constexpr int T_ROWS = 32 * NW;
+  __shared__ float weight[kJoinRows][kMostParts];
   const int per_row = a.dim / 4;
-  const Place at = place_of(blockIdx.x, a.kv_heads, 1, 0, 0);
+  const Place at = place_of(blockIdx.x, a.kv_heads, T_ROWS / kJoinRows, 0, 0);      // (eight rows: a part of the tile)
   const Slot slot = find_slot(offsets, a.segments, n, group, T_ROWS, at.slot);
-  const int64_t first = ((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts * T_ROWS;
-  for (int e = threadIdx.x; e < T_ROWS * per_row; e += 256) {
-    const int local = e / per_row, c = e % per_row * 4, row = slot.first + local;
-    if (row >= slot.length) break;
-    const int64_t to = ((int64_t)(slot.begin + row / group) * a.kv_heads + at.kv_head) * group + row % group;
-    float4v total = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (SUMS) {
-      for (int p = 0; p < a.parts; ++p) total += *reinterpret_cast<const float4v *>(sums + (first + (int64_t)p * T_ROWS + local) * a.dim + c);
-      total *= by;
-    } else {
-      const float *const lse = a.part_lse + first + local;
-      float most = -__builtin_inff();
-      for (int p = 0; p < a.parts; ++p) most = __builtin_fmaxf(most, lse[(int64_t)p * T_ROWS]);
-      float weight = 0.f;
-      bool any = false;
-      for (int p = 0; p < a.parts; ++p) {
-        const float l = lse[(int64_t)p * T_ROWS];
-        if (l == -__builtin_inff()) continue;      // (no keys there, and nothing written)
-        any = true;
-        const float w = __builtin_amdgcn_exp2f((l - most) * kLog2e);
-        weight += w;
-        total += w * *reinterpret_cast<const float4v *>(sums + (first + (int64_t)p * T_ROWS + local) * a.dim + c);
+  const int row0 = at.part * kJoinRows, rows = min(kJoinRows, slot.length - slot.first - row0);
+  if (rows <= 0) return;
+  const int64_t first = ((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts * T_ROWS + row0;
+  const auto place = [&](int local) {
+    const int row = slot.first + row0 + local;
+    return ((int64_t)(slot.begin + row / group) * a.kv_heads + at.kv_head) * group + row % group;
+  };
+  if constexpr (!SUMS) {
+    // 32 threads a row
+    const int local = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const float inf = __builtin_inff();
+    float most = -inf, total = 0.f;
+    if (local < rows)
+      for (int p = lane; p < a.parts; p += 32) {
+        const float lse = a.part_lse[first + (int64_t)p * T_ROWS + local];
+        weight[local][p] = lse;
+        most = __builtin_fmaxf(most, lse);
       }
-      if (any) total /= weight;
-      if (a.lse && c == 0) a.lse[to] = any ? most + __builtin_log2f(weight) * (1.f / kLog2e) : -__builtin_inff();
+    for (int d = 1; d < 32; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+    if (local < rows)
+      for (int p = lane; p < a.parts; p += 32) {
+        // (a part without keys has nothing written)
+        const float w = weight[local][p] == -inf ? 0.f : __builtin_amdgcn_exp2f((weight[local][p] - most) * kLog2e);
+        weight[local][p] = w;
+        total += w;
+      }
+    for (int d = 1; d < 32; d *= 2) total += __shfl_xor(total, d);
+    const bool any = most != -inf || total != 0.f;      // (not a number: kept)
+    if (local < rows) {
+      for (int p = lane; p < a.parts; p += 32) weight[local][p] = any ? weight[local][p] / total : 0.f;
+      if (a.lse && lane == 0) a.lse[place(local)] = any ? most + __builtin_log2f(total) * (1.f / kLog2e) : -inf;
     }
-    *reinterpret_cast<T4 *>(out + to * a.dim + c) = __builtin_convertvector(total, T4);
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < rows * per_row; e += 256) {
+    const int local = e / per_row, c = e % per_row * 4;
+    const float *const from = sums + (first + local) * a.dim + c;
+    const int64_t step = (int64_t)T_ROWS * a.dim;
+    float4v total = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < a.parts; p0 += 8) {
+      float4v v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool there = p0 + i < a.parts && (SUMS || weight[local][p0 + i] != 0.f);
+        v[i] = there ? *reinterpret_cast<const float4v *>(from + (p0 + i) * step) : float4v{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) total += SUMS ? v[i] : v[i] * (p0 + i < a.parts ? weight[local][p0 + i] : 0.f);
+    }
+    *reinterpret_cast<T4 *>(out + place(local) * a.dim + c) = __builtin_convertvector(total, T4);
   }
 }
 
@@ -528,11 +553,14 @@ inline int grid_of(int64_t blocks, unsigned *grid) {
 // segments have hardly more than 32 rows one wave a workgroup leaves none idle.
 inline int waves_for(int64_t rows, int64_t segments) { return rows > 48 * segments ? 4 : 1; }
 
-// Pieces of a long axis: until the chip has four workgroups to a CU, none shorter than 256 rows on average.
+// Pieces of a long axis: until the chip has `kPartsPerCu` workgroups to a CU (more than run at once, as segments and so their pieces differ in
+// length), none shorter than 256 rows on average.
+constexpr int64_t kPartsPerCu = 12;
 inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments) {
-  const int64_t want = 4 * (int64_t)num_cus() / (workgroups > 0 ? workgroups : 1), most = partners / (segments > 0 ? segments : 1) / 256;
+  if (workgroups > 2 * (int64_t)num_cus()) return 1;
+  const int64_t want = kPartsPerCu * num_cus() / (workgroups > 0 ? workgroups : 1), most = partners / (segments > 0 ? segments : 1) / 256;
   const int64_t parts = want < most ? want : most;
-  return parts < 2 ? 1 : parts > 1024 ? 1024 : (int)parts;
+  return parts < 2 ? 1 : parts > kMostParts ? kMostParts : (int)parts;
 }
 
 // Workgroups of a launch over tiles of `rows` rows: slots and order go into `a`.
@@ -566,7 +594,7 @@ int forward(AttentionArgs a) {
   if (rc != FGMS_OK) return rc;
   a.part_lse = a.part_sum + rows * a.dim;
   segment_attention_kernel<T, DP, NW, true><<<grid, NW * 64, 0, a.stream>>>(a);
-  join_parts_kernel<T, NW, false><<<(unsigned)tiles, 256, 0, a.stream>>>(a, a.q_offsets, a.n_q, group, a.part_sum, (T *)a.out, 1.f);
+  join_parts_kernel<T, NW, false><<<(unsigned)tiles * (32 * NW / kJoinRows), 256, 0, a.stream>>>(a, a.q_offsets, a.n_q, group, a.part_sum, (T *)a.out);
   return launched("segment attention");
 }
 
@@ -584,7 +612,7 @@ int query_grad(AttentionArgs a) {
   rc = workspace_get(a.stream, kSlotAttention, (size_t)tiles * a.parts * 32 * NW * a.dim * sizeof(float), (void **)&a.part_sum);
   if (rc != FGMS_OK) return rc;
   attention_query_grad_kernel<T, DP, NW, true><<<grid, NW * 64, 0, a.stream>>>(a);
-  join_parts_kernel<T, NW, true><<<(unsigned)tiles, 256, 0, a.stream>>>(a, a.q_offsets, a.n_q, group, a.part_sum, (T *)a.gq, 1.f);
+  join_parts_kernel<T, NW, true><<<(unsigned)tiles * (32 * NW / kJoinRows), 256, 0, a.stream>>>(a, a.q_offsets, a.n_q, group, a.part_sum, (T *)a.gq);
   return launched("segment attention, queries' gradient");
 }
 
@@ -602,8 +630,8 @@ int key_grad(AttentionArgs a) {
   rc = workspace_get(a.stream, kSlotAttention, 2 * all * sizeof(float), (void **)&a.part_sum);
   if (rc != FGMS_OK) return rc;
   attention_key_grad_kernel<T, DP, NW, true><<<grid, NW * 64, 0, a.stream>>>(a);
-  if (a.gk) join_parts_kernel<T, NW, true><<<(unsigned)tiles, 256, 0, a.stream>>>(a, a.k_offsets, a.n_k, 1, a.part_sum, (T *)a.gk, 1.f);
-  if (a.gv) join_parts_kernel<T, NW, true><<<(unsigned)tiles, 256, 0, a.stream>>>(a, a.k_offsets, a.n_k, 1, a.part_sum + all, (T *)a.gv, 1.f);
+  if (a.gk) join_parts_kernel<T, NW, true><<<(unsigned)tiles * (32 * NW / kJoinRows), 256, 0, a.stream>>>(a, a.k_offsets, a.n_k, 1, a.part_sum, (T *)a.gk);
+  if (a.gv) join_parts_kernel<T, NW, true><<<(unsigned)tiles * (32 * NW / kJoinRows), 256, 0, a.stream>>>(a, a.k_offsets, a.n_k, 1, a.part_sum + all, (T *)a.gv);
   return launched("segment attention, keys' gradients");
 }
 

@@ -175,18 +175,20 @@ __global__ __launch_bounds__(256) void norm_rotary_kernel(const NormRotaryArgs a
   }
 }
 
-// gscale[which][channel] = the workgroups' sums, 32 channels a workgroup, eight threads each.
+// gscale[which][channel] = the workgroups' sums, eight channels a workgroup, 128 threads each.
 template <typename T>
-__global__ __launch_bounds__(256) void scale_grad_kernel(const float *__restrict__ partial, int blocks, int dim, T *gq, T *gk) {
-  __shared__ float part[8][32];
-  const int column = blockIdx.x * 32 + threadIdx.x % 32, slice = threadIdx.x / 32;
+__global__ __launch_bounds__(1024) void scale_grad_kernel(const float *__restrict__ partial, int blocks, int dim, T *gq, T *gk) {
+  __shared__ float part[16][8];
+  const int c = threadIdx.x % 8, column = blockIdx.x * 8 + c, slice = threadIdx.x / 8;      // (dim is a multiple of 8)
   float sum = 0.f;
-  if (column < 2 * dim)
-    for (int b = slice; b < blocks; b += 8) sum += partial[(int64_t)b * 2 * dim + column];
-  part[slice][threadIdx.x % 32] = sum;
+#pragma unroll 8
+  for (int b = slice; b < blocks; b += 128) sum += partial[(int64_t)b * 2 * dim + column];
+  for (int d = 8; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if (threadIdx.x % 64 < 8) part[threadIdx.x / 64][c] = sum;
   __syncthreads();
-  if (slice || column >= 2 * dim) return;
-  for (int s = 1; s < 8; ++s) sum += part[s][threadIdx.x];
+  if (threadIdx.x >= 8) return;
+  sum = 0.f;
+  for (int s = 0; s < 16; ++s) sum += part[s][c];
   T *const to = column < dim ? gq : gk;
   if (to) to[column % dim] = (T)sum;
 }
@@ -220,7 +222,7 @@ int launch(const NormRotaryArgs &a) {
     return FGMS_E_INVALID;
   }
   norm_rotary_kernel<T, V, NEXT, BACKWARD><<<(unsigned)blocks, 256, lds, a.stream>>>(a, (int)tile, lanes, partial);
-  if (scales) scale_grad_kernel<T><<<(2 * a.dim + 31) / 32, 256, 0, a.stream>>>(partial, (int)blocks, a.dim, (T *)a.gscale[0], (T *)a.gscale[1]);
+  if (scales) scale_grad_kernel<T><<<2 * a.dim / 8, 1024, 0, a.stream>>>(partial, (int)blocks, a.dim, (T *)a.gscale[0], (T *)a.gscale[1]);
   FGMS_HIP_TRY(hipGetLastError());
   return FGMS_OK;
 }
