@@ -60,7 +60,8 @@ __device__ __forceinline__ int segment_begin(const int32_t *__restrict__ offsets
 
 struct Slot {
   int segment;
-  int begin, length;      // the segment's rows (times `group`: length in rows of the tile's matrix)
+  int begin, tokens;      // the segment's rows in the tensor
+  int length;             // ... in the tile's matrix: times `group`
   int first;              // the tile's first row, in the segment
 };
 
@@ -84,7 +85,8 @@ __device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, i
   r.segment = __builtin_amdgcn_readfirstlane(lo);
   r.begin = segment_begin(offsets, r.segment, segments, n);
   const int end = segment_begin(offsets, r.segment + 1, segments, n);
-  r.length = end > r.begin ? (end - r.begin) * group : 0;
+  r.tokens = max(end - r.begin, 0);
+  r.length = r.tokens * group;
   r.first = (slot - (r.begin * group / rows + r.segment)) * rows;
   return r;
 }

@@ -98,10 +98,10 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   if (slot.first >= slot.length) return;
   int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
-  const int ahead = k_count - slot.length / group;      // the last query sees the last key
+  const int ahead = k_count - slot.tokens;      // the last query sees the last key
 
   // keys that the rows see: those below `seen` for this lane's, of the workgroup's rows the last sees most, of a wave's the first least
-  const int token0 = slot.first / group, head0 = slot.first - token0 * group;      // the tile's first row
+  const int token0 = group == 1 ? slot.first : slot.first / group, head0 = slot.first - token0 * group;      // the tile's first row
   const float per_group = 1.f / group;
   const auto token_of = [&](int local) { return token0 + divide(head0 + local, per_group); };
   const int local = wave * 32 + lane % 32, token = token_of(local), head = at.kv_head * group + head0 + local - (token - token0) * group;
@@ -145,12 +145,11 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
       for (int i = 0; i < STEPS; ++i)
         if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s[kb], Rows::rows(k_tile, kb * 32, i, lane), q[i]);
     if (j + KB * 32 > whole) {
-      const int left = seen - j;
+      const int left = seen - j - 4 * (lane / 32);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (kb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 >= left) s[kb][r] = -inf;
+        for (int r = 0; r < 16; ++r) s[kb][r] = left > kb * 32 + 8 * (r / 4) + r % 4 ? s[kb][r] : -inf;
     }
     float top = s[0][0];
 #pragma unroll
@@ -316,9 +315,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   if (slot.first >= slot.length) return;
   int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
-  const int ahead = k_count - slot.length / group;
+  const int ahead = k_count - slot.tokens;
 
-  const int token0 = slot.first / group, head0 = slot.first - token0 * group;
+  const int token0 = group == 1 ? slot.first : slot.first / group, head0 = slot.first - token0 * group;
   const float per_group = 1.f / group;
   const auto token_of = [&](int local) { return token0 + divide(head0 + local, per_group); };
   const int local = wave * 32 + lane % 32, token = token_of(local), head = at.kv_head * group + head0 + local - (token - token0) * group;
@@ -365,10 +364,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], by, -lse)) * (dp[r] - delta);
     if (j + kb * 32 + 32 > whole) {
-      const int left = seen - j;
+      const int left = seen - j - kb * 32 - 4 * (lane / 32);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (kb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 >= left) s[r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = left > 8 * (r / 4) + r % 4 ? s[r] : 0.f;
     }
     add_weighted_rows<T, DP>(dq, k_tile, kb * 32, s, lane);
   };
@@ -439,7 +437,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   const float per_group = 1.f / group, inf = __builtin_inff();
   float next_lse, next_delta;
   const auto load = [&](int4v *q_tile, int4v *g_tile, int first) __attribute__((always_inline)) {
-    const int token0 = first / group, head0 = first - token0 * group;
+    const int token0 = group == 1 ? first : first / group, head0 = first - token0 * group;
     const __amdgpu_buffer_rsrc_t qs = rows_resource(q_base + token0 * q_row, kMaxBufferBytes), gs = rows_resource(g_base + token0 * g_row, kMaxBufferBytes);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -495,10 +493,12 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
       }
     }
     if (r0 + qb * 32 < whole) {
-      const int hidden = from - r0;
+      const int hidden = from - r0 - qb * 32 - 4 * (lane / 32);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (qb * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4 < hidden) p[r] = ds[r] = 0.f;
+      for (int r = 0; r < 16; ++r) {
+        p[r] = hidden > 8 * (r / 4) + r % 4 ? 0.f : p[r];
+        ds[r] = hidden > 8 * (r / 4) + r % 4 ? 0.f : ds[r];
+      }
     }
     add_weighted_rows<T, DP>(dv, g_tile, qb * 32, p, lane);
     add_weighted_rows<T, DP>(dk, q_tile, qb * 32, ds, lane);
