@@ -12,7 +12,7 @@ template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) == 4 
 
 // Waves to a SIMD that the registers are to leave room for.
 template <typename T, int DP> constexpr int waves_of_queries() { return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
-template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
+template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
 
 // 16 bytes a lane from a buffer to LDS, one lane's behind the other's from `to` on (the same for all lanes).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *to, unsigned offset) {
@@ -218,9 +218,9 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, 
                                                          const float *__restrict__ sums, T *__restrict__ out) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   constexpr int T_ROWS = 32 * NW;
-  __shared__ float weight[kJoinRows][kMostParts];
+  __shared__ float weight[kJoinRows][kMostParts + 1];      // (rows in different banks)
   const int per_row = a.dim / 4;
-  const Place at = place_of(blockIdx.x, a.kv_heads, T_ROWS / kJoinRows, 0, 0);      // (eight rows: a part of the tile)
+  const Place at = place_of(blockIdx.x, a.kv_heads, T_ROWS / kJoinRows, 0, 0);      // (its rows: a part of the tile)
   const Slot slot = find_slot(offsets, a.segments, n, group, T_ROWS, at.slot);
   const int row0 = at.part * kJoinRows, rows = min(kJoinRows, slot.length - slot.first - row0);
   if (rows <= 0) return;
@@ -230,28 +230,28 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, 
     return ((int64_t)(slot.begin + row / group) * a.kv_heads + at.kv_head) * group + row % group;
   };
   if constexpr (!SUMS) {
-    // 32 threads a row
-    const int local = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // eight threads a row
+    const int local = threadIdx.x / 8, lane = threadIdx.x % 8;
     const float inf = __builtin_inff();
     float most = -inf, total = 0.f;
     if (local < rows)
-      for (int p = lane; p < a.parts; p += 32) {
+      for (int p = lane; p < a.parts; p += 8) {
         const float lse = a.part_lse[first + (int64_t)p * T_ROWS + local];
         weight[local][p] = lse;
         most = __builtin_fmaxf(most, lse);
       }
-    for (int d = 1; d < 32; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+    for (int d = 1; d < 8; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
     if (local < rows)
-      for (int p = lane; p < a.parts; p += 32) {
+      for (int p = lane; p < a.parts; p += 8) {
         // (a part without keys has nothing written)
         const float w = weight[local][p] == -inf ? 0.f : __builtin_amdgcn_exp2f((weight[local][p] - most) * kLog2e);
         weight[local][p] = w;
         total += w;
       }
-    for (int d = 1; d < 32; d *= 2) total += __shfl_xor(total, d);
+    for (int d = 1; d < 8; d *= 2) total += __shfl_xor(total, d);
     const bool any = most != -inf || total != 0.f;      // (not a number: kept)
     if (local < rows) {
-      for (int p = lane; p < a.parts; p += 32) weight[local][p] = any ? weight[local][p] / total : 0.f;
+      for (int p = lane; p < a.parts; p += 8) weight[local][p] = any ? weight[local][p] / total : 0.f;
       if (a.lse && lane == 0) a.lse[place(local)] = any ? most + __builtin_log2f(total) * (1.f / kLog2e) : -inf;
     }
     __syncthreads();
@@ -551,14 +551,16 @@ inline int grid_of(int64_t blocks, unsigned *grid) {
 
 // Rows of a workgroup's tile go by the average segment: four waves of 32 share the staged tiles of the other side; where
 // segments have hardly more than 32 rows one wave a workgroup leaves none idle.
-inline int waves_for(int64_t rows, int64_t segments) { return rows > 48 * segments ? 4 : 1; }
+inline int waves_for(int64_t rows, int64_t segments) {
+  return rows > 256 * segments ? 4 : rows > 48 * segments ? 2 : 1;
+}
 
 // Pieces of a long axis: until the chip has `kPartsPerCu` workgroups to a CU (more than run at once, as segments and so their pieces differ in
-// length), none shorter than 256 rows on average.
+// length), none shorter than 256 rows on average (fp32, whose products take 16 times as long: 128).
 constexpr int64_t kPartsPerCu = 12;
-inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments) {
+inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments, int least) {
   if (workgroups > 2 * (int64_t)num_cus()) return 1;
-  const int64_t want = kPartsPerCu * num_cus() / (workgroups > 0 ? workgroups : 1), most = partners / (segments > 0 ? segments : 1) / 256;
+  const int64_t want = kPartsPerCu * num_cus() / (workgroups > 0 ? workgroups : 1), most = partners / (segments > 0 ? segments : 1) / least;
   const int64_t parts = want < most ? want : most;
   return parts < 2 ? 1 : parts > kMostParts ? kMostParts : (int)parts;
 }
@@ -566,7 +568,7 @@ inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments) {
 // Workgroups of a launch over tiles of `rows` rows: slots and order go into `a`.
 inline int plan_grid(AttentionArgs &a, int64_t rows, int tile, int64_t partners, unsigned *grid, int64_t *tiles) {
   const int64_t slots = attention_slots(rows, a.segments, tile), segments = a.segments > 0 ? a.segments : 1;
-  a.parts = parts_for((rows / tile + a.segments) * a.kv_heads, partners, a.segments);
+  a.parts = parts_for((rows / tile + a.segments) * a.kv_heads, partners, a.segments, a.dtype == FGMS_F32 ? 128 : 256);
   // (long: the partners of one segment and all heads are more than half of an XCD's L2)
   const int64_t element = a.dtype == FGMS_F32 ? 4 : 2;
   a.order = a.parts > 1 ? 0 : partners / segments * 2 * a.kv_heads * a.dim * element > (2 << 20) ? kPlaceByHead
@@ -635,9 +637,14 @@ int key_grad(AttentionArgs a) {
   return launched("segment attention, keys' gradients");
 }
 
+template <typename F>
+int by_waves(int waves, F f) {
+  return waves == 4 ? f(Blocks<4>()) : waves == 2 ? f(Blocks<2>()) : f(Blocks<1>());
+}
+
 template <typename T, int DP>
 int forward_any(const AttentionArgs &a) {
-  return waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments) == 4 ? forward<T, DP, 4>(a) : forward<T, DP, 1>(a);
+  return by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) { return forward<T, DP, decltype(w)::value>(a); });
 }
 
 template <typename T, int DP>
@@ -650,9 +657,9 @@ int backward_any(const AttentionArgs &a) {
     rc = launched("segment attention, backward");
   }
   if (rc == FGMS_OK && a.gq && a.n_q > 0)
-    rc = waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments) == 4 ? query_grad<T, DP, 4>(a) : query_grad<T, DP, 1>(a);
+    rc = by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) { return query_grad<T, DP, decltype(w)::value>(a); });
   if (rc == FGMS_OK && (a.gk || a.gv) && a.n_k > 0)
-    rc = waves_for(a.n_k, a.segments) == 4 ? key_grad<T, DP, 4>(a) : key_grad<T, DP, 1>(a);
+    rc = by_waves(waves_for(a.n_k, a.segments), [&](auto w) { return key_grad<T, DP, decltype(w)::value>(a); });
   return rc;
 }
 
