@@ -128,35 +128,56 @@ struct RowTile {
     else return (row >> 2) & 3;
   }
   static __device__ __forceinline__ int at(int row, int c) { return row * CH + (c ^ swizzle(row)); }
-  // operand with the tile's rows as its outer index: lane l has row row0 + l % 32, chunk 2 * step + l / 32
-  static __device__ __forceinline__ int4v rows(const int4v *tile, int row0, int step, int lane) {
-    return tile[at(row0 + lane % 32, 2 * step + lane / 32)];
+
+  // Where a lane reads, in bytes from a tile's first row: a tile's own place, and rows by 16s, go into the instructions.
+  static constexpr int STEPS = CH / 2, BLOCKS = DP / 32, COLUMNS = sizeof(T) == 2 ? 2 * BLOCKS : 8;
+  int row_at[STEPS], column_at[COLUMNS];
+  __device__ __forceinline__ void aim(int lane) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) row_at[i] = at(lane % 32, 2 * i + lane / 32) * 16;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, row = 4 * (lane >> 5) + (i >> 2), c = ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        column_at[2 * b] = at(row, 4 * b + c) * 16 + (i & 1) * 8;
+        column_at[2 * b + 1] = at(row + 8, 4 * b + c) * 16 + (i & 1) * 8;
+      }
+    } else {
+      const int col = BLOCKS * (lane % 32);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) column_at[r] = at(8 * (r / 4) + 4 * (lane / 32) + r % 4, col / 4) * 16 + col % 4 * 4;
+    }
   }
+  template <typename V>
+  static __device__ __forceinline__ V read(const int4v *tile, int from, int bytes) {
+    typedef __attribute__((address_space(3))) const char lds_char;
+    typedef __attribute__((address_space(3))) const V lds_v;
+    return *(lds_v *)((lds_char *)tile + from + bytes);
+  }
+  // operand with the tile's rows as its outer index: lane l has row row0 + l % 32, chunk 2 * step + l / 32
+  __device__ __forceinline__ int4v rows(const int4v *tile, int row0, int step) const { return read<int4v>(tile, row_at[step], row0 * CH * 16); }
   // 16-bit types: operand with the tile's columns as its outer index, contracted over its rows: lane l has column
-  // col0 + l % 32 of rows row0 + 4 * (l / 32) + {0 .. 3} and, 8 further down, four more -- the rows whose products the
+  // 32 b + l % 32 of rows row0 + 4 * (l / 32) + {0 .. 3} and, 8 further down, four more -- the rows whose products the
   // accumulator registers 8 i .. 8 i + 7 of that lane hold, so that these are the other operand as they are
-  static __device__ __forceinline__ int4v columns(const int4v *tile, int row0, int col0, int lane) {
+  __device__ __forceinline__ int4v columns(const int4v *tile, int row0, int b) const {
     typedef short short4v __attribute__((ext_vector_type(4)));
     typedef short short8v __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) const char lds_char;
     typedef __attribute__((address_space(3))) short4v lds_v4;
-    const int i = lane & 15, row = row0 + 4 * (lane >> 5) + (i >> 2), c = col0 / 8 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
-    const short *base = reinterpret_cast<const short *>(tile);
-    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4 *)(base + at(row, c) * 8 + (i & 1) * 4));
-    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4 *)(base + at(row + 8, c) * 8 + (i & 1) * 4));
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4 *)((lds_char *)tile + column_at[2 * b] + row0 * CH * 16));
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4 *)((lds_char *)tile + column_at[2 * b + 1] + row0 * CH * 16));
     const short8v v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(int4v, v);
   }
-  // float: channels (DP / 32) * (l % 32) + {0 .. DP / 32 - 1} of a row, one for each block of 32
-  static __device__ __forceinline__ void channels(float (&to)[DP / 32], const int4v *tile, int row, int lane) {
-    typedef float V __attribute__((ext_vector_type(DP / 32)));
-    const int col = DP / 32 * (lane % 32);
-    const float *const from = reinterpret_cast<const float *>(tile) + at(row, col / 4) * 4 + col % 4;
-    if constexpr (DP == 32) {
-      to[0] = *from;
+  // float: channels BLOCKS * (l % 32) + {0 .. BLOCKS - 1}, one for each block of 32, of the row whose product register r holds
+  __device__ __forceinline__ void channels(float (&to)[BLOCKS], const int4v *tile, int row0, int r) const {
+    typedef float V __attribute__((ext_vector_type(BLOCKS)));
+    if constexpr (BLOCKS == 1) {
+      to[0] = read<float>(tile, column_at[r % 8], (row0 + r / 8 * 16) * CH * 16);
     } else {
-      const V v = *reinterpret_cast<const V *>(from);
+      const V v = read<V>(tile, column_at[r % 8], (row0 + r / 8 * 16) * CH * 16);
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) to[b] = v[b];
+      for (int b = 0; b < BLOCKS; ++b) to[b] = v[b];
     }
   }
 };
@@ -165,8 +186,7 @@ struct RowTile {
 // accumulator holds it (register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32), rounded to T.  Which channels the rows
 // of out[b] are is free: 32 b + {0 .. 31} with the transposing read; float takes DP / 32 neighbouring ones a lane in one read.
 template <typename T, int DP>
-__device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], const int4v *tile, int row0, const float16v &w, int lane) {
-  using Rows = RowTile<T, DP>;
+__device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], const RowTile<T, DP> &at, const int4v *tile, int row0, const float16v &w) {
   if constexpr (sizeof(T) == 2) {
     typedef T T8 __attribute__((ext_vector_type(8)));
     typedef float float8v __attribute__((ext_vector_type(8)));
@@ -175,13 +195,13 @@ __device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], cons
       const float8v part = {w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3], w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]};
       const int4v b = __builtin_bit_cast(int4v, __builtin_convertvector(part, T8));
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) multiply<T>(out[db], Rows::columns(tile, row0 + 16 * i, db * 32, lane), b);
+      for (int db = 0; db < DP / 32; ++db) multiply<T>(out[db], at.columns(tile, row0 + 16 * i, db), b);
     }
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float rows[DP / 32];
-      Rows::channels(rows, tile, row0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4, lane);
+      at.channels(rows, tile, row0, r);
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) out[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(rows[db], w[r], out[db], 0, 0, 0);
     }
@@ -237,7 +257,7 @@ __device__ __forceinline__ void store_row(To *row, const float16v (&acc)[DP / 32
   }
 }
 
-template <int N> struct Blocks { static constexpr int value = N; };
+template <int N> struct Number { static constexpr int value = N; };
 
 constexpr float kLog2e = 1.4426950408889634f;
 

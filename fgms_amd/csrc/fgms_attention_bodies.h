@@ -54,8 +54,8 @@ __device__ __forceinline__ void tiles_ready() {
   __syncthreads();
 }
 
-// Where a launch's workgroup stands.  Long segments: head by head, so that the keys and values of few heads are in use at a time, and the
-// last tiles, which see most keys where the order is causal, first.  Short ones: the heads of a tile share lines of memory
+// Where a launch's workgroup stands.  Long segments: head by head, so that the keys and values of few heads are in use at a time, and
+// tiles with most partners where the order is causal first (the last queries, the first keys).  Short ones: the heads of a tile share lines of memory
 // (a row's heads lie side by side), so they and three neighbouring tiles go to one XCD (workgroup b runs on XCD b mod 8) one after the other;
 // launches too small for that take their tiles as they come.
 struct Place {
@@ -63,13 +63,15 @@ struct Place {
 };
 enum { kPlaceByHead = 1, kPlaceByXcd = 2 };
 constexpr int kPlaceTiles = 4;
+template <bool LAST_FIRST = true>
 __device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int parts, int order, int slots) {
   Place p;
   p.part = (int)(block % parts);
   block /= parts;
   if (order == kPlaceByHead) {
     p.kv_head = (int)(block / slots);
-    p.slot = slots - 1 - (int)(block % slots);
+    p.slot = (int)(block % slots);
+    if (LAST_FIRST) p.slot = slots - 1 - p.slot;
   } else {
     if (order == kPlaceByXcd) {
       const unsigned per = kPlaceTiles * kv_heads, i = block / 8;
@@ -92,6 +94,8 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   using Rows = RowTile<T, DP>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  Rows rows_at;
+  rows_at.aim(lane);
   const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
   if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot);
@@ -135,16 +139,16 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   constexpr float kSlack = 8.f;
   float most = -inf, base = 0.f, sum = 0.f;
   float16v o[DP / 32] = {};
-  // KB blocks of 32 keys
-  const auto take = [&](auto blocks, const int4v *k_tile, const int4v *v_tile, int j) __attribute__((always_inline)) {
+  // KB blocks of 32 keys, all seen by all rows or not
+  const auto take = [&](auto blocks, auto masked, const int4v *k_tile, const int4v *v_tile, int j) __attribute__((always_inline)) {
     constexpr int KB = decltype(blocks)::value;
     float16v s[KB] = {};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int i = 0; i < STEPS; ++i)
-        if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s[kb], Rows::rows(k_tile, kb * 32, i, lane), q[i]);
-    if (j + KB * 32 > whole) {
+        if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s[kb], rows_at.rows(k_tile, kb * 32, i), q[i]);
+    if constexpr (decltype(masked)::value != 0) {
       const int left = seen - j - 4 * (lane / 32);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -177,21 +181,41 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
       }
     sum += add[0] + add[1];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) add_weighted_rows<T, DP>(o, v_tile, kb * 32, s[kb], lane);
+    for (int kb = 0; kb < KB; ++kb) add_weighted_rows<T, DP>(o, rows_at, v_tile, kb * 32, s[kb]);
   };
-  const auto step = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+  const auto load_next = [&](int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
     tiles_ready();
     if (j + NK < end) {
       k.load(k_next, j + NK, k_count, wave);
       v.load(v_next, j + NK, k_count, wave);
     }
-    if (NK == 64 && j + 32 < wave_end) take(Blocks<NK / 32>(), k_tile, v_tile, j);
-    else if (j < wave_end) take(Blocks<1>(), k_tile, v_tile, j);
   };
-  for (int j = begin; j < end; j += 2 * NK) {
-    step(k_tile0, v_tile0, k_tile1, v_tile1, j);
-    if (j + NK >= end) break;
-    step(k_tile1, v_tile1, k_tile0, v_tile0, j + NK);
+  const auto all_of = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+    load_next(k_next, v_next, j);
+    take(Number<NK / 32>(), Number<0>(), k_tile, v_tile, j);
+  };
+  const auto some_of = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+    load_next(k_next, v_next, j);
+    if (NK == 64 && j + 32 < wave_end) take(Number<NK / 32>(), Number<1>(), k_tile, v_tile, j);
+    else if (j < wave_end) take(Number<1>(), Number<1>(), k_tile, v_tile, j);
+  };
+  // Tiles that all rows of the wave see whole have a loop of their own: with a choice in it the accumulators are moved from
+  // registers to registers at its end, which waits for their last product.
+  int j = begin;
+  const int all_end = __builtin_amdgcn_readfirstlane(begin + max(min(whole, wave_end) - begin, 0) / NK * NK);
+  bool second = false;      // whose turn it is
+  while (j < all_end) {
+    all_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
+    j += NK;
+    second = j >= all_end;
+    if (second) break;
+    all_of(k_tile1, v_tile1, k_tile0, v_tile0, j);
+    j += NK;
+  }
+  for (; j < end; j += NK) {
+    if (second) some_of(k_tile1, v_tile1, k_tile0, v_tile0, j);
+    else some_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
+    second = !second;
   }
 
   sum = both_sum(sum);
@@ -309,6 +333,8 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   using Rows = RowTile<T, DP>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  Rows rows_at;
+  rows_at.aim(lane);
   const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
   if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot);
@@ -353,37 +379,56 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
 
   const float by = a.scale * kLog2e;
   float16v dq[DP / 32] = {};
-  const auto take = [&](const int4v *k_tile, const int4v *v_tile, int kb, int j) __attribute__((always_inline)) {
+  const auto take = [&](auto masked, const int4v *k_tile, const int4v *v_tile, int kb, int j) __attribute__((always_inline)) {
     float16v s = {}, dp = {};
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
-      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s, Rows::rows(k_tile, kb * 32, i, lane), q[i]);
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(s, rows_at.rows(k_tile, kb * 32, i), q[i]);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
-      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(dp, Rows::rows(v_tile, kb * 32, i, lane), g[i]);
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(dp, rows_at.rows(v_tile, kb * 32, i), g[i]);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], by, -lse)) * (dp[r] - delta);
-    if (j + kb * 32 + 32 > whole) {
+    if constexpr (decltype(masked)::value != 0) {
       const int left = seen - j - kb * 32 - 4 * (lane / 32);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = left > 8 * (r / 4) + r % 4 ? s[r] : 0.f;
     }
-    add_weighted_rows<T, DP>(dq, k_tile, kb * 32, s, lane);
+    add_weighted_rows<T, DP>(dq, rows_at, k_tile, kb * 32, s);
   };
-  const auto step = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+  const auto load_next = [&](int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
     tiles_ready();
     if (j + NK < end) {
       k.load(k_next, j + NK, k_count, wave);
       v.load(v_next, j + NK, k_count, wave);
     }
+  };
+  const auto all_of = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+    load_next(k_next, v_next, j);
+#pragma unroll
+    for (int kb = 0; kb < NK / 32; ++kb) take(Number<0>(), k_tile, v_tile, kb, j);
+  };
+  const auto some_of = [&](const int4v *k_tile, const int4v *v_tile, int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
+    load_next(k_next, v_next, j);
 #pragma unroll
     for (int kb = 0; kb < NK / 32; ++kb)
-      if (j + kb * 32 < wave_end) take(k_tile, v_tile, kb, j);
+      if (j + kb * 32 < wave_end) take(Number<1>(), k_tile, v_tile, kb, j);
   };
-  for (int j = begin; j < end; j += 2 * NK) {
-    step(k_tile0, v_tile0, k_tile1, v_tile1, j);
-    if (j + NK >= end) break;
-    step(k_tile1, v_tile1, k_tile0, v_tile0, j + NK);
+  int j = begin;
+  const int all_end = __builtin_amdgcn_readfirstlane(begin + max(min(whole, wave_end) - begin, 0) / NK * NK);
+  bool second = false;
+  while (j < all_end) {
+    all_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
+    j += NK;
+    second = j >= all_end;
+    if (second) break;
+    all_of(k_tile1, v_tile1, k_tile0, v_tile0, j);
+    j += NK;
+  }
+  for (; j < end; j += NK) {
+    if (second) some_of(k_tile1, v_tile1, k_tile0, v_tile0, j);
+    else some_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
+    second = !second;
   }
   const float scale = a.scale * pow2(-ds_shift<T>());
   if constexpr (PARTS) {
@@ -404,7 +449,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   __shared__ int4v q_tile0[NQ * Rows::CH], g_tile0[NQ * Rows::CH], q_tile1[NQ * Rows::CH], g_tile1[NQ * Rows::CH];
   __shared__ float4v lse_tile0[NQ / 4], delta_tile0[NQ / 4], lse_tile1[NQ / 4], delta_tile1[NQ / 4];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  Rows rows_at;
+  rows_at.aim(lane);
+  const Place at = place_of<false>(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
   if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.k_offsets, a.segments, a.n_k, 1, T_ROWS, at.slot);
   if (slot.first >= slot.length) return;
@@ -473,15 +520,15 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   load_row<T, DP>(v, mine ? (const T *)a.v + (slot.begin + key) * a.v_row + at.kv_head * a.v_head : nullptr, a.dim, lane);
   const float by = a.scale * kLog2e;
   float16v dk[DP / 32] = {}, dv[DP / 32] = {};
-  const auto take = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
+  const auto take = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
                         int r0) __attribute__((always_inline)) {
     float16v p = {}, ds = {};
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
-      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(p, Rows::rows(q_tile, qb * 32, i, lane), k[i]);
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(p, rows_at.rows(q_tile, qb * 32, i), k[i]);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
-      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(ds, Rows::rows(g_tile, qb * 32, i, lane), v[i]);
+      if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(ds, rows_at.rows(g_tile, qb * 32, i), v[i]);
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const float4v lse = lse_tile[qb * 8 + 2 * r4 + lane / 32], delta = delta_tile[qb * 8 + 2 * r4 + lane / 32];
@@ -492,7 +539,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
         ds[r] = p[r] * ((ds[r] - delta[e]) * pow2(ds_shift<T>() - p_shift<T>()));
       }
     }
-    if (r0 + qb * 32 < whole) {
+    if constexpr (decltype(masked)::value != 0) {
       const int hidden = from - r0 - qb * 32 - 4 * (lane / 32);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -500,24 +547,51 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
         ds[r] = hidden > 8 * (r / 4) + r % 4 ? 0.f : ds[r];
       }
     }
-    add_weighted_rows<T, DP>(dv, g_tile, qb * 32, p, lane);
-    add_weighted_rows<T, DP>(dk, q_tile, qb * 32, ds, lane);
+    add_weighted_rows<T, DP>(dv, rows_at, g_tile, qb * 32, p);
+    add_weighted_rows<T, DP>(dk, rows_at, q_tile, qb * 32, ds);
   };
-  const auto step = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
-                        float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
+  const auto all_of = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
+                          float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
+    tiles_ready();
+    const bool more = r0 + NQ < end;
+    if (more) load(q_next, g_next, r0 + NQ);
+#pragma unroll
+    for (int qb = 0; qb < NQ / 32; ++qb) take(Number<0>(), q_tile, g_tile, lse_tile, delta_tile, qb, r0);
+    if (more) keep(lse_next, delta_next);
+  };
+  const auto some_of = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
+                           float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
     tiles_ready();
     const bool more = r0 + NQ < end;
     if (more) load(q_next, g_next, r0 + NQ);
 #pragma unroll
     for (int qb = 0; qb < NQ / 32; ++qb)
-      if (r0 + qb * 32 + 31 >= wave_from && r0 + qb * 32 < end) take(q_tile, g_tile, lse_tile, delta_tile, qb, r0);
+      if (r0 + qb * 32 + 31 >= wave_from && r0 + qb * 32 < end) take(Number<1>(), q_tile, g_tile, lse_tile, delta_tile, qb, r0);
     if (more) keep(lse_next, delta_next);
   };
-  for (int r0 = begin; r0 < end; r0 += 2 * NQ) {
-    step(q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
-    if (r0 + NQ >= end) break;
-    step(q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0 + NQ);
+  int r0 = begin;
+  bool second = false;
+  const auto some_until = [&](int stop) __attribute__((always_inline)) {
+    for (; r0 < stop; r0 += NQ) {
+      if (second) some_of(q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
+      else some_of(q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
+      second = !second;
+    }
+  };
+  // As in the forward kernel, a loop of their own for tiles that see all keys of the wave, from the first pair of buffers on.
+  const int all_from = __builtin_amdgcn_readfirstlane(awake ? begin + (max(whole - begin, 0) + NQ - 1) / NQ * NQ : end);
+  some_until(min(all_from, end));
+  if (second) some_until(min(r0 + NQ, end));
+  const int all_end = r0 + max(end - r0, 0) / NQ * NQ;
+  while (awake && r0 < all_end) {
+    all_of(q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
+    r0 += NQ;
+    second = r0 >= all_end;
+    if (second) break;
+    all_of(q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
+    r0 += NQ;
   }
+  some_until(end);
   const float k_by = a.scale * pow2(-ds_shift<T>()), v_by = pow2(-p_shift<T>());
   if (!mine) return;
   if constexpr (PARTS) {
@@ -639,7 +713,7 @@ int key_grad(AttentionArgs a) {
 
 template <typename F>
 int by_waves(int waves, F f) {
-  return waves == 4 ? f(Blocks<4>()) : waves == 2 ? f(Blocks<2>()) : f(Blocks<1>());
+  return waves == 4 ? f(Number<4>()) : waves == 2 ? f(Number<2>()) : f(Number<1>());
 }
 
 template <typename T, int DP>
