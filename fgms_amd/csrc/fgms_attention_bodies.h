@@ -550,48 +550,52 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
     add_weighted_rows<T, DP>(dv, rows_at, g_tile, qb * 32, p);
     add_weighted_rows<T, DP>(dk, rows_at, q_tile, qb * 32, ds);
   };
-  const auto all_of = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
+  const auto all_of = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
                           float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
     tiles_ready();
     const bool more = r0 + NQ < end;
     if (more) load(q_next, g_next, r0 + NQ);
 #pragma unroll
-    for (int qb = 0; qb < NQ / 32; ++qb) take(Number<0>(), q_tile, g_tile, lse_tile, delta_tile, qb, r0);
+    for (int qb = 0; qb < NQ / 32; ++qb) take(masked, q_tile, g_tile, lse_tile, delta_tile, qb, r0);
     if (more) keep(lse_next, delta_next);
   };
-  const auto some_of = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
-                           float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
+  const auto rest_of = [&](const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int r0) __attribute__((always_inline)) {
     tiles_ready();
-    const bool more = r0 + NQ < end;
-    if (more) load(q_next, g_next, r0 + NQ);
-#pragma unroll
-    for (int qb = 0; qb < NQ / 32; ++qb)
-      if (r0 + qb * 32 + 31 >= wave_from && r0 + qb * 32 < end) take(Number<1>(), q_tile, g_tile, lse_tile, delta_tile, qb, r0);
-    if (more) keep(lse_next, delta_next);
+    if (!awake) return;
+    take(Number<1>(), q_tile, g_tile, lse_tile, delta_tile, 0, r0);
+    if (NQ == 64 && r0 + 32 < end) take(Number<1>(), q_tile, g_tile, lse_tile, delta_tile, NQ / 32 - 1, r0);
   };
+  // Tiles that no key of the wave is seen from, tiles that some are not seen from (even numbers of both: the loops behind start with the
+  // first pair of buffers), whole tiles, and what is left.  As in the forward kernel the loops have no choice in them that the
+  // accumulators depend on.
   int r0 = begin;
+  const int wave_begin = __builtin_amdgcn_readfirstlane(awake ? min(begin + max(wave_from - begin, 0) / (2 * NQ) * (2 * NQ), end) : end);
+  for (bool second = false; r0 < wave_begin; r0 += NQ) {
+    tiles_ready();
+    second = !second;      // (the pair to be filled)
+    if (r0 + NQ >= end) continue;
+    load(second ? q_tile1 : q_tile0, second ? g_tile1 : g_tile0, r0 + NQ);
+    keep(second ? lse_tile1 : lse_tile0, second ? delta_tile1 : delta_tile0);
+  }
   bool second = false;
-  const auto some_until = [&](int stop) __attribute__((always_inline)) {
-    for (; r0 < stop; r0 += NQ) {
-      if (second) some_of(q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
-      else some_of(q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
-      second = !second;
+  const auto all_until = [&](auto masked, int stop) __attribute__((always_inline)) {
+    while (r0 < stop) {
+      all_of(masked, q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
+      r0 += NQ;
+      second = r0 >= stop;
+      if (second) break;
+      all_of(masked, q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
+      r0 += NQ;
     }
   };
-  // As in the forward kernel, a loop of their own for tiles that see all keys of the wave, from the first pair of buffers on.
-  const int all_from = __builtin_amdgcn_readfirstlane(awake ? begin + (max(whole - begin, 0) + NQ - 1) / NQ * NQ : end);
-  some_until(min(all_from, end));
-  if (second) some_until(min(r0 + NQ, end));
-  const int all_end = r0 + max(end - r0, 0) / NQ * NQ;
-  while (awake && r0 < all_end) {
-    all_of(q_tile0, g_tile0, lse_tile0, delta_tile0, q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
-    r0 += NQ;
-    second = r0 >= all_end;
-    if (second) break;
-    all_of(q_tile1, g_tile1, lse_tile1, delta_tile1, q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
-    r0 += NQ;
+  const int all_end = begin + max(end - begin, 0) / NQ * NQ;
+  const int masked_end = __builtin_amdgcn_readfirstlane(min(r0 + (max(whole - r0, 0) + 2 * NQ - 1) / (2 * NQ) * (2 * NQ), all_end));
+  all_until(Number<1>(), masked_end);
+  all_until(Number<0>(), all_end);
+  if (r0 < end) {
+    if (second) rest_of(q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
+    else rest_of(q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
   }
-  some_until(end);
   const float k_by = a.scale * pow2(-ds_shift<T>()), v_by = pow2(-p_shift<T>());
   if (!mine) return;
   if constexpr (PARTS) {
