@@ -69,22 +69,36 @@ struct Slot {
 // less than (x + 1/2) 2^-23 / by.
 __device__ __forceinline__ int divide(int x, float reciprocal) { return (int)(((float)x + 0.5f) * reciprocal); }
 
-// The slot's segment, by a search that asks 64 of them at a time.  `group`: rows of the matrix to a row of the tensor; all rows of
-// the tensor times `group` are less than 2^31.
-__device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, int segments, int n, int group, int rows, int slot) {
+// The slot's segment: 64 of them are asked at a time, first those around the place it has if all are of one length (windows of a cloud are
+// near enough: one round of loads), then by steps.  `group`: rows of the matrix to a row of the tensor; all rows of the tensor times
+// `group` are less than 2^31.  Whatever stands in the offsets, the segment found is one that begins at or before the slot.
+__device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, int segments, int n, int group, int rows, int slot, int slots) {
   const int lane = threadIdx.x % 64;
-  int lo = 0, hi = segments + 1;
-  while (hi - lo > 1) {
-    const int step = (int)(((unsigned)(hi - lo) + 63u) / 64u), at = (int)min((unsigned)lo + (lane + 1u) * (unsigned)step, (unsigned)hi);
-    const bool before = at < hi && segment_begin(offsets, at, segments, n) * group / rows + at <= slot;
-    const unsigned long long after = ~__builtin_amdgcn_ballot_w64(before);
-    lo += (after ? __builtin_ctzll(after) : 64) * step;      // (an entry that did begin before, in whatever order the others are)
-    hi = min(hi, lo + step);
+  // segments [lo, hi) are in question, and lo begins at or before the slot
+  int lo = 0, hi = segments + 1, step = 1;
+  int first = (int)((float)slot * (float)hi / (float)slots) - 32;
+  first = max(min(first, hi - 64), 0);
+  int count, value;
+  for (;;) {
+    const int at = (int)min((unsigned)first + (unsigned)lane * (unsigned)step, (unsigned)hi);
+    value = segment_begin(offsets, at, segments, n);
+    const unsigned long long after = ~__builtin_amdgcn_ballot_w64(at < hi && value * group / rows + at <= slot);
+    count = after ? __builtin_ctzll(after) : 64;
+    if (count == 0) {      // (all behind the slot: only if the first guess was)
+      hi = first;
+      first = lo;
+    } else {
+      lo = first + (count - 1) * step;
+      hi = count < 64 ? min(hi, lo + step) : hi;
+      if (hi - lo <= 1 && step == 1) break;
+      first = lo;
+    }
+    step = (int)(((unsigned)(hi - lo) + 63u) / 64u);
   }
   Slot r;
   r.segment = __builtin_amdgcn_readfirstlane(lo);
-  r.begin = segment_begin(offsets, r.segment, segments, n);
-  const int end = segment_begin(offsets, r.segment + 1, segments, n);
+  r.begin = __builtin_amdgcn_readlane(value, count - 1);
+  const int end = count < 64 ? __builtin_amdgcn_readlane(value, count) : segment_begin(offsets, r.segment + 1, segments, n);
   r.tokens = max(end - r.begin, 0);
   r.length = r.tokens * group;
   r.first = (slot - (r.begin * group / rows + r.segment)) * rows;

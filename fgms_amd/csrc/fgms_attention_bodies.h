@@ -98,10 +98,10 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   rows_at.aim(lane);
   const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
   if (at.slot >= a.slots) return;
-  const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot);
-  if (slot.first >= slot.length) return;
+  const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot, a.slots);
   int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
+  if (slot.first >= slot.length) return;
   const int ahead = k_count - slot.tokens;      // the last query sees the last key
 
   // keys that the rows see: those below `seen` for this lane's, of the workgroup's rows the last sees most, of a wave's the first least
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, 
   __shared__ float weight[kJoinRows][kMostParts + 1];      // (rows in different banks)
   const int per_row = a.dim / 4;
   const Place at = place_of(blockIdx.x, a.kv_heads, T_ROWS / kJoinRows, 0, 0);      // (its rows: a part of the tile)
-  const Slot slot = find_slot(offsets, a.segments, n, group, T_ROWS, at.slot);
+  const Slot slot = find_slot(offsets, a.segments, n, group, T_ROWS, at.slot, a.slots);
   const int row0 = at.part * kJoinRows, rows = min(kJoinRows, slot.length - slot.first - row0);
   if (rows <= 0) return;
   const int64_t first = ((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts * T_ROWS + row0;
@@ -307,22 +307,31 @@ template <typename T> constexpr int p_shift() { return __is_same(T, _Float16) ? 
 template <typename T> constexpr int ds_shift() { return __is_same(T, _Float16) ? 4 : 0; }
 constexpr float pow2(int e) { return e >= 0 ? (float)(1 << e) : 1.f / (float)(1 << -e); }
 
-// delta = g_out . out of each row and head: eight lanes a row.
-template <typename T>
+// delta = g_out . out of a lane's row, shared with its partner.
+template <typename T, int DP>
+__device__ __forceinline__ float row_delta(const int4v (&g)[DP / (32 / (int)sizeof(T))], const T *out, int dim, int lane) {
+  constexpr int E = 16 / (int)sizeof(T), STEPS = DP / (2 * E);
+  typedef T Te __attribute__((ext_vector_type(E)));
+  int4v o[STEPS];
+  load_row<T, DP>(o, out, dim, lane);
+  float delta = 0.f;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) delta = __builtin_fmaf((float)__builtin_bit_cast(Te, o[i])[e], (float)__builtin_bit_cast(Te, g[i])[e], delta);
+  return both_sum(delta);
+}
+
+// All rows' delta, where the queries' gradient, which has them on its way, is not wanted.
+template <typename T, int DP>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const T *__restrict__ g_out, const T *__restrict__ out,
                                                               float *__restrict__ delta, int64_t rows, int dim) {
-  typedef T T8 __attribute__((ext_vector_type(8)));
-  const int64_t row = (int64_t)blockIdx.x * 32 + threadIdx.x / 8;
-  float sum = 0.f;
-  if (row < rows)
-    for (int c = threadIdx.x % 8 * 8; c < dim; c += 64) {
-      const T8 x = *reinterpret_cast<const T8 *>(g_out + row * dim + c), y = *reinterpret_cast<const T8 *>(out + row * dim + c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)x[e], (float)y[e], sum);
-    }
-#pragma unroll
-  for (int d = 1; d < 8; d *= 2) sum += __shfl_xor(sum, d);
-  if (row < rows && threadIdx.x % 8 == 0) delta[row] = sum;
+  const int lane = threadIdx.x % 64;
+  const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x / 64 * 32 + lane % 32;
+  int4v g[DP / (32 / (int)sizeof(T))];
+  load_row<T, DP>(g, row < rows ? g_out + row * dim : nullptr, dim, lane);
+  const float sum = row_delta<T, DP>(g, row < rows ? out + row * dim : nullptr, dim, lane);
+  if (row < rows && lane < 32) delta[row] = sum;
 }
 
 // Queries' gradients.  As the forward kernel: a wave's 32 query rows are columns, so that a row's log-sum and delta are one value a lane,
@@ -337,10 +346,10 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   rows_at.aim(lane);
   const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
   if (at.slot >= a.slots) return;
-  const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot);
-  if (slot.first >= slot.length) return;
+  const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot, a.slots);
   int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
+  if (slot.first >= slot.length) return;
   const int ahead = k_count - slot.tokens;
 
   const int token0 = group == 1 ? slot.first : slot.first / group, head0 = slot.first - token0 * group;
@@ -375,7 +384,8 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   const float inf = __builtin_inff();
   float lse = mine ? a.lse[to] : inf;
   lse = lse == -inf ? inf : lse * kLog2e - ds_shift<T>();      // (no keys: all probabilities 0)
-  const float delta = mine ? a.delta[to] : 0.f;
+  const float delta = row_delta<T, DP>(g, mine ? (const T *)a.out + to * a.dim : nullptr, a.dim, lane);
+  if (mine && lane < 32 && (!PARTS || at.part == 0)) a.delta[to] = delta;      // (for the keys' gradients)
 
   const float by = a.scale * kLog2e;
   float16v dq[DP / 32] = {};
@@ -453,10 +463,10 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   rows_at.aim(lane);
   const Place at = place_of<false>(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
   if (at.slot >= a.slots) return;
-  const Slot slot = find_slot(a.k_offsets, a.segments, a.n_k, 1, T_ROWS, at.slot);
-  if (slot.first >= slot.length) return;
+  const Slot slot = find_slot(a.k_offsets, a.segments, a.n_k, 1, T_ROWS, at.slot, a.slots);
   int q_begin, q_count;
   partner_rows(a.q_offsets, nullptr, slot.segment, a.segments, a.n_q, q_begin, q_count);
+  if (slot.first >= slot.length) return;
   const int ahead = slot.length - q_count, rows = q_count * group;
 
   const int local = wave * 32 + lane % 32, key = slot.first + local;
@@ -728,14 +738,15 @@ int forward_any(const AttentionArgs &a) {
 template <typename T, int DP>
 int backward_any(const AttentionArgs &a) {
   const int64_t rows = (int64_t)a.n_q * a.heads;
-  unsigned grid;
-  int rc = grid_of((rows + 31) / 32, &grid);
-  if (rc == FGMS_OK && rows > 0) {
-    attention_delta_kernel<T><<<grid, 256, 0, a.stream>>>((const T *)a.g_out, (const T *)a.out, a.delta, rows, a.dim);
+  int rc = FGMS_OK;
+  if (a.gq && a.n_q > 0) {
+    rc = by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) { return query_grad<T, DP, decltype(w)::value>(a); });
+  } else if (rows > 0) {
+    unsigned grid;
+    if ((rc = grid_of((rows + 127) / 128, &grid)) != FGMS_OK) return rc;
+    attention_delta_kernel<T, DP><<<grid, 256, 0, a.stream>>>((const T *)a.g_out, (const T *)a.out, a.delta, rows, a.dim);
     rc = launched("segment attention, backward");
   }
-  if (rc == FGMS_OK && a.gq && a.n_q > 0)
-    rc = by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) { return query_grad<T, DP, decltype(w)::value>(a); });
   if (rc == FGMS_OK && (a.gk || a.gv) && a.n_k > 0)
     rc = by_waves(waves_for(a.n_k, a.segments), [&](auto w) { return key_grad<T, DP, decltype(w)::value>(a); });
   return rc;
