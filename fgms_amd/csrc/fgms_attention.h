@@ -58,6 +58,10 @@ __device__ __forceinline__ int segment_begin(const int32_t *__restrict__ offsets
   return s <= 0 ? 0 : s > segments ? n : min(max(at, 0), n);
 }
 
+// A value that the compiler does not know to be the wave's: what follows from it goes to the scalar unit (and a buffer's address that does
+// not is looped over lane by lane).
+__device__ __forceinline__ int same_for_all(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct Slot {
   int segment;
   int begin, tokens;      // the segment's rows in the tensor
@@ -96,9 +100,9 @@ __device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, i
     step = (int)(((unsigned)(hi - lo) + 63u) / 64u);
   }
   Slot r;
-  r.segment = __builtin_amdgcn_readfirstlane(lo);
+  r.segment = same_for_all(lo);
   r.begin = __builtin_amdgcn_readlane(value, count - 1);
-  const int end = count < 64 ? __builtin_amdgcn_readlane(value, count) : segment_begin(offsets, r.segment + 1, segments, n);
+  const int end = count < 64 ? __builtin_amdgcn_readlane(value, count) : same_for_all(segment_begin(offsets, r.segment + 1, segments, n));
   r.tokens = max(end - r.begin, 0);
   r.length = r.tokens * group;
   r.first = (slot - (r.begin * group / rows + r.segment)) * rows;
@@ -108,10 +112,10 @@ __device__ __forceinline__ Slot find_slot(const int32_t *__restrict__ offsets, i
 // The rows of the other side that go with segment s.
 __device__ __forceinline__ void partner_rows(const int32_t *__restrict__ offsets, const int32_t *__restrict__ lengths, int s,
                                              int segments, int n, int &begin, int &length) {
-  begin = segment_begin(offsets, s, segments, n);
-  const int end = segment_begin(offsets, s + 1, segments, n);
+  begin = same_for_all(segment_begin(offsets, s, segments, n));
+  const int end = same_for_all(segment_begin(offsets, s + 1, segments, n));
   length = s < segments && end > begin ? end - begin : 0;
-  if (lengths && s < segments) length = min(max(lengths[s], 0), length);
+  if (lengths && s < segments) length = min(max(same_for_all(lengths[s]), 0), length);
 }
 
 // acc += a x b, 16 bytes of the contracted axis a lane: 16 deep for 16-bit types, 8 for float.

@@ -40,7 +40,7 @@ struct Stager {
   }
   // rows [first, first + ROWS) of `count`
   __device__ __forceinline__ void load(int4v *tile, int first, int count, int wave) const {
-    const int there = min(max(count - first, 0), ROWS);
+    const int there = same_for_all(min(max(count - first, 0), ROWS));
     const __amdgpu_buffer_rsrc_t rows = rows_resource(base + first * stride, (unsigned)there * (unsigned)stride);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
   const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   }
   const int seen = a.causal ? min(k_count, token + ahead + 1) : k_count;
   const int whole = min(end, a.causal ? token_of(wave * 32) + ahead + 1 : k_count);
-  const int wave_end = __builtin_amdgcn_readfirstlane(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
+  const int wave_end = same_for_all(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
 
   Stager<T, DP, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   // Tiles that all rows of the wave see whole have a loop of their own: with a choice in it the accumulators are moved from
   // registers to registers at its end, which waits for their last product.
   int j = begin;
-  const int all_end = __builtin_amdgcn_readfirstlane(begin + max(min(whole, wave_end) - begin, 0) / NK * NK);
+  const int all_end = same_for_all(begin + max(min(whole, wave_end) - begin, 0) / NK * NK);
   bool second = false;      // whose turn it is
   while (j < all_end) {
     all_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
   const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   }
   const int seen = a.causal ? min(k_count, token + ahead + 1) : k_count;
   const int whole = min(end, a.causal ? token_of(wave * 32) + ahead + 1 : k_count);
-  const int wave_end = __builtin_amdgcn_readfirstlane(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
+  const int wave_end = same_for_all(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
 
   Stager<T, DP, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
       if (j + kb * 32 < wave_end) take(Number<1>(), k_tile, v_tile, kb, j);
   };
   int j = begin;
-  const int all_end = __builtin_amdgcn_readfirstlane(begin + max(min(whole, wave_end) - begin, 0) / NK * NK);
+  const int all_end = same_for_all(begin + max(min(whole, wave_end) - begin, 0) / NK * NK);
   bool second = false;
   while (j < all_end) {
     all_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   constexpr int PER = NQ * Rows::CH / (64 * NW);
   __shared__ int4v q_tile0[NQ * Rows::CH], g_tile0[NQ * Rows::CH], q_tile1[NQ * Rows::CH], g_tile1[NQ * Rows::CH];
   __shared__ float4v lse_tile0[NQ / 4], delta_tile0[NQ / 4], lse_tile1[NQ / 4], delta_tile1[NQ / 4];
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = a.heads / a.kv_heads;
+  const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
   const Place at = place_of<false>(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   // first pair of buffers), whole tiles, and what is left.  As in the forward kernel the loops have no choice in them that the
   // accumulators depend on.
   int r0 = begin;
-  const int wave_begin = __builtin_amdgcn_readfirstlane(awake ? min(begin + max(wave_from - begin, 0) / (2 * NQ) * (2 * NQ), end) : end);
+  const int wave_begin = same_for_all(awake ? min(begin + max(wave_from - begin, 0) / (2 * NQ) * (2 * NQ), end) : end);
   for (bool second = false; r0 < wave_begin; r0 += NQ) {
     tiles_ready();
     second = !second;      // (the pair to be filled)
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
     }
   };
   const int all_end = begin + max(end - begin, 0) / NQ * NQ;
-  const int masked_end = __builtin_amdgcn_readfirstlane(min(r0 + (max(whole - r0, 0) + 2 * NQ - 1) / (2 * NQ) * (2 * NQ), all_end));
+  const int masked_end = same_for_all(min(r0 + (max(whole - r0, 0) + 2 * NQ - 1) / (2 * NQ) * (2 * NQ), all_end));
   all_until(Number<1>(), masked_end);
   all_until(Number<0>(), all_end);
   if (r0 < end) {
