@@ -485,31 +485,51 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   }
   if (a.causal) begin = max(begin, max(0, slot.first - ahead) * group / NQ * NQ);
 
-  // Rows on their way to LDS: row r is head r % group of token r / group, whose place in the tensors is found anew for every tile.
+  // Rows on their way to LDS: row r is head r % group of token r / group.  Where a lane's rows lie behind their tile's first token is the same
+  // for all tiles if these begin with a group's first head, which tiles of NQ rows do where the group divides NQ.
   const int64_t q_row = a.q_row * (int)sizeof(T), q_head = a.q_head * (int)sizeof(T), g_row = (int64_t)a.heads * a.dim * (int)sizeof(T);
   const char *const q_base = (const char *)a.q + q_begin * q_row + at.kv_head * group * q_head;
   const char *const g_base = (const char *)a.g_out + q_begin * g_row + (int64_t)at.kv_head * group * a.dim * (int)sizeof(T);
   const float *const lse_base = a.lse + (int64_t)q_begin * a.heads + at.kv_head * group;
   const float *const delta_base = a.delta + (int64_t)q_begin * a.heads + at.kv_head * group;
   const float per_group = 1.f / group, inf = __builtin_inff();
-  float next_lse, next_delta;
-  const auto load = [&](int4v *q_tile, int4v *g_tile, int first) __attribute__((always_inline)) {
-    const int token0 = group == 1 ? first : first / group, head0 = first - token0 * group;
-    const __amdgpu_buffer_rsrc_t qs = rows_resource(q_base + token0 * q_row, kMaxBufferBytes), gs = rows_resource(g_base + token0 * g_row, kMaxBufferBytes);
+  const bool steady = NQ % group == 0;
+  unsigned q_at[PER], g_at[PER], row_sum_at;
+  const auto aim = [&](int head0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = (wave + i * NW) * 64 + lane, row = e / Rows::CH, c = (e % Rows::CH) ^ Rows::swizzle(row);
       const int token = divide(head0 + row, per_group), head = head0 + row - token * group;
-      const bool there = first + row < rows && c * Rows::E < a.dim;
-      load_to_lds(qs, q_tile + (wave + i * NW) * 64,
-                  there ? (unsigned)token * (unsigned)q_row + (unsigned)head * (unsigned)q_head + c * 16 : kAbsentRow);
-      load_to_lds(gs, g_tile + (wave + i * NW) * 64,
-                  there ? (unsigned)token * (unsigned)g_row + (unsigned)(head * a.dim * (int)sizeof(T)) + c * 16 : kAbsentRow);
+      const bool there = c * Rows::E < a.dim;
+      q_at[i] = there ? (unsigned)token * (unsigned)q_row + (unsigned)head * (unsigned)q_head + c * 16 : kAbsentRow;
+      g_at[i] = there ? (unsigned)token * (unsigned)g_row + (unsigned)(head * a.dim * (int)sizeof(T)) + c * 16 : kAbsentRow;
     }
-    if (wave == 0 && lane < NQ) {
-      const int token = divide(head0 + lane, per_group), head = head0 + lane - token * group;
-      const bool there = first + lane < rows;
-      const int64_t to = there ? (int64_t)(token0 + token) * a.heads + head : 0;
+    const int token = divide(head0 + lane, per_group);
+    row_sum_at = (unsigned)token * a.heads + (head0 + lane - token * group);
+  };
+  aim(steady ? 0 : same_for_all(begin % group));
+  float next_lse = 0.f, next_delta = 0.f;
+  const auto load = [&](int4v *q_tile, int4v *g_tile, int first) __attribute__((always_inline)) {
+    const int token0 = same_for_all(group == 1 ? first : first / group);
+    if (!steady) aim(first - token0 * group);
+    const __amdgpu_buffer_rsrc_t qs = rows_resource(q_base + token0 * q_row, kMaxBufferBytes), gs = rows_resource(g_base + token0 * g_row, kMaxBufferBytes);
+    if (first + NQ <= rows) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        load_to_lds(qs, q_tile + (wave + i * NW) * 64, q_at[i]);
+        load_to_lds(gs, g_tile + (wave + i * NW) * 64, g_at[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const bool there = first + ((wave + i * NW) * 64 + lane) / Rows::CH < rows;
+        load_to_lds(qs, q_tile + (wave + i * NW) * 64, there ? q_at[i] : kAbsentRow);
+        load_to_lds(gs, g_tile + (wave + i * NW) * 64, there ? g_at[i] : kAbsentRow);
+      }
+    }
+    if (wave == 0) {
+      const bool there = lane < NQ && first + lane < rows;
+      const int64_t to = (int64_t)token0 * a.heads + (there ? row_sum_at : 0);
       next_lse = lse_base[to], next_delta = delta_base[to];
       next_lse = there ? next_lse : -inf;      // (no such row: all probabilities 0)
       next_delta = there ? next_delta : 0.f;
