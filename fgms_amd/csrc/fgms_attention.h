@@ -32,7 +32,8 @@ struct AttentionArgs {
   const void *g_out;     // [n_q, heads, dim]
   float *delta;          // [n_q, heads]: g_out . out
   void *gq, *gk, *gv;    // contiguous, any of them may be nullptr
-  int order, slots;      // of the workgroups (place_of), and the tiles of each key head
+  int slots;             // tiles of each key head
+  bool by_xcd;           // order of the workgroups (place_of)
   // a long axis cut into `parts` pieces, joined by a second launch
   int parts;
   float *part_sum;       // [slot][kv head][part][tile row][dim]

@@ -54,32 +54,27 @@ __device__ __forceinline__ void tiles_ready() {
   __syncthreads();
 }
 
-// Where a launch's workgroup stands.  Long segments: head by head, so that the keys and values of few heads are in use at a time, and
-// tiles with most partners where the order is causal first (the last queries, the first keys).  Short ones: the heads of a tile share lines of memory
-// (a row's heads lie side by side), so they and three neighbouring tiles go to one XCD (workgroup b runs on XCD b mod 8) one after the other;
-// launches too small for that take their tiles as they come.
+// Where a launch's workgroup stands: the heads of a tile one after the other, tiles with most partners where the order is causal first (the
+// last queries, the first keys): workgroups start in this order, and the long ones are then not the last to end.  (Three causal scans
+// of 12 k rows together, 16 heads of 64, both passes: 619 us; head by head, as few of them share the L2s then, 795.)
+// Short segments: the heads of a tile share lines of memory (a row's heads lie side by side), so they and three neighbouring tiles go
+// to one XCD (workgroup b runs on XCD b mod 8); not where that leaves XCDs without work.
 struct Place {
   int slot, kv_head, part;
 };
-enum { kPlaceByHead = 1, kPlaceByXcd = 2 };
 constexpr int kPlaceTiles = 4;
 template <bool LAST_FIRST = true>
-__device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int parts, int order, int slots) {
+__device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int parts, bool by_xcd, int slots) {
   Place p;
   p.part = (int)(block % parts);
   block /= parts;
-  if (order == kPlaceByHead) {
-    p.kv_head = (int)(block / slots);
-    p.slot = (int)(block % slots);
-    if (LAST_FIRST) p.slot = slots - 1 - p.slot;
-  } else {
-    if (order == kPlaceByXcd) {
-      const unsigned per = kPlaceTiles * kv_heads, i = block / 8;
-      block = (i / per * 8 + block % 8) * per + i % per;
-    }
-    p.kv_head = (int)(block % kv_heads);
-    p.slot = (int)(block / kv_heads);
+  if (by_xcd) {
+    const unsigned per = kPlaceTiles * kv_heads, i = block / 8;
+    block = (i / per * 8 + block % 8) * per + i % per;
   }
+  p.kv_head = (int)(block % kv_heads);
+  p.slot = (int)(block / kv_heads);
+  if (LAST_FIRST && p.slot < slots) p.slot = slots - 1 - p.slot;
   return p;
 }
 
@@ -96,7 +91,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
   if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot, a.slots);
   int k_begin, k_count;
@@ -244,7 +239,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, 
   constexpr int T_ROWS = 32 * NW;
   __shared__ float weight[kJoinRows][kMostParts + 1];      // (rows in different banks)
   const int per_row = a.dim / 4;
-  const Place at = place_of(blockIdx.x, a.kv_heads, T_ROWS / kJoinRows, 0, 0);      // (its rows: a part of the tile)
+  const Place at = place_of<false>(blockIdx.x, a.kv_heads, T_ROWS / kJoinRows, false, a.slots);      // (its rows: a part of the tile)
   const Slot slot = find_slot(offsets, a.segments, n, group, T_ROWS, at.slot, a.slots);
   const int row0 = at.part * kJoinRows, rows = min(kJoinRows, slot.length - slot.first - row0);
   if (rows <= 0) return;
@@ -344,7 +339,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
   if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot, a.slots);
   int k_begin, k_count;
@@ -461,7 +456,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
-  const Place at = place_of<false>(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.order, a.slots);
+  const Place at = place_of<false>(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
   if (at.slot >= a.slots) return;
   const Slot slot = find_slot(a.k_offsets, a.segments, a.n_k, 1, T_ROWS, at.slot, a.slots);
   int q_begin, q_count;
@@ -673,17 +668,16 @@ inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments, int
   return parts < 2 ? 1 : parts > kMostParts ? kMostParts : (int)parts;
 }
 
-// Workgroups of a launch over tiles of `rows` rows: slots and order go into `a`.
+// Workgroups of a launch over tiles of `rows` rows: slots, parts and order go into `a`.
 inline int plan_grid(AttentionArgs &a, int64_t rows, int tile, int64_t partners, unsigned *grid, int64_t *tiles) {
   const int64_t slots = attention_slots(rows, a.segments, tile), segments = a.segments > 0 ? a.segments : 1;
   a.parts = parts_for((rows / tile + a.segments) * a.kv_heads, partners, a.segments, a.dtype == FGMS_F32 ? 128 : 256);
-  // (long: the partners of one segment and all heads are more than half of an XCD's L2)
+  // (short: the partners of a segment, all heads, are less than half of an XCD's L2)
   const int64_t element = a.dtype == FGMS_F32 ? 4 : 2;
-  a.order = a.parts > 1 ? 0 : partners / segments * 2 * a.kv_heads * a.dim * element > (2 << 20) ? kPlaceByHead
-            : slots * a.kv_heads >= 64 * kPlaceTiles * a.kv_heads ? kPlaceByXcd : 0;
+  a.by_xcd = a.parts == 1 && slots >= 64 * kPlaceTiles && partners / segments * 2 * a.kv_heads * a.dim * element <= (2 << 20);
   *tiles = slots * a.kv_heads;
   const int64_t per = (int64_t)kPlaceTiles * a.kv_heads * 8;
-  const int rc = grid_of((a.order == kPlaceByXcd ? (*tiles + per - 1) / per * per : *tiles) * a.parts, grid);
+  const int rc = grid_of((a.by_xcd ? (*tiles + per - 1) / per * per : *tiles) * a.parts, grid);
   a.slots = (int)slots;
   return rc;
 }
