@@ -236,6 +236,11 @@ __device__ __forceinline__ float both_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
   return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
+// Lane l % 32 + 32's.
+__device__ __forceinline__ float of_upper(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return __builtin_bit_cast(float, (unsigned)r[1]);
+}
 
 // Row `row` (or nullptr) of `dim` channels into fragments, zeros where there is nothing.
 template <typename T, int DP>

@@ -22,7 +22,8 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *
 
 // Rows of a strided tensor on their way to a tile in LDS, past the registers: every lane asks for the chunk that belongs where
 // its 16 bytes land.  Chunks behind the channels, and rows behind the last, are out of the buffer's range and arrive as zeros.
-template <typename T, int DP, int ROWS, int NW>
+// (KEEP: chunks behind the channels stay as they are.)
+template <typename T, int DP, int ROWS, int NW, bool KEEP = false>
 struct Stager {
   using Rows = RowTile<T, DP>;
   static constexpr int PER = ROWS * Rows::CH / (64 * NW);
@@ -44,7 +45,7 @@ struct Stager {
     const __amdgpu_buffer_rsrc_t rows = rows_resource(base + first * stride, (unsigned)there * (unsigned)stride);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      load_to_lds(rows, tile + (wave + i * NW) * 64, offset[i]);
+      if (!KEEP || offset[i] != kAbsentRow) load_to_lds(rows, tile + (wave + i * NW) * 64, offset[i]);
   }
 };
 
@@ -82,8 +83,10 @@ __device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int part
 // A wave holds 32 query rows as columns: scores come out of the matrix unit transposed (keys down the registers, a query a
 // lane and its partner 32 lanes on), so that a row's maximum and sum are taken inside two lanes, and the exponentials are
 // the right operand of the second product as they stand, with no exchange between lanes.  Tiles of keys and values pass through
-// two pairs of buffers: the next one is on its way while this one is worked on.
-template <typename T, int DP, int NW, bool PARTS>
+// two pairs of buffers: the next one is on its way while this one is worked on.  ONES: a head has fewer channels than the tile (16-bit types);
+// the values' last column then holds ones, and the rows' sums come out of the second product, a sixth of the vector instructions less
+// (of the probabilities as rounded for it, so that a row's weights add up to one).
+template <typename T, int DP, int NW, bool PARTS, bool ONES>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_attention_kernel(const AttentionArgs a) {
   constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
@@ -119,11 +122,20 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
 
   Stager<T, DP, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
-  Stager<T, DP, NK, NW> v;
+  Stager<T, DP, NK, NW, ONES> v;
   v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
   if (begin < end) {
     k.load(k_tile0, begin, k_count, wave);
     v.load(v_tile0, begin, k_count, wave);
+  }
+  if constexpr (ONES) {
+    // (chunks behind the channels: zeros, and a one at the end of a row; no load touches them)
+    const int4v last = {0, 0, 0, (int)((unsigned)__builtin_bit_cast(unsigned short, (T)1.f) << 16)};
+    for (int e = threadIdx.x; e < NK * Rows::CH; e += 64 * NW) {
+      const int row = e / Rows::CH, c = e % Rows::CH;
+      if (c * Rows::E < a.dim) continue;
+      v_tile0[Rows::at(row, c)] = v_tile1[Rows::at(row, c)] = c == Rows::CH - 1 ? last : int4v{0, 0, 0, 0};
+    }
   }
   int4v q[STEPS];
   load_row<T, DP>(q, mine ? (const T *)a.q + (slot.begin + token) * a.q_row + head * a.q_head : nullptr, a.dim, lane);
@@ -162,7 +174,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
       const float keep = mine ? __builtin_amdgcn_exp2f(most - top) : 1.f;
       most = mine ? top : most;
       base = mine ? top : base;
-      sum *= keep;
+      if constexpr (!ONES) sum *= keep;
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db) o[db] *= keep;
     }
@@ -172,9 +184,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], by, -base));
-        add[r % 2] += s[kb][r];
+        if constexpr (!ONES) add[r % 2] += s[kb][r];
       }
-    sum += add[0] + add[1];
+    if constexpr (!ONES) sum += add[0] + add[1];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) add_weighted_rows<T, DP>(o, rows_at, v_tile, kb * 32, s[kb]);
   };
@@ -213,7 +225,8 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
     second = !second;
   }
 
-  sum = both_sum(sum);
+  // (the last column's products: row 31 of the last block, register 15 of the upper lanes)
+  sum = ONES ? of_upper(o[DP / 32 - 1][15]) : both_sum(sum);
   const bool none = seen <= begin || end <= begin;      // no key for this row (here)
   const float inverse = none ? 0.f : 1.f / sum;
   const float lse = none ? -inf : (base + __builtin_log2f(sum)) * (1.f / kLog2e);
@@ -682,7 +695,7 @@ inline int plan_grid(AttentionArgs &a, int64_t rows, int tile, int64_t partners,
   return rc;
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool ONES>
 int forward(AttentionArgs a) {
   const int group = a.heads / a.kv_heads;
   unsigned grid;
@@ -690,14 +703,14 @@ int forward(AttentionArgs a) {
   int rc = plan_grid(a, (int64_t)a.n_q * group, 32 * NW, a.n_k, &grid, &tiles);
   if (rc != FGMS_OK) return rc;
   if (a.parts == 1) {
-    segment_attention_kernel<T, DP, NW, false><<<grid, NW * 64, 0, a.stream>>>(a);
+    segment_attention_kernel<T, DP, NW, false, ONES><<<grid, NW * 64, 0, a.stream>>>(a);
     return launched("segment attention");
   }
   const size_t rows = (size_t)tiles * a.parts * 32 * NW;
   rc = workspace_get(a.stream, kSlotAttention, rows * (a.dim + 1) * sizeof(float), (void **)&a.part_sum);
   if (rc != FGMS_OK) return rc;
   a.part_lse = a.part_sum + rows * a.dim;
-  segment_attention_kernel<T, DP, NW, true><<<grid, NW * 64, 0, a.stream>>>(a);
+  segment_attention_kernel<T, DP, NW, true, ONES><<<grid, NW * 64, 0, a.stream>>>(a);
   join_parts_kernel<T, NW, false><<<(unsigned)tiles * (32 * NW / kJoinRows), 256, 0, a.stream>>>(a, a.q_offsets, a.n_q, group, a.part_sum, (T *)a.out);
   return launched("segment attention");
 }
@@ -746,7 +759,11 @@ int by_waves(int waves, F f) {
 
 template <typename T, int DP>
 int forward_any(const AttentionArgs &a) {
-  return by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) { return forward<T, DP, decltype(w)::value>(a); });
+  return by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) {
+    if constexpr (sizeof(T) == 2)
+      if (a.dim < DP) return forward<T, DP, decltype(w)::value, true>(a);
+    return forward<T, DP, decltype(w)::value, false>(a);
+  });
 }
 
 template <typename T, int DP>
