@@ -137,7 +137,7 @@ __device__ __forceinline__ void multiply(float16v &acc, const int4v &a, const in
 // for the same chunk, one of columns (16-bit types: the transposing read) by 16 lanes that ask four rows for four chunks,
 // two rows' worth beside it.  Chunk c of a row lies at c ^ swizzle(row): both kinds then cover all banks, the first over 16 rows,
 // the second over its four (rows of 256 bytes: the row's lowest two bits move groups of four chunks, the next two the chunks
-// in them; of 128: bit 1 moves groups, as two rows share 256 bytes; of 64: four rows do).
+// in them; of 128, or 384: bit 1 moves groups, as two rows share 256 bytes; of 64, or 192: the groups move by themselves).
 template <typename T, int DP>
 struct RowTile {
   static constexpr int E = 16 / (int)sizeof(T), CH = DP / E;
@@ -162,7 +162,7 @@ struct RowTile {
         column_at[2 * b + 1] = at(row + 8, 4 * b + c) * 16 + (i & 1) * 8;
       }
     } else {
-      const int col = BLOCKS * (lane % 32);
+      const int col = (BLOCKS == 3 ? 1 : BLOCKS) * (lane % 32);
 #pragma unroll
       for (int r = 0; r < 8; ++r) column_at[r] = at(8 * (r / 4) + 4 * (lane / 32) + r % 4, col / 4) * 16 + col % 4 * 4;
     }
@@ -188,11 +188,14 @@ struct RowTile {
     const short8v v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(int4v, v);
   }
-  // float: channels BLOCKS * (l % 32) + {0 .. BLOCKS - 1}, one for each block of 32, of the row whose product register r holds
+  // float: channels BLOCKS * (l % 32) + {0 .. BLOCKS - 1}, one for each block of 32, of the row whose product register r holds (three
+  // blocks: 32 b + l % 32, as three floats in a row may lie in two chunks)
   __device__ __forceinline__ void channels(float (&to)[BLOCKS], const int4v *tile, int row0, int r) const {
     typedef float V __attribute__((ext_vector_type(BLOCKS)));
-    if constexpr (BLOCKS == 1) {
-      to[0] = read<float>(tile, column_at[r % 8], (row0 + r / 8 * 16) * CH * 16);
+    if constexpr (BLOCKS == 1 || BLOCKS == 3) {
+      // (32 channels on: eight chunks, which the swizzle of such rows leaves alone)
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) to[b] = read<float>(tile, column_at[r % 8], (row0 + r / 8 * 16) * CH * 16 + b * 128);
     } else {
       const V v = read<V>(tile, column_at[r % 8], (row0 + r / 8 * 16) * CH * 16);
 #pragma unroll
@@ -203,7 +206,7 @@ struct RowTile {
 
 // out[channel][lane's row] += sum over 32 rows of the tile from row0 on of tile[row][channel] * w[row][lane's row]; w as an
 // accumulator holds it (register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32), rounded to T.  Which channels the rows
-// of out[b] are is free: 32 b + {0 .. 31} with the transposing read; float takes DP / 32 neighbouring ones a lane in one read.
+// of out[b] are is free: 32 b + {0 .. 31} with the transposing read; float takes DP / 32 neighbouring ones a lane in one read (96: as 16-bit types).
 template <typename T, int DP>
 __device__ __forceinline__ void add_weighted_rows(float16v (&out)[DP / 32], const RowTile<T, DP> &at, const int4v *tile, int row0, const float16v &w) {
   if constexpr (sizeof(T) == 2) {
@@ -256,7 +259,7 @@ __device__ __forceinline__ void load_row(int4v (&to)[DP / (32 / (int)sizeof(T))]
 // A lane's row of a result, from accumulators of T's products that hold it as columns, times `by`.
 template <typename T, typename To, int DP>
 __device__ __forceinline__ void store_row(To *row, const float16v (&acc)[DP / 32], float by, int dim, int lane) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2 || DP == 96) {
     typedef To To4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)

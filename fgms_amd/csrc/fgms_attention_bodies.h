@@ -7,12 +7,12 @@
 namespace fgms {
 namespace {
 
-// Keys (queries in the keys' gradients) to a tile.
-template <typename T, int DP> constexpr int tile_rows() { return sizeof(T) == 4 ? 32 : 64; }
+// Keys (queries in the keys' gradients) to a tile: 64 where the four of them then take no more than 16 KB of LDS a wave.
+template <typename T, int DP, int NW> constexpr int tile_rows() { return sizeof(T) == 4 || 64 * DP / NW > 2048 ? 32 : 64; }
 
 // Waves to a SIMD that the registers are to leave room for.
 template <typename T, int DP> constexpr int waves_of_queries() { return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
-template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
+template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP >= 96 ? 1 : 2) : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
 
 // 16 bytes a lane from a buffer to LDS, one lane's behind the other's from `to` on (the same for all lanes).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *to, unsigned offset) {
@@ -88,7 +88,7 @@ __device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int part
 // (of the probabilities as rounded for it, so that a row's weights add up to one).
 template <typename T, int DP, int NW, bool PARTS, bool ONES>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_attention_kernel(const AttentionArgs a) {
-  constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
+  constexpr int NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T *__restric
 // and ds the right operand of dq^T = k^T ds as it stands.
 template <typename T, int DP, int NW, bool PARTS>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attention_query_grad_kernel(const AttentionArgs a) {
-  constexpr int NK = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
+  constexpr int NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
 // dk^T = q^T ds, dv^T = g_out^T p take ds and p as they stand.
 template <typename T, int DP, int NW, bool PARTS>
 __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_key_grad_kernel(const AttentionArgs a) {
-  constexpr int NQ = tile_rows<T, DP>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
+  constexpr int NQ = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, DP>;
   constexpr int PER = NQ * Rows::CH / (64 * NW);
   __shared__ int4v q_tile0[NQ * Rows::CH], g_tile0[NQ * Rows::CH], q_tile1[NQ * Rows::CH], g_tile1[NQ * Rows::CH];
@@ -671,20 +671,23 @@ inline int waves_for(int64_t rows, int64_t segments) {
   return rows > 256 * segments ? 4 : rows > 48 * segments ? 2 : 1;
 }
 
-// Pieces of a long axis: until the chip has `kPartsPerCu` workgroups to a CU (more than run at once, as segments and so their pieces differ in
-// length), none shorter than 256 rows on average (fp32, whose products take 16 times as long: 128).
-constexpr int64_t kPartsPerCu = 12;
-inline int parts_for(int64_t workgroups, int64_t partners, int64_t segments, int least) {
-  if (workgroups > 2 * (int64_t)num_cus()) return 1;
-  const int64_t want = kPartsPerCu * num_cus() / (workgroups > 0 ? workgroups : 1), most = partners / (segments > 0 ? segments : 1) / least;
+// Pieces of a long axis: until a CU has 16 waves (fp32, and single waves: twelve workgroups, more than run at once, as segments and so
+// their pieces differ in length), none shorter than 128 rows on average, and only where a segment has four such (fp32: two): the join is a
+// launch of five to ten microseconds, in which a workgroup gets through 300 to 500 rows.  (fp32, 37 segments of 540 keys, heads of
+// 40, forward: two pieces 79 us, four 68, seven 75; bf16, two of 1185, heads of 72: four 36, five 35, nine 43.)
+inline int parts_for(int64_t workgroups, int waves, int64_t partners, int64_t segments, int dtype) {
+  const int64_t least = 128, each = partners / (segments > 0 ? segments : 1);
+  if (each < (dtype == FGMS_F32 ? 2 : 4) * least) return 1;
+  const int64_t per_cu = dtype == FGMS_F32 || waves == 1 ? 12 : 16 / waves;
+  const int64_t want = per_cu * num_cus() / (workgroups > 0 ? workgroups : 1), most = each / least;
   const int64_t parts = want < most ? want : most;
-  return parts < 2 ? 1 : parts > kMostParts ? kMostParts : (int)parts;
+  return parts < 2 || workgroups > 2 * num_cus() ? 1 : parts > kMostParts ? kMostParts : (int)parts;
 }
 
 // Workgroups of a launch over tiles of `rows` rows: slots, parts and order go into `a`.
 inline int plan_grid(AttentionArgs &a, int64_t rows, int tile, int64_t partners, unsigned *grid, int64_t *tiles) {
   const int64_t slots = attention_slots(rows, a.segments, tile), segments = a.segments > 0 ? a.segments : 1;
-  a.parts = parts_for((rows / tile + a.segments) * a.kv_heads, partners, a.segments, a.dtype == FGMS_F32 ? 128 : 256);
+  a.parts = parts_for((rows / tile + a.segments) * a.kv_heads, tile / 32, partners, a.segments, a.dtype);
   // (short: the partners of a segment, all heads, are less than half of an XCD's L2)
   const int64_t element = a.dtype == FGMS_F32 ? 4 : 2;
   a.by_xcd = a.parts == 1 && slots >= 64 * kPlaceTiles && partners / segments * 2 * a.kv_heads * a.dim * element <= (2 << 20);
@@ -787,12 +790,12 @@ int backward_any(const AttentionArgs &a) {
 
 template <typename T>
 int attention_fwd(const AttentionArgs &a) {
-  return a.dim <= 32 ? forward_any<T, 32>(a) : a.dim <= 64 ? forward_any<T, 64>(a) : forward_any<T, 128>(a);
+  return a.dim <= 32 ? forward_any<T, 32>(a) : a.dim <= 64 ? forward_any<T, 64>(a) : a.dim <= 96 ? forward_any<T, 96>(a) : forward_any<T, 128>(a);
 }
 
 template <typename T>
 int attention_bwd(const AttentionArgs &a) {
-  return a.dim <= 32 ? backward_any<T, 32>(a) : a.dim <= 64 ? backward_any<T, 64>(a) : backward_any<T, 128>(a);
+  return a.dim <= 32 ? backward_any<T, 32>(a) : a.dim <= 64 ? backward_any<T, 64>(a) : a.dim <= 96 ? backward_any<T, 96>(a) : backward_any<T, 128>(a);
 }
 
 }  // namespace fgms
