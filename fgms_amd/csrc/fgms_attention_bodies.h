@@ -12,7 +12,7 @@ template <typename T, int DP, int NW> constexpr int tile_rows() { return sizeof(
 
 // Waves to a SIMD that the registers are to leave room for.
 template <typename T, int DP> constexpr int waves_of_queries() { return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
-template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP >= 96 ? 1 : 2) : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
+template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP >= 96 ? 1 : 2) : DP == 32 ? 3 : DP == 128 ? 1 : 2; }
 
 // 16 bytes a lane from a buffer to LDS, one lane's behind the other's from `to` on (the same for all lanes).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *to, unsigned offset) {
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   const int last = min(T_ROWS, slot.length - slot.first) - 1, wave_last = min(wave * 32 + 31, last);
   int begin = 0, end = a.causal ? min(k_count, token_of(last) + ahead + 1) : k_count;
   if constexpr (PARTS) {
-    const int piece = ((k_count + a.parts - 1) / a.parts + NK - 1) / NK * NK;
+    const int piece = ((max(end, 0) + a.parts - 1) / a.parts + NK - 1) / NK * NK;      // (of the keys that are seen)
     begin = at.part * piece;
     end = min(end, begin + piece);
   }
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   const int last = min(T_ROWS, slot.length - slot.first) - 1, wave_last = min(wave * 32 + 31, last);
   int begin = 0, end = a.causal ? min(k_count, token_of(last) + ahead + 1) : k_count;
   if constexpr (PARTS) {
-    const int piece = ((k_count + a.parts - 1) / a.parts + NK - 1) / NK * NK;
+    const int piece = ((max(end, 0) + a.parts - 1) / a.parts + NK - 1) / NK * NK;      // (of the keys that are seen)
     begin = at.part * piece;
     end = min(end, begin + piece);
   }
@@ -486,12 +486,12 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   const int from = a.causal ? max(0, key - ahead) * group : 0;
   const int wave_from = awake ? a.causal ? max(0, slot.first + wave * 32 - ahead) * group : 0 : rows;
   const int whole = a.causal ? max(0, slot.first + wave * 32 + 31 - ahead) * group : 0;
+  if (a.causal) begin = max(0, slot.first - ahead) * group / NQ * NQ;
   if constexpr (PARTS) {
-    const int piece = ((rows + a.parts - 1) / a.parts + NQ - 1) / NQ * NQ;
-    begin = at.part * piece;
+    const int piece = ((max(rows - begin, 0) + a.parts - 1) / a.parts + NQ - 1) / NQ * NQ;
+    begin += at.part * piece;
     end = min(end, begin + piece);
   }
-  if (a.causal) begin = max(begin, max(0, slot.first - ahead) * group / NQ * NQ);
 
   // Rows on their way to LDS: row r is head r % group of token r / group.  Where a lane's rows lie behind their tile's first token is the same
   // for all tiles if these begin with a group's first head, which tiles of NQ rows do where the group divides NQ.
