@@ -18,7 +18,7 @@ int refuse(const char *what, const char *why) {
 }
 
 constexpr int64_t kMostRowBytes = 16 << 20;      // 128 rows of a tile below 2^31
-constexpr int64_t kMostRows = INT32_MAX - (1 << 18);
+constexpr int64_t kMostRows = INT32_MAX - (1 << 25);
 
 bool aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -66,7 +66,7 @@ int check_attention(const char *what, const AttentionArgs &a, int64_t n_q, int64
   if (rc != FGMS_OK) return rc;
   if (a.kv_heads < 1 || a.heads % a.kv_heads) return refuse(what, "the query heads must be a multiple of the key heads");
   if (n_q < 0 || n_k < 0 || n_k > kMostRows || n_q > kMostRows / (a.heads / a.kv_heads))
-    return refuse(what, "the rows, times the heads of a group, must be fewer than 2^31 - 2^18");
+    return refuse(what, "the rows, times the heads of a group, must be fewer than 2^31 - 2^25");
   if (a.segments < 0 || a.segments > kMostRows) return refuse(what, "the number of segments is out of range");
   if (!a.q_offsets || !a.k_offsets) return refuse(what, "null offsets");
   if (!(a.scale > 0.f) || !(a.scale < 1e30f)) return refuse(what, "scale must be positive and finite");

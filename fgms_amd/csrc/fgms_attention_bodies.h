@@ -561,12 +561,16 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   const auto take = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
                         int r0) __attribute__((always_inline)) {
     float16v p = {}, ds = {};
+    // (heads of 96: what one step reads is not fetched during the one before, which the registers have no room for: 836 -> 775 us over 9 k rows)
+    const auto phase = []() __attribute__((always_inline)) { if constexpr (DP == 96) __builtin_amdgcn_sched_barrier(0); };
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
       if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(p, rows_at.rows(q_tile, qb * 32, i), k[i]);
+    phase();
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
       if (sizeof(T) == 2 || i * 2 * Rows::E < a.dim) multiply<T>(ds, rows_at.rows(g_tile, qb * 32, i), v[i]);
+    phase();
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const float4v lse = lse_tile[qb * 8 + 2 * r4 + lane / 32], delta = delta_tile[qb * 8 + 2 * r4 + lane / 32];
@@ -585,7 +589,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
         ds[r] = hidden > 8 * (r / 4) + r % 4 ? 0.f : ds[r];
       }
     }
+    phase();
     add_weighted_rows<T, DP>(dv, rows_at, g_tile, qb * 32, p);
+    phase();
     add_weighted_rows<T, DP>(dk, rows_at, q_tile, qb * 32, ds);
   };
   const auto all_of = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
