@@ -17,7 +17,7 @@ int refuse(const char *what, const char *why) {
   return FGMS_E_INVALID;
 }
 
-constexpr int64_t kMostRowBytes = 16 << 20;      // 128 rows of a tile below 2^31
+constexpr int64_t kMostRowBytes = 16 << 20;      // 64 rows of a tile, and 512 MB between the heads of a group: below 2^31
 constexpr int64_t kMostRows = INT32_MAX - (1 << 25);
 
 bool aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -30,7 +30,7 @@ int check_rows(const char *what, const void *p, bool there, int64_t row, int64_t
   if (!aligned(p) || row < 0 || head < 0 || row * bytes % 16 || head * bytes % 16)
     return refuse(what, "rows and heads have to begin on 16 bytes");
   // (a tile's rows are reached by 32-bit offsets)
-  if (row * bytes > kMostRowBytes || head > kMostRowBytes) return refuse(what, "rows lie too far apart");
+  if (row * bytes > kMostRowBytes) return refuse(what, "rows lie too far apart");
   return FGMS_OK;
 }
 
@@ -75,8 +75,8 @@ int check_attention(const char *what, const AttentionArgs &a, int64_t n_q, int64
   if ((rc = check_rows(what, a.v, n_k > 0, a.v_row, a.v_head, a.dtype))) return rc;
   // (a tile's rows end where the buffer over them does)
   if ((n_k > 1 && (a.k_row < a.dim || a.v_row < a.dim))) return refuse(what, "rows of k and v overlap");
-  if ((int64_t)a.heads * (a.q_head > a.dim ? a.q_head : a.dim) * element_bytes(a.dtype) > (int64_t)512 << 20)
-    return refuse(what, "the heads of a row lie too far apart");
+  if (a.q_head > ((int64_t)512 << 20) / element_bytes(a.dtype) / (a.heads / a.kv_heads))
+    return refuse(what, "the heads of a group lie too far apart");
   return FGMS_OK;
 }
 

@@ -7,12 +7,14 @@
 namespace fgms {
 namespace {
 
+// Channels of a tile in LDS, heads of up to DP: the products whose columns these are come in 32s (heads of up to 16 are contracted over 16).
+template <int DP> constexpr int tile_width() { return DP < 32 ? 32 : DP; }
 // Keys (queries in the keys' gradients) to a tile: 64 where the four of them then take no more than 16 KB of LDS a wave.
-template <typename T, int DP, int NW> constexpr int tile_rows() { return sizeof(T) == 4 || 64 * DP / NW > 2048 ? 32 : 64; }
+template <typename T, int DP, int NW> constexpr int tile_rows() { return sizeof(T) == 4 || 64 * tile_width<DP>() / NW > 2048 ? 32 : 64; }
 
 // Waves to a SIMD that the registers are to leave room for.
-template <typename T, int DP> constexpr int waves_of_queries() { return (DP == 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
-template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP >= 96 ? 1 : 2) : DP == 32 ? 3 : DP == 128 ? 1 : 2; }
+template <typename T, int DP> constexpr int waves_of_queries() { return (DP <= 32 ? 4 : DP == 64 ? 3 : 2) - (sizeof(T) == 4 ? 1 : 0); }
+template <typename T, int DP> constexpr int waves_of_keys() { return sizeof(T) == 4 ? (DP >= 96 ? 1 : 2) : DP <= 32 ? 3 : DP == 128 ? 1 : 2; }
 
 // 16 bytes a lane from a buffer to LDS, one lane's behind the other's from `to` on (the same for all lanes).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *to, unsigned offset) {
@@ -88,8 +90,8 @@ __device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int part
 // (of the probabilities as rounded for it, so that a row's weights add up to one).
 template <typename T, int DP, int NW, bool PARTS, bool ONES>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_attention_kernel(const AttentionArgs a) {
-  constexpr int NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
-  using Rows = RowTile<T, DP>;
+  constexpr int W = tile_width<DP>(), NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
+  using Rows = RowTile<T, W>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
@@ -120,9 +122,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   const int whole = min(end, a.causal ? token_of(wave * 32) + ahead + 1 : k_count);
   const int wave_end = same_for_all(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
 
-  Stager<T, DP, NK, NW> k;
+  Stager<T, W, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
-  Stager<T, DP, NK, NW, ONES> v;
+  Stager<T, W, NK, NW, ONES> v;
   v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
   if (begin < end) {
     k.load(k_tile0, begin, k_count, wave);
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   // of the scores so far, times `by`: a number that none exceeds by more than kSlack, -inf before the first (and what is subtracted from them)
   constexpr float kSlack = 8.f;
   float most = -inf, base = 0.f, sum = 0.f;
-  float16v o[DP / 32] = {};
+  float16v o[W / 32] = {};
   // KB blocks of 32 keys, all seen by all rows or not
   const auto take = [&](auto blocks, auto masked, const int4v *k_tile, const int4v *v_tile, int j) __attribute__((always_inline)) {
     constexpr int KB = decltype(blocks)::value;
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
       base = mine ? top : base;
       if constexpr (!ONES) sum *= keep;
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) o[db] *= keep;
+      for (int db = 0; db < W / 32; ++db) o[db] *= keep;
     }
     float add[2] = {0.f, 0.f};
 #pragma unroll
@@ -188,7 +190,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
       }
     if constexpr (!ONES) sum += add[0] + add[1];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) add_weighted_rows<T, DP>(o, rows_at, v_tile, kb * 32, s[kb]);
+    for (int kb = 0; kb < KB; ++kb) add_weighted_rows<T, W>(o, rows_at, v_tile, kb * 32, s[kb]);
   };
   const auto load_next = [&](int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
     tiles_ready();
@@ -226,17 +228,17 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   }
 
   // (the last column's products: row 31 of the last block, register 15 of the upper lanes)
-  sum = ONES ? of_upper(o[DP / 32 - 1][15]) : both_sum(sum);
+  sum = ONES ? of_upper(o[W / 32 - 1][15]) : both_sum(sum);
   const bool none = seen <= begin || end <= begin;      // no key for this row (here)
   const float inverse = none ? 0.f : 1.f / sum;
   const float lse = none ? -inf : (base + __builtin_log2f(sum)) * (1.f / kLog2e);
   if constexpr (PARTS) {
     const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
-    if (mine && !none) store_row<T, float, DP>(a.part_sum + tile * a.dim, o, inverse, a.dim, lane);
+    if (mine && !none) store_row<T, float, W>(a.part_sum + tile * a.dim, o, inverse, a.dim, lane);
     if (mine && lane < 32) a.part_lse[tile] = lse;
   } else if (mine) {
     const int64_t to = (int64_t)(slot.begin + token) * a.heads + head;
-    store_row<T, T, DP>((T *)a.out + to * a.dim, o, inverse, a.dim, lane);
+    store_row<T, T, W>((T *)a.out + to * a.dim, o, inverse, a.dim, lane);
     if (a.lse && lane < 32) a.lse[to] = lse;
   }
 }
@@ -346,8 +348,8 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T *__restric
 // and ds the right operand of dq^T = k^T ds as it stands.
 template <typename T, int DP, int NW, bool PARTS>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attention_query_grad_kernel(const AttentionArgs a) {
-  constexpr int NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
-  using Rows = RowTile<T, DP>;
+  constexpr int W = tile_width<DP>(), NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
+  using Rows = RowTile<T, W>;
   __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
@@ -377,9 +379,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   const int whole = min(end, a.causal ? token_of(wave * 32) + ahead + 1 : k_count);
   const int wave_end = same_for_all(!awake ? begin : a.causal ? min(end, token_of(wave_last) + ahead + 1) : end);
 
-  Stager<T, DP, NK, NW> k;
+  Stager<T, W, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
-  Stager<T, DP, NK, NW> v;
+  Stager<T, W, NK, NW> v;
   v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
   if (begin < end) {
     k.load(k_tile0, begin, k_count, wave);
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   if (mine && lane < 32 && (!PARTS || at.part == 0)) a.delta[to] = delta;      // (for the keys' gradients)
 
   const float by = a.scale * kLog2e;
-  float16v dq[DP / 32] = {};
+  float16v dq[W / 32] = {};
   const auto take = [&](auto masked, const int4v *k_tile, const int4v *v_tile, int kb, int j) __attribute__((always_inline)) {
     float16v s = {}, dp = {};
 #pragma unroll
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = left > 8 * (r / 4) + r % 4 ? s[r] : 0.f;
     }
-    add_weighted_rows<T, DP>(dq, rows_at, k_tile, kb * 32, s);
+    add_weighted_rows<T, W>(dq, rows_at, k_tile, kb * 32, s);
   };
   const auto load_next = [&](int4v *k_next, int4v *v_next, int j) __attribute__((always_inline)) {
     tiles_ready();
@@ -451,9 +453,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   const float scale = a.scale * pow2(-ds_shift<T>());
   if constexpr (PARTS) {
     const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
-    if (mine) store_row<T, float, DP>(a.part_sum + tile * a.dim, dq, scale, a.dim, lane);
+    if (mine) store_row<T, float, W>(a.part_sum + tile * a.dim, dq, scale, a.dim, lane);
   } else if (mine) {
-    store_row<T, T, DP>((T *)a.gq + to * a.dim, dq, scale, a.dim, lane);
+    store_row<T, T, W>((T *)a.gq + to * a.dim, dq, scale, a.dim, lane);
   }
 }
 
@@ -461,8 +463,8 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
 // dk^T = q^T ds, dv^T = g_out^T p take ds and p as they stand.
 template <typename T, int DP, int NW, bool PARTS>
 __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_key_grad_kernel(const AttentionArgs a) {
-  constexpr int NQ = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
-  using Rows = RowTile<T, DP>;
+  constexpr int W = tile_width<DP>(), NQ = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
+  using Rows = RowTile<T, W>;
   constexpr int PER = NQ * Rows::CH / (64 * NW);
   __shared__ int4v q_tile0[NQ * Rows::CH], g_tile0[NQ * Rows::CH], q_tile1[NQ * Rows::CH], g_tile1[NQ * Rows::CH];
   __shared__ float4v lse_tile0[NQ / 4], delta_tile0[NQ / 4], lse_tile1[NQ / 4], delta_tile1[NQ / 4];
@@ -557,7 +559,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   load_row<T, DP>(k, mine ? (const T *)a.k + (slot.begin + key) * a.k_row + at.kv_head * a.k_head : nullptr, a.dim, lane);
   load_row<T, DP>(v, mine ? (const T *)a.v + (slot.begin + key) * a.v_row + at.kv_head * a.v_head : nullptr, a.dim, lane);
   const float by = a.scale * kLog2e;
-  float16v dk[DP / 32] = {}, dv[DP / 32] = {};
+  float16v dk[W / 32] = {}, dv[W / 32] = {};
   const auto take = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
                         int r0) __attribute__((always_inline)) {
     float16v p = {}, ds = {};
@@ -590,9 +592,9 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
       }
     }
     phase();
-    add_weighted_rows<T, DP>(dv, rows_at, g_tile, qb * 32, p);
+    add_weighted_rows<T, W>(dv, rows_at, g_tile, qb * 32, p);
     phase();
-    add_weighted_rows<T, DP>(dk, rows_at, q_tile, qb * 32, ds);
+    add_weighted_rows<T, W>(dk, rows_at, q_tile, qb * 32, ds);
   };
   const auto all_of = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int4v *q_next, int4v *g_next,
                           float4v *lse_next, float4v *delta_next, int r0) __attribute__((always_inline)) {
@@ -645,12 +647,12 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   if constexpr (PARTS) {
     const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
     const int64_t all = (int64_t)a.slots * a.kv_heads * a.parts * T_ROWS * a.dim;
-    store_row<T, float, DP>(a.part_sum + tile * a.dim, dk, k_by, a.dim, lane);
-    store_row<T, float, DP>(a.part_sum + all + tile * a.dim, dv, v_by, a.dim, lane);
+    store_row<T, float, W>(a.part_sum + tile * a.dim, dk, k_by, a.dim, lane);
+    store_row<T, float, W>(a.part_sum + all + tile * a.dim, dv, v_by, a.dim, lane);
   } else {
     const int64_t to = ((int64_t)(slot.begin + key) * a.kv_heads + at.kv_head) * a.dim;
-    if (a.gk) store_row<T, T, DP>((T *)a.gk + to, dk, k_by, a.dim, lane);
-    if (a.gv) store_row<T, T, DP>((T *)a.gv + to, dv, v_by, a.dim, lane);
+    if (a.gk) store_row<T, T, W>((T *)a.gk + to, dk, k_by, a.dim, lane);
+    if (a.gv) store_row<T, T, W>((T *)a.gv + to, dv, v_by, a.dim, lane);
   }
 }
 
@@ -769,9 +771,9 @@ int by_waves(int waves, F f) {
 template <typename T, int DP>
 int forward_any(const AttentionArgs &a) {
   return by_waves(waves_for((int64_t)a.n_q * (a.heads / a.kv_heads), a.segments), [&](auto w) {
-    if constexpr (sizeof(T) == 2)
-      if (a.dim < DP) return forward<T, DP, decltype(w)::value, true>(a);
-    return forward<T, DP, decltype(w)::value, false>(a);
+    if constexpr (DP < 32) return forward<T, DP, decltype(w)::value, true>(a);
+    else if constexpr (sizeof(T) == 4) return forward<T, DP, decltype(w)::value, false>(a);
+    else return a.dim < DP ? forward<T, DP, decltype(w)::value, true>(a) : forward<T, DP, decltype(w)::value, false>(a);
   });
 }
 
@@ -796,11 +798,15 @@ int backward_any(const AttentionArgs &a) {
 
 template <typename T>
 int attention_fwd(const AttentionArgs &a) {
+  if constexpr (sizeof(T) == 2)
+    if (a.dim <= 16) return forward_any<T, 16>(a);
   return a.dim <= 32 ? forward_any<T, 32>(a) : a.dim <= 64 ? forward_any<T, 64>(a) : a.dim <= 96 ? forward_any<T, 96>(a) : forward_any<T, 128>(a);
 }
 
 template <typename T>
 int attention_bwd(const AttentionArgs &a) {
+  if constexpr (sizeof(T) == 2)
+    if (a.dim <= 16) return backward_any<T, 16>(a);
   return a.dim <= 32 ? backward_any<T, 32>(a) : a.dim <= 64 ? backward_any<T, 64>(a) : a.dim <= 96 ? backward_any<T, 96>(a) : backward_any<T, 128>(a);
 }
 

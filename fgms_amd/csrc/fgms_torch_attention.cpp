@@ -12,7 +12,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
-#include <cmath>
+#include <algorithm>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -61,11 +61,13 @@ void refuse_tangent(const at::Tensor &t, const char *op, const char *name) {
 }
 
 // [rows, heads, channels] as the kernels read it: the channels of a head side by side, every head of a row on 16 bytes.
-// Slices of one projection and expanded tensors are taken as they lie; anything else is copied.
-at::Tensor by_rows(const at::Tensor &t) {
-  const int64_t size = t.element_size();
-  const bool fits = t.stride(2) == 1 && t.stride(0) * size % 16 == 0 && t.stride(1) * size % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+// Slices of one projection and heads expanded from one are taken as they lie; anything else is copied.  (A tile's rows are reached
+// by 32-bit offsets, rows of keys and values end where the next begins or before: see fgms_segment_attention_fwd's checks.)
+at::Tensor by_rows(const at::Tensor &t, int64_t group = 1) {
+  const int64_t size = t.element_size(), row = t.size(0) > 1 ? t.stride(0) : t.size(2), head = t.size(1) > 1 ? t.stride(1) : t.size(2);
+  const bool fits = t.stride(2) == 1 && row * size % 16 == 0 && head * size % 16 == 0 && t.stride(0) * size % 16 == 0 &&
+                    t.stride(1) * size % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row >= t.size(2) &&
+                    row * size <= 16 << 20 && t.stride(0) * size <= 16 << 20 && t.stride(1) * size * group <= 512 << 20;
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 // ... and a tensor that has to be contiguous.
@@ -232,7 +234,7 @@ struct SegmentAttentionBackward final : public torch::autograd::Node {
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x[0].device());
     at::Tensor gx[3];
     for (int i = 0; i < 3; ++i) {
-      x[i] = by_rows(x[i]);
+      x[i] = by_rows(x[i], i ? 1 : x[0].size(1) / std::max<int64_t>(x[1].size(1), 1));
       if (task_should_compute_output(i)) gx[i] = result(x[i].sizes(), x[i]);
     }
     o = packed(o);
@@ -281,7 +283,7 @@ at::Tensor segment_attention_node(const at::Tensor &q, const at::Tensor &k, cons
   {
     at::AutoGradMode no_grad(false);
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-    x[0] = by_rows(q), x[1] = by_rows(k), x[2] = by_rows(v);
+    x[0] = by_rows(q, q.size(1) / std::max<int64_t>(k.size(1), 1)), x[1] = by_rows(k), x[2] = by_rows(v);
     out = result(q.sizes(), q);
     if (wants_grad) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false));
     check(fgms_segment_attention_fwd(data(x[0]), data(x[1]), data(x[2]), data(out), (float *)data(lse), ints(q_offsets), ints(k_offsets),

@@ -294,3 +294,30 @@ def test_empty_sizes():
             out = nn.segment_attention(*x, U.offsets([0] * len(lengths)), U.offsets(lengths))
             assert out.shape == (0, 2, 16)
             assert not any(t.any() for t in torch.autograd.grad(out, x, k))
+
+
+def test_layouts_that_are_copied():
+    """Keys expanded over rows, rows that overlap, and heads too far apart for a tile's offsets give what copies of them give."""
+    from FGMS import nn
+    torch.manual_seed(11)
+    at, d = U.offsets([50, 30]), 32
+    q, v = torch.randn(80, 4, d, device="cuda").half(), torch.randn(80, 2, d, device="cuda").half()
+    same = torch.randn(1, 2, d, device="cuda").half().expand(80, -1, -1)
+    sliding = torch.randn(80 * 16 + 64, device="cuda").half().as_strided((80, 2, d), (16, 32, 1))
+    for k in (same, sliding):
+        for x in ((q, k, v), (q, v, k)):
+            want = U.attention(*x, [50, 30], [50, 30], True, 1 / math.sqrt(d), q)
+            leaves = [t.detach().requires_grad_() for t in x]
+            out = nn.segment_attention(*leaves, at, causal=True)
+            U.within(out, want.out, want.out_off, "out")
+            for n, g in zip(("gq", "gk", "gv"), torch.autograd.grad(out, leaves, q)):
+                U.within(g, getattr(want, n), getattr(want, n + "_off"), n)
+    apart = torch.zeros(4, (300 << 20) // 2, dtype=torch.float16, device="cuda")[:, :80 * d].unflatten(1, (80, d)).transpose(0, 1)
+    apart.copy_(q)
+    k, v = torch.randn(2, 80, 1, d, device="cuda").half()
+    leaves = [apart.requires_grad_(), k.requires_grad_(), v.requires_grad_()]
+    out = nn.segment_attention(*leaves, at)
+    want = U.attention(q, k, v, [50, 30], [50, 30], False, 1 / math.sqrt(d), q)
+    U.within(out, want.out, want.out_off, "out")
+    for n, g in zip(("gq", "gk", "gv"), torch.autograd.grad(out, leaves, q)):
+        U.within(g, getattr(want, n), getattr(want, n + "_off"), n)
