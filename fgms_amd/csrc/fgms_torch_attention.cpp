@@ -30,9 +30,11 @@ void check(int rc) {
   throw std::runtime_error(fgms_last_error());
 }
 
-void need(bool ok, const std::string &what) {
-  if (!ok) throw std::invalid_argument(what);
-}
+// (the message is only put together where it is wanted: a small call takes six microseconds)
+#define FGMS_NEED(ok, what) \
+  do {                      \
+    if (!(ok)) throw std::invalid_argument(what); \
+  } while (0)
 
 int dtype_of(const at::Tensor &t) {
   switch (t.scalar_type()) {
@@ -44,15 +46,15 @@ int dtype_of(const at::Tensor &t) {
 }
 
 void need_features(const at::Tensor &t, const at::Tensor &like, const char *name) {
-  need(t.is_cuda(), std::string(name) + " must be a GPU tensor");
-  need(t.device() == like.device(), std::string(name) + " must be on the device of q");
-  need(t.scalar_type() == like.scalar_type(), std::string(name) + " must have the dtype of q");
+  FGMS_NEED(t.is_cuda(), std::string(name) + " must be a GPU tensor");
+  FGMS_NEED(t.device() == like.device(), std::string(name) + " must be on the device of q");
+  FGMS_NEED(t.scalar_type() == like.scalar_type(), std::string(name) + " must have the dtype of q");
 }
 
 void need_ints(const at::Tensor &t, const at::Tensor &like, int dims, const char *name) {
-  need(t.scalar_type() == at::ScalarType::Int && t.is_cuda() && t.is_contiguous() && t.dim() == dims,
+  FGMS_NEED(t.scalar_type() == at::ScalarType::Int && t.is_cuda() && t.is_contiguous() && t.dim() == dims,
        std::string(name) + " must be a contiguous int32 tensor of " + std::to_string(dims) + " dimension(s) on the GPU");
-  need(t.device() == like.device(), std::string(name) + " must be on the device of q");
+  FGMS_NEED(t.device() == like.device(), std::string(name) + " must be on the device of q");
 }
 
 void refuse_tangent(const at::Tensor &t, const char *op, const char *name) {
@@ -129,7 +131,7 @@ struct NormRotaryBackward final : public torch::autograd::Node {
       if (w[i].defined()) w[i] = packed(w[i]);
       // (no gradient reaches this output: its part of all sums is zero)
       g[i] = grads[i].defined() ? packed(grads[i]) : at::zeros(x[i].sizes(), x[i].options().requires_grad(false));
-      need(g[i].scalar_type() == x[i].scalar_type(), "the output gradient must have the dtype of q");
+      FGMS_NEED(g[i].scalar_type() == x[i].scalar_type(), "the output gradient must have the dtype of q");
       if (task_should_compute_output(i)) gx[i] = result(x[i].sizes(), x[i]);
       if (w[i].defined() && task_should_compute_output(2 + i)) gw[i] = result(w[i].sizes(), w[i]);
     }
@@ -154,7 +156,7 @@ std::tuple<at::Tensor, at::Tensor> norm_rotary_node(const at::Tensor &q, const a
                                                     const at::Tensor &freqs, at::IntArrayRef sections, double eps, bool interleaved) {
   static const char op[] = "norm_rotary";
   const at::Tensor scale[2] = {q_scale_.value_or(at::Tensor()), k_scale_.value_or(at::Tensor())};
-  need(q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2),
+  FGMS_NEED(q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2),
        "expected q [N, heads, D] and k [N, key heads, D]");
   need_features(q, q, "q");
   need_features(k, q, "k");
@@ -162,23 +164,23 @@ std::tuple<at::Tensor, at::Tensor> norm_rotary_node(const at::Tensor &q, const a
   for (const at::Tensor &s : scale)
     if (s.defined()) {
       need_features(s, q, "a scale");
-      need(s.dim() == 1 && s.size(0) == q.size(2), "a scale must have one value for each channel of a head");
+      FGMS_NEED(s.dim() == 1 && s.size(0) == q.size(2), "a scale must have one value for each channel of a head");
     }
   need_ints(coords, q, 2, "coords");
-  need(coords.size(0) == q.size(0) && coords.size(1) == (int64_t)sections.size(),
+  FGMS_NEED(coords.size(0) == q.size(0) && coords.size(1) == (int64_t)sections.size(),
        "coords must be [N, axes], with one of the sections for each axis");
   int64_t pairs = 0;
   Turn turn{coords, freqs, {}, eps, interleaved};
   for (int64_t s : sections) {
-    need(s >= 0 && s <= 64, "a section must be between 0 and half the channels of a head");
+    FGMS_NEED(s >= 0 && s <= 64, "a section must be between 0 and half the channels of a head");
     turn.sections.push_back((int)s);
     pairs += s;
   }
-  need(freqs.scalar_type() == at::ScalarType::Float && freqs.is_cuda() && freqs.device() == q.device() && freqs.is_contiguous() &&
+  FGMS_NEED(freqs.scalar_type() == at::ScalarType::Float && freqs.is_cuda() && freqs.device() == q.device() && freqs.is_contiguous() &&
            freqs.dim() == 1 && freqs.size(0) == pairs,
        "freqs must be a contiguous float32 tensor on the device of q, with a value for each pair of the sections");
   const bool grad_mode = at::GradMode::is_enabled();
-  need(!(grad_mode && freqs.requires_grad()), "norm_rotary forms no gradient of freqs");
+  FGMS_NEED(!(grad_mode && freqs.requires_grad()), "norm_rotary forms no gradient of freqs");
   refuse_tangent(q, op, "q");
   refuse_tangent(k, op, "k");
   refuse_tangent(freqs, op, "freqs");
@@ -240,7 +242,7 @@ struct SegmentAttentionBackward final : public torch::autograd::Node {
     o = packed(o);
     l = packed(l);
     const at::Tensor g = packed(grads[0]);
-    need(g.scalar_type() == x[0].scalar_type(), "the output gradient must have the dtype of q");
+    FGMS_NEED(g.scalar_type() == x[0].scalar_type(), "the output gradient must have the dtype of q");
     check(fgms_segment_attention_bwd(data(g), data(x[0]), data(x[1]), data(x[2]), data(o), (const float *)data(l), data(gx[0]), data(gx[1]),
                                      data(gx[2]), ints(segments.q_offsets), ints(segments.k_offsets), x[0].size(0), x[1].size(0),
                                      (int)segments.q_offsets.numel() - 1, (int)x[0].size(1), (int)x[1].size(1), (int)x[0].size(2),
@@ -261,7 +263,7 @@ at::Tensor segment_attention_node(const at::Tensor &q, const at::Tensor &k, cons
                                   const at::Tensor &k_offsets, const c10::optional<at::Tensor> &k_lengths_, bool causal, double scale) {
   static const char op[] = "segment_attention";
   const at::Tensor k_lengths = k_lengths_.value_or(at::Tensor());
-  need(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && q.size(2) == k.size(2),
+  FGMS_NEED(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && q.size(2) == k.size(2),
        "expected q [Nq, heads, D], k and v [Nk, key heads, D]");
   need_features(q, q, "q");
   need_features(k, q, "k");
@@ -269,13 +271,13 @@ at::Tensor segment_attention_node(const at::Tensor &q, const at::Tensor &k, cons
   const int dtype = dtype_of(q);
   need_ints(q_offsets, q, 1, "q_offsets");
   need_ints(k_offsets, q, 1, "k_offsets");
-  need(q_offsets.numel() >= 1 && q_offsets.numel() == k_offsets.numel(), "q_offsets and k_offsets must have one more entry than there are segments");
+  FGMS_NEED(q_offsets.numel() >= 1 && q_offsets.numel() == k_offsets.numel(), "q_offsets and k_offsets must have one more entry than there are segments");
   if (k_lengths.defined()) {
     need_ints(k_lengths, q, 1, "k_lengths");
-    need(k_lengths.numel() == q_offsets.numel() - 1, "k_lengths must have an entry for each segment");
+    FGMS_NEED(k_lengths.numel() == q_offsets.numel() - 1, "k_lengths must have an entry for each segment");
   }
   const bool wants_grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
-  need(!(wants_grad && k_lengths.defined()), "segment_attention forms no gradients over caches (k_lengths)");
+  FGMS_NEED(!(wants_grad && k_lengths.defined()), "segment_attention forms no gradients over caches (k_lengths)");
   refuse_tangent(q, op, "q");
   refuse_tangent(k, op, "k");
   refuse_tangent(v, op, "v");

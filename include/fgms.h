@@ -326,8 +326,10 @@ int fgms_norm_rotary_bwd(const void *q_out_grad, const void *k_out_grad,
  * Few queries over many keys (a new row and its cache) are cut along the keys, in a workspace of the stream.
  * The backward call forms the probabilities again from q, k and lse; it writes the gradients whose pointers
  * are not NULL, sums over the heads of a group included.  No atomics: the same bits every time.
- * Values of v that are infinite or NaN reach rows that see them, and with `causal` may turn other rows of the
- * same segment into NaN.
+ * Infinities and NaN in v reach the rows that see them, and with `causal` may turn up to 63 rows before those into NaN;
+ * keys that a row does not see may hold anything.
+ * Rows of k and v must not overlap, rows of any tensor lie at most 16 MB and the heads of a group 512 MB apart; n_k, and n_q
+ * times the heads of a group, at most 2^31 - 2^25.
  */
 int fgms_segment_attention_fwd(const void *q, const void *k, const void *v, void *out, float *lse,
                                const int32_t *q_offsets, const int32_t *k_offsets, const int32_t *k_lengths,

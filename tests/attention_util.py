@@ -1,14 +1,26 @@
 """Plain attention inside segments and plain norms with rotation, in 64 bits on the CPU, with how far a kernel's results
 may be off: each rounding of the kernels (to the inputs' type, of an fp32 sum) carried through the formulas."""
+import ctypes
 import math
 from types import SimpleNamespace
 
 import torch
 
+from fgms_amd import capi
+
 DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
 UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}      # half a step
 TINY = {torch.float16: 2.0 ** -24, torch.bfloat16: 0.0, torch.float32: 0.0}                   # fp16's last step
 SUM = 2.0 ** -24
+
+
+def own_stream():
+    """A stream of the caller's own, not one of torch's pool (made through the runtime that the library is linked to)."""
+    runtime = ctypes.CDLL(capi.LIB_PATH)
+    runtime.hipStreamCreateWithFlags.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_uint]
+    handle = ctypes.c_void_p()
+    assert runtime.hipStreamCreateWithFlags(ctypes.byref(handle), 1) == 0      # hipStreamNonBlocking
+    return torch.cuda.ExternalStream(handle.value)
 
 
 def offsets(lengths, device="cuda"):

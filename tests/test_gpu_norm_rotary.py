@@ -137,7 +137,7 @@ def test_streams_and_graphs():
         return tuple(t.detach() for t in out) + torch.autograd.grad(out, leaves, (gq, gk))
 
     want = step()
-    side = torch.cuda.Stream()
+    side = U.own_stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         got = step()

@@ -242,7 +242,7 @@ def test_streams_and_graphs():
         return (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)
 
     want = step()
-    side = torch.cuda.Stream()
+    side = U.own_stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         got = step()
