@@ -32,9 +32,16 @@ struct Stager {
   const char *base;
   int64_t stride;              // bytes
   unsigned offset[PER];
-  __device__ __forceinline__ void open(const T *from, int64_t row_stride, int dim, int wave, int lane) {
+  // (`like`: the other tensor's, whose lanes ask for the same places if its rows lie as far apart)
+  template <bool K2 = KEEP>
+  __device__ __forceinline__ void open(const T *from, int64_t row_stride, int dim, int wave, int lane, const Stager<T, DP, ROWS, NW, K2> *like = nullptr) {
     base = (const char *)from;
     stride = row_stride * (int)sizeof(T);
+    if (like && like->stride == stride) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) offset[i] = like->offset[i];
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = (wave + i * NW) * 64 + lane, row = e / Rows::CH, c = (e % Rows::CH) ^ Rows::swizzle(row);
@@ -89,9 +96,8 @@ __device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int part
 // the values' last column then holds ones, and the rows' sums come out of the second product, a sixth of the vector instructions less
 // (of the probabilities as rounded for it, so that a row's weights add up to one).
 // 16/4 heads of 128, two causal scans of 24 k rows together, bf16: 1.38 ms, 1.10 PFLOP/s where a large library product reaches 1.14; 16
-// heads of 64 over 12 k rows 142 us, 815 TFLOP/s: a score costs its wave 28 cycles of vector instructions (an exponential takes
-// two turns), its products 16, and the two do not overlap on a SIMD.  Windows of 160 voxels on average, 4 heads of 16, 200 k voxels: 64 us, 20
-// for its bytes.
+// heads of 64 over 12 k rows 142 us, 815 TFLOP/s: the vector pipe is busy 75 % of the time, the matrix pipe 46 % (heads of 128: 54 % and
+// 64 %; an exponential takes two turns).  Windows of 160 voxels on average, 4 heads of 16, 200 k voxels: 62 us, 20 for its bytes.
 template <typename T, int DP, int NW, bool PARTS, bool ONES>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_attention_kernel(const AttentionArgs a) {
   constexpr int W = tile_width<DP>(), NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
@@ -129,7 +135,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   Stager<T, W, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
   Stager<T, W, NK, NW, ONES> v;
-  v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
+  v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane, &k);
   if (begin < end) {
     k.load(k_tile0, begin, k_count, wave);
     v.load(v_tile0, begin, k_count, wave);
@@ -137,11 +143,8 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   if constexpr (ONES) {
     // (chunks behind the channels: zeros, and a one at the end of a row; no load touches them)
     const int4v last = {0, 0, 0, (int)((unsigned)__builtin_bit_cast(unsigned short, (T)1.f) << 16)};
-    for (int e = threadIdx.x; e < NK * Rows::CH; e += 64 * NW) {
-      const int row = e / Rows::CH, c = e % Rows::CH;
-      if (c * Rows::E < a.dim) continue;
-      v_tile0[Rows::at(row, c)] = v_tile1[Rows::at(row, c)] = c == Rows::CH - 1 ? last : int4v{0, 0, 0, 0};
-    }
+    for (int row = threadIdx.x; row < NK; row += 64 * NW)
+      for (int c = a.dim / Rows::E; c < Rows::CH; ++c) v_tile0[Rows::at(row, c)] = v_tile1[Rows::at(row, c)] = c == Rows::CH - 1 ? last : int4v{0, 0, 0, 0};
   }
   int4v q[STEPS];
   load_row<T, DP>(q, mine ? (const T *)a.q + (slot.begin + token) * a.q_row + head * a.q_head : nullptr, a.dim, lane);
@@ -388,7 +391,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   Stager<T, W, NK, NW> k;
   k.open((const T *)a.k + k_begin * a.k_row + at.kv_head * a.k_head, a.k_row, a.dim, wave, lane);
   Stager<T, W, NK, NW> v;
-  v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane);
+  v.open((const T *)a.v + k_begin * a.v_row + at.kv_head * a.v_head, a.v_row, a.dim, wave, lane, &k);
   if (begin < end) {
     k.load(k_tile0, begin, k_count, wave);
     v.load(v_tile0, begin, k_count, wave);
