@@ -89,6 +89,8 @@ AttentionArgs attention_args(const void *q, const void *k, const void *v, const 
   a.q_offsets = q_offsets, a.k_offsets = k_offsets, a.k_lengths = k_lengths;
   a.n_q = (int)n_q, a.n_k = (int)n_k, a.segments = segments, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  // (a single row may carry any stride, 0 where it was expanded; the kernels end a row of k and v where its stride does)
+  if (n_k == 1) a.k_row = a.v_row = dim;
   a.causal = causal, a.scale = scale, a.dtype = dtype, a.stream = (hipStream_t)stream, a.parts = 1;
   return a;
 }
