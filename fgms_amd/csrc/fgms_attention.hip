@@ -140,7 +140,7 @@ extern "C" int fgms_norm_rotary_bwd(const void *q_out_grad, const void *k_out_gr
                                       axes, sections, interleaved, eps, dtype, stream);
   const int rc = check_norm_rotary(what, a);
   if (rc != FGMS_OK) return rc;
-  a.gscale[0] = q_scale_grad, a.gscale[1] = k_heads > 0 ? k_scale_grad : nullptr;
+  a.gscale[0] = q_scale_grad, a.gscale[1] = k_scale_grad;      // (without key heads: zeros)
   if (n == 0) {
     const size_t bytes = (size_t)head_dim * element_bytes(dtype);
     int filled = FGMS_OK;
