@@ -46,7 +46,24 @@ struct WsBuf {
 };
 std::mutex g_ws_mutex;
 std::map<WsKey, WsBuf> g_ws;
+std::map<std::pair<int, hipStream_t>, std::mutex> g_turns;      // (never erased: whoever waits for one has its address)
 }  // namespace
+
+StreamTurn::StreamTurn(hipStream_t stream) : mutex_(nullptr) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return;      // (the look-up reports it)
+  std::mutex *turn;
+  {
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    turn = &g_turns[{dev, stream}];
+  }
+  turn->lock();
+  mutex_ = turn;
+}
+
+StreamTurn::~StreamTurn() {
+  if (mutex_) static_cast<std::mutex *>(mutex_)->unlock();
+}
 
 bool is_capturing(hipStream_t stream) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;

@@ -195,6 +195,7 @@ int launch_attention_fwd(AttentionArgs a) {
 }
 
 int launch_attention_bwd(AttentionArgs a) {
+  const StreamTurn turn(a.stream);
   const int rc = workspace_get(a.stream, kSlotAttentionDelta, (size_t)a.n_q * a.heads * sizeof(float), (void **)&a.delta);
   if (rc != FGMS_OK) return rc;
   return a.dtype == FGMS_F32 ? attention_bwd<float>(a) : a.dtype == FGMS_F16 ? attention_bwd<_Float16>(a) : attention_bwd<__bf16>(a);

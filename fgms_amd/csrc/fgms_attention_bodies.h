@@ -729,6 +729,7 @@ int forward(AttentionArgs a) {
     segment_attention_kernel<T, DP, NW, false, ONES><<<grid, NW * 64, 0, a.stream>>>(a);
     return launched("segment attention");
   }
+  const StreamTurn turn(a.stream);
   const size_t rows = (size_t)tiles * a.parts * 32 * NW;
   rc = workspace_get(a.stream, kSlotAttention, rows * (a.dim + 1) * sizeof(float), (void **)&a.part_sum);
   if (rc != FGMS_OK) return rc;

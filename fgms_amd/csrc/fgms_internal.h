@@ -232,6 +232,18 @@ bool is_capturing(hipStream_t stream);   // into a HIP graph
 // *fresh (optional) is set when the buffer was (re)allocated by this call.
 constexpr int kSlotAttention = 9, kSlotAttentionDelta = 10, kSlotScaleSums = 11;
 int workspace_get(hipStream_t stream, int slot, size_t bytes, void **ptr, bool *fresh = nullptr);
+// A call whose launches hand something over in a workspace has the stream to itself from the look-up to its last launch: another thread's
+// call on the stream would else write the buffer between two of them, or grow it, which gives the old one back.
+class StreamTurn {
+ public:
+  explicit StreamTurn(hipStream_t stream);
+  ~StreamTurn();
+  StreamTurn(const StreamTurn &) = delete;
+  StreamTurn &operator=(const StreamTurn &) = delete;
+
+ private:
+  void *mutex_;
+};
 // Buffer for a re-laid copy of a.w in `layout` (any number that tells the layouts of one weight
 // tensor apart): the stream's workspace, to be filled (*fill = true), or -- for weights under
 // fgms_weights_pin -- a kept copy that a first call fills (relaid_weights_filled once its fill

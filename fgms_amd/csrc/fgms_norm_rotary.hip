@@ -6,6 +6,8 @@
 // with inputs that change, 40 at the rate of a copy; 120 k rows of 4 + 4 heads of 32, fp16: 25 us forward, 41 + 3.5 back.)
 #include "fgms_norm_rotary.h"
 
+#include <optional>
+
 #include "fgms_internal.h"
 #include "fgms_mma.h"
 
@@ -208,6 +210,8 @@ int launch(const NormRotaryArgs &a) {
   float *partial = nullptr;
   size_t lds = (size_t)tile * (a.dim / 2) * sizeof(float2);
   const bool scales = BACKWARD && (a.gscale[0] || a.gscale[1]);
+  std::optional<StreamTurn> turn;
+  if (scales) turn.emplace(a.stream);
   if (BACKWARD) {
     const int64_t most = 4 * num_cus();      // (each leaves sums behind)
     blocks = blocks < most ? blocks : most;
