@@ -1073,6 +1073,7 @@ int backward(const void *out_feats_grad, const void *in_feats, const void *kerne
   const Plan *p = plan_resolve(plan, stream, &rc);
   CheckFlush flush{p, stream};
   if (rc) return rc;
+  const StreamTurn turn(stream);
   GmsArgs d{};
   d.src = out_feats_grad; d.w = kernel; d.dst = in_feats_grad; d.kpos = kpos;
   d.gmap = out_map; d.smap = in_map;   // roles swap, as at backend/spconv.cu:460,559
@@ -1165,6 +1166,7 @@ int fgms_fusion_fwd(const void *in_feats, const void *kernel, int sum_nnz, void 
   const Plan *p = plan_resolve(plan, s, &rc);
   CheckFlush flush{p, s};
   if (rc) return rc;
+  const StreamTurn turn(s);
   return run_gms(a, p);
 }
 
@@ -1204,6 +1206,7 @@ int fgms_fwd(const void *in_feats, const void *kernel, int sum_nnz, void *out_fe
   const Plan *p = plan_resolve(plan, s, &rc);
   CheckFlush flush{p, s};
   if (rc) return rc;
+  const StreamTurn turn(s);
   if (separate_mid) a.centre = mid_of(k_vol) + 1;
   return run_gms(a, p);
 }
@@ -1224,6 +1227,7 @@ int fgms_dgrad(const void *out_feats_grad, const void *kernel, void *in_feats_gr
   const Plan *p = plan_resolve(plan, a.stream, &rc);
   CheckFlush flush{p, a.stream};
   if (rc) return rc;
+  const StreamTurn turn(a.stream);
   return run_gms(a, p);
 }
 
@@ -1242,6 +1246,7 @@ int fgms_wgrad(const void *in_feats, const void *out_feats_grad, void *kernel_gr
   a.plan = plan_resolve(plan, a.stream, &rc);
   CheckFlush flush{a.plan, a.stream};
   if (rc) return rc;
+  const StreamTurn turn(a.stream);
   return run_wgrad(a);
 }
 
@@ -1287,6 +1292,7 @@ int fgms_conv_fwd(const void *in_feats, const void *kernel, void *out_feats, con
   const Plan *p = plan_resolve(plan, s, &rc);
   CheckFlush flush{p, s};
   if (rc) return rc;
+  const StreamTurn turn(s);
   return run_gms(a, p);
 }
 
