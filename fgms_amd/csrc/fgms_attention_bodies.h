@@ -151,8 +151,10 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
 
   const float by = a.scale * kLog2e;
   const float inf = __builtin_inff();
-  // of the scores so far, times `by`: a number that none exceeds by more than kSlack, -inf before the first (and what is subtracted from them)
-  constexpr float kSlack = 8.f;
+  // of the scores so far, times `by`: a number that none exceeds by more than kSlack, -inf before the first (and what is subtracted from them).
+  // fp16 holds the probabilities times 2^7: they grow to 2^15 within the slack, and half a step of the smallest is 2^-32 of the largest instead
+  // of 2^-25 (of 65 k keys beside one that is 2^25 times each, 0.2 % of the row).
+  constexpr float kSlack = 8.f, kUp = __is_same(T, _Float16) ? 7.f : 0.f;
   float most = -inf, base = 0.f, sum = 0.f;
   float16v o[W / 32] = {};
   // KB blocks of 32 keys, all seen by all rows or not
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
       const bool mine = top > most + kSlack;
       const float keep = mine ? __builtin_amdgcn_exp2f(most - top) : 1.f;
       most = mine ? top : most;
-      base = mine ? top : base;
+      base = mine ? top - kUp : base;
       if constexpr (!ONES) sum *= keep;
 #pragma unroll
       for (int db = 0; db < W / 32; ++db) o[db] *= keep;
