@@ -322,10 +322,48 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const AttentionArgs a, 
 // --- backward -------------------------------------------------------------------------------------------------
 // ds = p (g_out . v - delta) is rounded to T for its two products, p for its one.  In fp16 a power of two goes with them, taken out
 // of the sums again: p is 1 / N in a row of N like keys and would lose bits from 2^-14 on, with 2^10 from 2^-24 on; ds has 2^4
-// (steps of 2^-28; it may reach 4094).
+// (steps of 2^-28; it may reach 4094).  Where ds reaches further, the sums of its row (its key) come out infinite or as no number in every
+// channel; these rows alone are then formed again with 2^-11, and with 2^-26 where that is not enough, which bears the 2^40 of two
+// products of 128 channels of 65504.  (Half a step of such a row is 2^-26 of its largest ds.)
 template <typename T> constexpr int p_shift() { return __is_same(T, _Float16) ? 10 : 0; }
 template <typename T> constexpr int ds_shift() { return __is_same(T, _Float16) ? 4 : 0; }
+template <typename T> constexpr bool ds_shifted() { return ds_shift<T>() != 0; }
+constexpr int kShiftDown = 15, kLeastShift = 4 - 2 * kShiftDown;
 constexpr float pow2(int e) { return e >= 0 ? (float)(1 << e) : 1.f / (float)(1 << -e); }
+
+// Whether a lane of the workgroup says so, by way of a tile that all waves are done with when they have come here (16 bytes of their own
+// would leave room for a workgroup less on a CU).
+template <int NW>
+__device__ __forceinline__ bool any_lane(bool mine, int4v *tile) {
+  const bool here = __builtin_amdgcn_ballot_w64(mine) != 0;
+  if constexpr (NW == 1) return here;
+  int *const says = (int *)tile;
+  __syncthreads();
+  if (threadIdx.x % 64 == 0) says[threadIdx.x / 64] = here;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) any |= says[w];
+  return same_for_all(any) != 0;
+}
+
+// A round that forms rows again is a function of its own, so that nothing of it is kept while the first one runs (as a loop around that one
+// it took 8 to 23 % of the gradients' time, in registers).  It is given the kernel's arguments where they lie; what a call passes is the
+// same for all lanes here, which the compiler has to be told again.
+typedef __attribute__((address_space(4))) const AttentionArgs args_in_place;
+template <typename E> using Lds = __attribute__((address_space(3))) E;
+__device__ __forceinline__ AttentionArgs same_args(args_in_place *args) {
+  const unsigned long long at = (unsigned long long)args;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
+  args_in_place *const there = (args_in_place *)((unsigned long long)hi << 32 | lo);
+  AttentionArgs a;
+  __builtin_memcpy(&a, (const AttentionArgs *)there, sizeof(a));
+  return a;
+}
+template <typename E>
+__device__ __forceinline__ E *same_tile(Lds<E> *p) {
+  return (E *)(Lds<E> *)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)p);
+}
 
 // delta = g_out . out of a lane's row, shared with its partner.
 template <typename T, int DP>
@@ -358,19 +396,19 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T *__restric
 // and ds the right operand of dq^T = k^T ds as it stands.  Three products (16 heads of 64, three causal scans of 12 k rows together, bf16:
 // 178 us, 975 TFLOP/s); a kernel of its own and not a by-product of the keys' gradients, whose sums over key tiles would need atomics.
 template <typename T, int DP, int NW, bool PARTS>
-__global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attention_query_grad_kernel(const AttentionArgs a) {
+__device__ __forceinline__ bool query_grad_rows(const AttentionArgs &a, int4v *k_tile0, int4v *v_tile0, int4v *k_tile1, int4v *v_tile1,
+                                                unsigned block, int shift, bool open) {
   constexpr int W = tile_width<DP>(), NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, W>;
-  __shared__ int4v k_tile0[NK * Rows::CH], v_tile0[NK * Rows::CH], k_tile1[NK * Rows::CH], v_tile1[NK * Rows::CH];
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
-  const Place at = place_of(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
-  if (at.slot >= a.slots) return;
+  const Place at = place_of(block, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
+  if (at.slot >= a.slots) return false;
   const Slot slot = find_slot(a.q_offsets, a.segments, a.n_q, group, T_ROWS, at.slot, a.slots);
   int k_begin, k_count;
   partner_rows(a.k_offsets, a.k_lengths, slot.segment, a.segments, a.n_k, k_begin, k_count);
-  if (slot.first >= slot.length) return;
+  if (slot.first >= slot.length) return false;
   const int ahead = k_count - slot.tokens;
 
   const int token0 = group == 1 ? slot.first : slot.first / group, head0 = slot.first - token0 * group;
@@ -404,7 +442,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
   load_row<T, DP>(g, mine ? (const T *)a.g_out + to * a.dim : nullptr, a.dim, lane);
   const float inf = __builtin_inff();
   float lse = mine ? a.lse[to] : inf;
-  lse = lse == -inf ? inf : lse * kLog2e - ds_shift<T>();      // (no keys: all probabilities 0)
+  lse = lse == -inf ? inf : lse * kLog2e - shift;      // (no keys: all probabilities 0)
   const float delta = row_delta<T, DP>(g, mine ? (const T *)a.out + to * a.dim : nullptr, a.dim, lane);
   if (mine && lane < 32 && (!PARTS || at.part == 0)) a.delta[to] = delta;      // (for the keys' gradients)
 
@@ -461,13 +499,40 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
     else some_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
     second = !second;
   }
-  const float scale = a.scale * pow2(-ds_shift<T>());
+  const bool fits = !ds_shifted<T>() || shift <= kLeastShift || __builtin_fabsf(dq[0][0]) < inf, ends = mine && open && fits;
+  const float scale = a.scale * __builtin_amdgcn_ldexpf(1.f, -shift);
   if constexpr (PARTS) {
     const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
-    if (mine) store_row<T, float, W>(a.part_sum + tile * a.dim, dq, scale, a.dim, lane);
-  } else if (mine) {
+    if (ends) store_row<T, float, W>(a.part_sum + tile * a.dim, dq, scale, a.dim, lane);
+  } else if (ends) {
     store_row<T, T, W>((T *)a.gq + to * a.dim, dq, scale, a.dim, lane);
   }
+  return mine && open && !fits;
+}
+
+template <typename T, int DP, int NW, bool PARTS>
+__device__ __attribute__((noinline)) void query_grad_again(args_in_place *args, Lds<int4v> *k_tile0, Lds<int4v> *v_tile0, Lds<int4v> *k_tile1,
+                                                           Lds<int4v> *v_tile1, unsigned block, bool open) {
+  const AttentionArgs a = same_args(args);
+  block = same_for_all((int)block);
+  int4v *const k0 = same_tile<int4v>(k_tile0), *const v0 = same_tile<int4v>(v_tile0);
+  int4v *const k1 = same_tile<int4v>(k_tile1), *const v1 = same_tile<int4v>(v_tile1);
+  int shift = ds_shift<T>();
+  do {
+    shift -= kShiftDown;
+    open = query_grad_rows<T, DP, NW, PARTS>(a, k0, v0, k1, v1, block, shift, open);
+  } while (any_lane<NW>(open, k1));
+}
+
+template <typename T, int DP, int NW, bool PARTS>
+__global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attention_query_grad_kernel(const AttentionArgs a) {
+  constexpr int CHUNKS = tile_rows<T, DP, NW>() * RowTile<T, tile_width<DP>()>::CH;
+  __shared__ int4v k_tile0[CHUNKS], v_tile0[CHUNKS], k_tile1[CHUNKS], v_tile1[CHUNKS];
+  const bool open = query_grad_rows<T, DP, NW, PARTS>(a, k_tile0, v_tile0, k_tile1, v_tile1, blockIdx.x, ds_shift<T>(), true);
+  if constexpr (ds_shifted<T>())
+    if (any_lane<NW>(open, k_tile1))
+      query_grad_again<T, DP, NW, PARTS>((args_in_place *)__builtin_amdgcn_kernarg_segment_ptr(), (Lds<int4v> *)k_tile0, (Lds<int4v> *)v_tile0,
+                                         (Lds<int4v> *)k_tile1, (Lds<int4v> *)v_tile1, blockIdx.x, open);
 }
 
 // Keys' and values' gradients: a wave's 32 keys are columns, the queries of all heads of the group pass by as rows, and
@@ -475,21 +540,20 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void attentio
 // sums fill 254 registers at heads of 64, and every fragment of q and g_out comes out of LDS twice.  (A second block of keys to a wave halves
 // those reads and leaves one wave a SIMD: 389 us.)
 template <typename T, int DP, int NW, bool PARTS>
-__global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_key_grad_kernel(const AttentionArgs a) {
+__device__ __forceinline__ bool key_grad_rows(const AttentionArgs &a, int4v *q_tile0, int4v *g_tile0, int4v *q_tile1, int4v *g_tile1, float4v *lse_tile0,
+                                              float4v *delta_tile0, float4v *lse_tile1, float4v *delta_tile1, unsigned block, int shift, bool open) {
   constexpr int W = tile_width<DP>(), NQ = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
   using Rows = RowTile<T, W>;
   constexpr int PER = NQ * Rows::CH / (64 * NW);
-  __shared__ int4v q_tile0[NQ * Rows::CH], g_tile0[NQ * Rows::CH], q_tile1[NQ * Rows::CH], g_tile1[NQ * Rows::CH];
-  __shared__ float4v lse_tile0[NQ / 4], delta_tile0[NQ / 4], lse_tile1[NQ / 4], delta_tile1[NQ / 4];
   const int lane = threadIdx.x % 64, wave = same_for_all(threadIdx.x / 64), group = a.heads / a.kv_heads;
   Rows rows_at;
   rows_at.aim(lane);
-  const Place at = place_of<false>(blockIdx.x, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
-  if (at.slot >= a.slots) return;
+  const Place at = place_of<false>(block, a.kv_heads, PARTS ? a.parts : 1, a.by_xcd, a.slots);
+  if (at.slot >= a.slots) return false;
   const Slot slot = find_slot(a.k_offsets, a.segments, a.n_k, 1, T_ROWS, at.slot, a.slots);
   int q_begin, q_count;
   partner_rows(a.q_offsets, nullptr, slot.segment, a.segments, a.n_q, q_begin, q_count);
-  if (slot.first >= slot.length) return;
+  if (slot.first >= slot.length) return false;
   const int ahead = slot.length - q_count, rows = q_count * group;
 
   const int local = wave * 32 + lane % 32, key = slot.first + local;
@@ -572,6 +636,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
   load_row<T, DP>(k, mine ? (const T *)a.k + (slot.begin + key) * a.k_row + at.kv_head * a.k_head : nullptr, a.dim, lane);
   load_row<T, DP>(v, mine ? (const T *)a.v + (slot.begin + key) * a.v_row + at.kv_head * a.v_head : nullptr, a.dim, lane);
   const float by = a.scale * kLog2e;
+  const float ds_by = __builtin_amdgcn_ldexpf(1.f, shift - p_shift<T>());      // (p's power of two taken out)
   float16v dk[W / 32] = {}, dv[W / 32] = {};
   const auto take = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
                         int r0) __attribute__((always_inline)) {
@@ -593,7 +658,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * r4 + e;
         p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], by, -lse[e]));
-        ds[r] = p[r] * ((ds[r] - delta[e]) * pow2(ds_shift<T>() - p_shift<T>()));
+        ds[r] = p[r] * ((ds[r] - delta[e]) * ds_by);
       }
     }
     if constexpr (decltype(masked)::value != 0) {
@@ -655,18 +720,52 @@ __global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_k
     if (second) rest_of(q_tile1, g_tile1, lse_tile1, delta_tile1, r0);
     else rest_of(q_tile0, g_tile0, lse_tile0, delta_tile0, r0);
   }
-  const float k_by = a.scale * pow2(-ds_shift<T>()), v_by = pow2(-p_shift<T>());
-  if (!mine) return;
-  if constexpr (PARTS) {
-    const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
-    const int64_t all = (int64_t)a.slots * a.kv_heads * a.parts * T_ROWS * a.dim;
-    store_row<T, float, W>(a.part_sum + tile * a.dim, dk, k_by, a.dim, lane);
-    store_row<T, float, W>(a.part_sum + all + tile * a.dim, dv, v_by, a.dim, lane);
-  } else {
-    const int64_t to = ((int64_t)(slot.begin + key) * a.kv_heads + at.kv_head) * a.dim;
-    if (a.gk) store_row<T, T, W>((T *)a.gk + to, dk, k_by, a.dim, lane);
-    if (a.gv) store_row<T, T, W>((T *)a.gv + to, dv, v_by, a.dim, lane);
+  const bool fits = !ds_shifted<T>() || !a.gk || shift <= kLeastShift || __builtin_fabsf(dk[0][0]) < inf;
+  const float k_by = a.scale * __builtin_amdgcn_ldexpf(1.f, -shift), v_by = pow2(-p_shift<T>());
+  if (mine && open && fits) {
+    if constexpr (PARTS) {
+      const int64_t tile = (((int64_t)at.slot * a.kv_heads + at.kv_head) * a.parts + at.part) * T_ROWS + local;
+      const int64_t all = (int64_t)a.slots * a.kv_heads * a.parts * T_ROWS * a.dim;
+      store_row<T, float, W>(a.part_sum + tile * a.dim, dk, k_by, a.dim, lane);
+      store_row<T, float, W>(a.part_sum + all + tile * a.dim, dv, v_by, a.dim, lane);
+    } else {
+      const int64_t to = ((int64_t)(slot.begin + key) * a.kv_heads + at.kv_head) * a.dim;
+      if (a.gk) store_row<T, T, W>((T *)a.gk + to, dk, k_by, a.dim, lane);
+      if (a.gv) store_row<T, T, W>((T *)a.gv + to, dv, v_by, a.dim, lane);
+    }
   }
+  return mine && open && !fits;
+}
+
+template <typename T, int DP, int NW, bool PARTS>
+__device__ __attribute__((noinline)) void key_grad_again(args_in_place *args, Lds<int4v> *q_tile0, Lds<int4v> *g_tile0, Lds<int4v> *q_tile1,
+                                                         Lds<int4v> *g_tile1, Lds<float4v> *lse_tile0, Lds<float4v> *delta_tile0,
+                                                         Lds<float4v> *lse_tile1, Lds<float4v> *delta_tile1, unsigned block, bool open) {
+  const AttentionArgs a = same_args(args);
+  block = same_for_all((int)block);
+  int4v *const q0 = same_tile<int4v>(q_tile0), *const g0 = same_tile<int4v>(g_tile0);
+  int4v *const q1 = same_tile<int4v>(q_tile1), *const g1 = same_tile<int4v>(g_tile1);
+  float4v *const lse0 = same_tile<float4v>(lse_tile0), *const delta0 = same_tile<float4v>(delta_tile0);
+  float4v *const lse1 = same_tile<float4v>(lse_tile1), *const delta1 = same_tile<float4v>(delta_tile1);
+  int shift = ds_shift<T>();
+  do {
+    shift -= kShiftDown;
+    open = key_grad_rows<T, DP, NW, PARTS>(a, q0, g0, q1, g1, lse0, delta0, lse1, delta1, block, shift, open);
+  } while (any_lane<NW>(open, q1));
+}
+
+template <typename T, int DP, int NW, bool PARTS>
+__global__ __launch_bounds__(NW * 64, (waves_of_keys<T, DP>())) void attention_key_grad_kernel(const AttentionArgs a) {
+  constexpr int NQ = tile_rows<T, DP, NW>(), CHUNKS = NQ * RowTile<T, tile_width<DP>()>::CH;
+  __shared__ int4v q_tile0[CHUNKS], g_tile0[CHUNKS], q_tile1[CHUNKS], g_tile1[CHUNKS];
+  __shared__ float4v lse_tile0[NQ / 4], delta_tile0[NQ / 4], lse_tile1[NQ / 4], delta_tile1[NQ / 4];
+  const bool open = key_grad_rows<T, DP, NW, PARTS>(a, q_tile0, g_tile0, q_tile1, g_tile1, lse_tile0, delta_tile0, lse_tile1, delta_tile1, blockIdx.x,
+                                                    ds_shift<T>(), true);
+  if constexpr (ds_shifted<T>())
+    if (any_lane<NW>(open, q_tile1))
+      key_grad_again<T, DP, NW, PARTS>((args_in_place *)__builtin_amdgcn_kernarg_segment_ptr(), (Lds<int4v> *)q_tile0, (Lds<int4v> *)g_tile0,
+                                       (Lds<int4v> *)q_tile1, (Lds<int4v> *)g_tile1, (Lds<float4v> *)lse_tile0, (Lds<float4v> *)delta_tile0,
+                                       (Lds<float4v> *)lse_tile1, (Lds<float4v> *)delta_tile1, blockIdx.x, open);
 }
 
 // --- launches --------------------------------------------------------------------------------------------------
