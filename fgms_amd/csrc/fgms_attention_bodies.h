@@ -238,7 +238,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
 
   // (the last column's products: row 31 of the last block, register 15 of the upper lanes)
   sum = ONES ? of_upper(o[W / 32 - 1][15]) : both_sum(sum);
-  const bool none = seen <= begin || end <= begin;      // no key for this row (here)
+  const bool none = sum == 0.f;      // no key for this row (here), or none with a score above -inf: the largest adds one or more
   const float inverse = none ? 0.f : 1.f / sum;
   const float lse = none ? -inf : (base + __builtin_log2f(sum)) * (1.f / kLog2e);
   if constexpr (PARTS) {
