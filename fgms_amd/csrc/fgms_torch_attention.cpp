@@ -103,9 +103,24 @@ struct Saved {
   }
 };
 
+// A tensor that both passes read and that has no gradient: the backward pass refuses it where it was written to in between.  (Kept as it is, not
+// as a saved tensor, which those of inference mode cannot be; they count no changes.)
+struct Index {
+  at::Tensor tensor;
+  int64_t version = 0;
+
+  Index() = default;
+  explicit Index(const at::Tensor &t) : tensor(t), version(version_of(t)) {}
+  static int64_t version_of(const at::Tensor &t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
+  const at::Tensor &unchanged(const char *op, const char *name) const {
+    TORCH_CHECK(version_of(tensor) == version, op, ": ", name, " has been modified by an inplace operation between the forward and the backward pass");
+    return tensor;
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ norms and rotation
 struct Turn {
-  at::Tensor coords, freqs;
+  Index coords, freqs;
   std::vector<int> sections;
   double eps = 0;
   bool interleaved = false;
@@ -135,8 +150,8 @@ struct NormRotaryBackward final : public torch::autograd::Node {
       if (task_should_compute_output(i)) gx[i] = result(x[i].sizes(), x[i]);
       if (w[i].defined() && task_should_compute_output(2 + i)) gw[i] = result(w[i].sizes(), w[i]);
     }
-    check(fgms_norm_rotary_bwd(data(g[0]), data(g[1]), data(x[0]), data(x[1]), data(w[0]), data(w[1]), ints(turn.coords),
-                               (const float *)data(turn.freqs), data(gx[0]), data(gx[1]), data(gw[0]), data(gw[1]), x[0].size(0),
+    check(fgms_norm_rotary_bwd(data(g[0]), data(g[1]), data(x[0]), data(x[1]), data(w[0]), data(w[1]), ints(turn.coords.unchanged(op, "coords")),
+                               (const float *)data(turn.freqs.unchanged(op, "freqs")), data(gx[0]), data(gx[1]), data(gw[0]), data(gw[1]), x[0].size(0),
                                (int)x[0].size(1), (int)x[1].size(1), (int)x[0].size(2), x[0].stride(0), x[0].stride(1), x[1].stride(0),
                                x[1].stride(1), (int)turn.sections.size(), turn.sections.data(), turn.interleaved, (float)turn.eps,
                                dtype_of(x[0]), current_stream()));
@@ -170,7 +185,7 @@ std::tuple<at::Tensor, at::Tensor> norm_rotary_node(const at::Tensor &q, const a
   FGMS_NEED(coords.size(0) == q.size(0) && coords.size(1) == (int64_t)sections.size(),
        "coords must be [N, axes], with one of the sections for each axis");
   int64_t pairs = 0;
-  Turn turn{coords, freqs, {}, eps, interleaved};
+  Turn turn{Index(coords), Index(freqs), {}, eps, interleaved};
   for (int64_t s : sections) {
     FGMS_NEED(s >= 0 && s <= 64, "a section must be between 0 and half the channels of a head");
     turn.sections.push_back((int)s);
@@ -215,7 +230,7 @@ std::tuple<at::Tensor, at::Tensor> norm_rotary_node(const at::Tensor &q, const a
 
 // ------------------------------------------------------------------------------------------------ attention
 struct Segments {
-  at::Tensor q_offsets, k_offsets;
+  Index q_offsets, k_offsets;
   bool causal = false;
   double scale = 1;
 };
@@ -241,11 +256,12 @@ struct SegmentAttentionBackward final : public torch::autograd::Node {
     }
     o = packed(o);
     l = packed(l);
-    const at::Tensor g = packed(grads[0]);
+    const at::Tensor g = packed(grads[0]), &q_offsets = segments.q_offsets.unchanged(op, "q_offsets"),
+                     &k_offsets = segments.k_offsets.unchanged(op, "k_offsets");
     FGMS_NEED(g.scalar_type() == x[0].scalar_type(), "the output gradient must have the dtype of q");
     check(fgms_segment_attention_bwd(data(g), data(x[0]), data(x[1]), data(x[2]), data(o), (const float *)data(l), data(gx[0]), data(gx[1]),
-                                     data(gx[2]), ints(segments.q_offsets), ints(segments.k_offsets), x[0].size(0), x[1].size(0),
-                                     (int)segments.q_offsets.numel() - 1, (int)x[0].size(1), (int)x[1].size(1), (int)x[0].size(2),
+                                     data(gx[2]), ints(q_offsets), ints(k_offsets), x[0].size(0), x[1].size(0),
+                                     (int)q_offsets.numel() - 1, (int)x[0].size(1), (int)x[1].size(1), (int)x[0].size(2),
                                      x[0].stride(0), x[0].stride(1), x[1].stride(0), x[1].stride(1), x[2].stride(0), x[2].stride(1),
                                      segments.causal, (float)segments.scale, dtype_of(x[0]), current_stream()));
     return {gx[0], gx[1], gx[2]};
@@ -300,7 +316,7 @@ at::Tensor segment_attention_node(const at::Tensor &q, const at::Tensor &k, cons
     node->k.save(x[1]);
     node->v.save(x[2]);
     node->lse.save(lse);
-    node->segments = Segments{q_offsets, k_offsets, causal, scale};
+    node->segments = Segments{Index(q_offsets), Index(k_offsets), causal, scale};
     torch::autograd::set_history(out, node);
     node->out.save(out, true);
   }
