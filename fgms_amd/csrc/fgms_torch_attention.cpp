@@ -51,10 +51,12 @@ void need_features(const at::Tensor &t, const at::Tensor &like, const char *name
   FGMS_NEED(t.scalar_type() == like.scalar_type(), std::string(name) + " must have the dtype of q");
 }
 
-void need_ints(const at::Tensor &t, const at::Tensor &like, int dims, const char *name) {
-  FGMS_NEED(t.scalar_type() == at::ScalarType::Int && t.is_cuda() && t.is_contiguous() && t.dim() == dims,
-       std::string(name) + " must be a contiguous int32 tensor of " + std::to_string(dims) + " dimension(s) on the GPU");
+// (a slice of a wider tensor, such as the coordinates of a batched cloud, is copied)
+at::Tensor need_ints(const at::Tensor &t, const at::Tensor &like, int dims, const char *name) {
+  FGMS_NEED(t.scalar_type() == at::ScalarType::Int && t.is_cuda() && t.dim() == dims,
+       std::string(name) + " must be an int32 tensor of " + std::to_string(dims) + " dimension(s) on the GPU");
   FGMS_NEED(t.device() == like.device(), std::string(name) + " must be on the device of q");
+  return t.is_contiguous() ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 void refuse_tangent(const at::Tensor &t, const char *op, const char *name) {
@@ -167,8 +169,8 @@ struct NormRotaryBackward final : public torch::autograd::Node {
 };
 
 std::tuple<at::Tensor, at::Tensor> norm_rotary_node(const at::Tensor &q, const at::Tensor &k, const c10::optional<at::Tensor> &q_scale_,
-                                                    const c10::optional<at::Tensor> &k_scale_, const at::Tensor &coords,
-                                                    const at::Tensor &freqs, at::IntArrayRef sections, double eps, bool interleaved) {
+                                                    const c10::optional<at::Tensor> &k_scale_, const at::Tensor &coords_,
+                                                    const at::Tensor &freqs_, at::IntArrayRef sections, double eps, bool interleaved) {
   static const char op[] = "norm_rotary";
   const at::Tensor scale[2] = {q_scale_.value_or(at::Tensor()), k_scale_.value_or(at::Tensor())};
   FGMS_NEED(q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2),
@@ -181,24 +183,26 @@ std::tuple<at::Tensor, at::Tensor> norm_rotary_node(const at::Tensor &q, const a
       need_features(s, q, "a scale");
       FGMS_NEED(s.dim() == 1 && s.size(0) == q.size(2), "a scale must have one value for each channel of a head");
     }
-  need_ints(coords, q, 2, "coords");
+  const at::Tensor coords = need_ints(coords_, q, 2, "coords");
   FGMS_NEED(coords.size(0) == q.size(0) && coords.size(1) == (int64_t)sections.size(),
        "coords must be [N, axes], with one of the sections for each axis");
   int64_t pairs = 0;
-  Turn turn{Index(coords), Index(freqs), {}, eps, interleaved};
+  std::vector<int> each;
   for (int64_t s : sections) {
     FGMS_NEED(s >= 0 && s <= 64, "a section must be between 0 and half the channels of a head");
-    turn.sections.push_back((int)s);
+    each.push_back((int)s);
     pairs += s;
   }
-  FGMS_NEED(freqs.scalar_type() == at::ScalarType::Float && freqs.is_cuda() && freqs.device() == q.device() && freqs.is_contiguous() &&
-           freqs.dim() == 1 && freqs.size(0) == pairs,
-       "freqs must be a contiguous float32 tensor on the device of q, with a value for each pair of the sections");
+  FGMS_NEED(freqs_.scalar_type() == at::ScalarType::Float && freqs_.is_cuda() && freqs_.device() == q.device() && freqs_.dim() == 1 &&
+           freqs_.size(0) == pairs,
+       "freqs must be a float32 tensor on the device of q, with a value for each pair of the sections");
   const bool grad_mode = at::GradMode::is_enabled();
-  FGMS_NEED(!(grad_mode && freqs.requires_grad()), "norm_rotary forms no gradient of freqs");
+  FGMS_NEED(!(grad_mode && freqs_.requires_grad()), "norm_rotary forms no gradient of freqs");
   refuse_tangent(q, op, "q");
   refuse_tangent(k, op, "k");
-  refuse_tangent(freqs, op, "freqs");
+  refuse_tangent(freqs_, op, "freqs");
+  const at::Tensor freqs = freqs_.is_contiguous() ? freqs_ : freqs_.clone(at::MemoryFormat::Contiguous);
+  const Turn turn{Index(coords), Index(freqs), each, eps, interleaved};
   at::Tensor x[2], w[2], y[2];
   {
     at::AutoGradMode no_grad(false);
@@ -275,21 +279,20 @@ struct SegmentAttentionBackward final : public torch::autograd::Node {
   std::string name() const override { return "SegmentAttentionBackward"; }
 };
 
-at::Tensor segment_attention_node(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &q_offsets,
-                                  const at::Tensor &k_offsets, const c10::optional<at::Tensor> &k_lengths_, bool causal, double scale) {
+at::Tensor segment_attention_node(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &q_offsets_,
+                                  const at::Tensor &k_offsets_, const c10::optional<at::Tensor> &k_lengths_, bool causal, double scale) {
   static const char op[] = "segment_attention";
-  const at::Tensor k_lengths = k_lengths_.value_or(at::Tensor());
+  at::Tensor k_lengths = k_lengths_.value_or(at::Tensor());
   FGMS_NEED(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && q.size(2) == k.size(2),
        "expected q [Nq, heads, D], k and v [Nk, key heads, D]");
   need_features(q, q, "q");
   need_features(k, q, "k");
   need_features(v, q, "v");
   const int dtype = dtype_of(q);
-  need_ints(q_offsets, q, 1, "q_offsets");
-  need_ints(k_offsets, q, 1, "k_offsets");
+  const at::Tensor q_offsets = need_ints(q_offsets_, q, 1, "q_offsets"), k_offsets = need_ints(k_offsets_, q, 1, "k_offsets");
   FGMS_NEED(q_offsets.numel() >= 1 && q_offsets.numel() == k_offsets.numel(), "q_offsets and k_offsets must have one more entry than there are segments");
   if (k_lengths.defined()) {
-    need_ints(k_lengths, q, 1, "k_lengths");
+    k_lengths = need_ints(k_lengths, q, 1, "k_lengths");
     FGMS_NEED(k_lengths.numel() == q_offsets.numel() - 1, "k_lengths must have an entry for each segment");
   }
   const bool wants_grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
