@@ -180,11 +180,15 @@ class VoxelAttention(torch.nn.Module):
     def __init__(self, channels, heads, kv_heads=None, sections=None, base=100.0, causal=False, dtype=None, device=None):
         super().__init__()
         self.heads, self.kv_heads, self.causal = heads, kv_heads or heads, causal
-        if channels % heads or heads % self.kv_heads:
+        if heads < 1 or self.kv_heads < 1 or channels % heads or heads % self.kv_heads:
             raise ValueError("channels must be a multiple of heads, and heads of kv_heads")
         self.dim = channels // heads
+        if self.dim % 8 or not 8 <= self.dim <= 128:
+            raise ValueError("the channels of a head, channels / heads, must be a multiple of 8 from 8 to 128")
         pairs = self.dim // 2
         self.sections = tuple(sections) if sections is not None else (pairs - 2 * (pairs // 3), pairs // 3, pairs // 3)
+        if not 1 <= len(self.sections) <= 4 or min(self.sections) < 0 or sum(self.sections) > pairs:
+            raise ValueError("sections must be one to four shares of the %d pairs of a head" % pairs)
         self.qkv = torch.nn.Linear(channels, (heads + 2 * self.kv_heads) * self.dim, bias=False, dtype=dtype, device=device)
         self.q_scale = torch.nn.Parameter(torch.ones(self.dim, dtype=dtype, device=device))
         self.k_scale = torch.nn.Parameter(torch.ones(self.dim, dtype=dtype, device=device))
