@@ -162,8 +162,9 @@ class VoxelCache:
         self.offsets = torch.arange(segments + 1, dtype=torch.int32, device=device) * capacity
         self.lengths = torch.zeros(segments, dtype=torch.int32, device=device)
 
+    @torch.no_grad()
     def append(self, k, v):
-        """One new row for every scan; a full scan keeps its last row replaced."""
+        """One new row for every scan (its values: a cache is in no graph); a full scan keeps its last row replaced."""
         rows = (self.offsets[:-1] + self.lengths.clamp(max=self.capacity - 1)).long()
         self.k.index_copy_(0, rows, k)
         self.v.index_copy_(0, rows, v)
@@ -209,7 +210,10 @@ class VoxelAttention(torch.nn.Module):
         return self.out(segment_attention(q, k, v, offsets, causal=self.causal).flatten(1))
 
     def step(self, feats, coords, cache):
-        """One new row of every scan: its keys and values join the cache, its query sees all of them."""
+        """One new row of every scan: its keys and values join the cache, its query sees all of them.  There are no gradients over
+        caches: call it under ``torch.no_grad()`` where the layer or the rows ask for some."""
+        if torch.is_grad_enabled() and (feats.requires_grad or any(p.requires_grad for p in self.parameters())):
+            raise ValueError("a step over a cache has no gradients: call it under torch.no_grad()")
         q, k, v = self._heads(feats, coords)
         cache.append(k, v)
         ones = torch.arange(feats.shape[0] + 1, dtype=torch.int32, device=feats.device)
