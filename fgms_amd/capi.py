@@ -387,6 +387,14 @@ def _need_rows(t, name, like):
         raise ValueError("%s must be [rows, heads, channels] of q's dtype on the GPU, channels side by side" % name)
 
 
+def _need_shaped(t, name, dtype, shape):
+    """None, or a contiguous GPU tensor of this shape: the kernels go by the shapes of q and k alone."""
+    if t is not None:
+        _need(t, name, dtype)
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError("%s must have shape %s" % (name, tuple(shape)))
+
+
 def _turn(q, k, coords, freqs, sections, interleaved, eps):
     _need_rows(q, "q", q)
     _need_rows(k, "k", q)
@@ -401,9 +409,8 @@ def _turn(q, k, coords, freqs, sections, interleaved, eps):
 
 def norm_rotary_fwd(q, k, q_scale, k_scale, coords, freqs, sections, q_out, k_out, eps=1e-6, interleaved=False):
     """``fgms_norm_rotary_fwd``; scales may be None."""
-    for t, n in ((q_scale, "q_scale"), (k_scale, "k_scale"), (q_out, "q_out"), (k_out, "k_out")):
-        if t is not None:
-            _need(t, n, q.dtype)
+    for t, n, like in ((q_scale, "q_scale", q.shape[2:]), (k_scale, "k_scale", q.shape[2:]), (q_out, "q_out", q.shape), (k_out, "k_out", k.shape)):
+        _need_shaped(t, n, q.dtype, like)
     rest = _turn(q, k, coords, freqs, sections, interleaved, eps)
     _check(lib().fgms_norm_rotary_fwd(_p(q), _p(k), _p(q_scale), _p(k_scale), _p(coords), _p(freqs), _p(q_out), _p(k_out), *rest))
 
@@ -411,10 +418,10 @@ def norm_rotary_fwd(q, k, q_scale, k_scale, coords, freqs, sections, q_out, k_ou
 def norm_rotary_bwd(q_out_grad, k_out_grad, q, k, q_scale, k_scale, coords, freqs, sections, q_grad, k_grad, q_scale_grad=None,
                     k_scale_grad=None, eps=1e-6, interleaved=False):
     """``fgms_norm_rotary_bwd``: gradients are written; None: not wanted."""
-    for t, n in ((q_out_grad, "q_out_grad"), (k_out_grad, "k_out_grad"), (q_scale, "q_scale"), (k_scale, "k_scale"), (q_grad, "q_grad"),
-                 (k_grad, "k_grad"), (q_scale_grad, "q_scale_grad"), (k_scale_grad, "k_scale_grad")):
-        if t is not None:
-            _need(t, n, q.dtype)
+    for t, n, like in ((q_out_grad, "q_out_grad", q.shape), (k_out_grad, "k_out_grad", k.shape), (q_scale, "q_scale", q.shape[2:]),
+                       (k_scale, "k_scale", q.shape[2:]), (q_grad, "q_grad", q.shape), (k_grad, "k_grad", k.shape),
+                       (q_scale_grad, "q_scale_grad", q.shape[2:]), (k_scale_grad, "k_scale_grad", q.shape[2:])):
+        _need_shaped(t, n, q.dtype, like)
     rest = _turn(q, k, coords, freqs, sections, interleaved, eps)
     _check(lib().fgms_norm_rotary_bwd(_p(q_out_grad), _p(k_out_grad), _p(q), _p(k), _p(q_scale), _p(k_scale), _p(coords), _p(freqs),
                                       _p(q_grad), _p(k_grad), _p(q_scale_grad), _p(k_scale_grad), *rest))
@@ -433,20 +440,19 @@ def _segments(q, k, v, q_offsets, k_offsets, causal, scale):
 
 def segment_attention_fwd(q, k, v, out, lse, q_offsets, k_offsets, k_lengths=None, causal=False, scale=1.0):
     """``fgms_segment_attention_fwd``; lse (fp32 [rows, heads]) may be None."""
-    _need(out, "out", q.dtype)
-    for t, n, d in ((lse, "lse", torch.float32), (k_lengths, "k_lengths", torch.int32)):
-        if t is not None:
-            _need(t, n, d)
+    for t, n, d, like in ((out, "out", q.dtype, q.shape), (lse, "lse", torch.float32, q.shape[:2]),
+                          (k_lengths, "k_lengths", torch.int32, (q_offsets.numel() - 1,))):
+        _need_shaped(t, n, d, like)
     rest = _segments(q, k, v, q_offsets, k_offsets, causal, scale)
     _check(lib().fgms_segment_attention_fwd(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(q_offsets), _p(k_offsets), _p(k_lengths), *rest))
 
 
 def segment_attention_bwd(out_grad, q, k, v, out, lse, q_grad, k_grad, v_grad, q_offsets, k_offsets, causal=False, scale=1.0):
     """``fgms_segment_attention_bwd``: gradients are written; None: not wanted."""
-    for t, n in ((out_grad, "out_grad"), (out, "out"), (q_grad, "q_grad"), (k_grad, "k_grad"), (v_grad, "v_grad")):
-        if t is not None:
-            _need(t, n, q.dtype)
-    _need(lse, "lse", torch.float32)
+    for t, n, like in ((out_grad, "out_grad", q.shape), (out, "out", q.shape), (q_grad, "q_grad", q.shape), (k_grad, "k_grad", k.shape),
+                       (v_grad, "v_grad", k.shape)):
+        _need_shaped(t, n, q.dtype, like)
+    _need_shaped(lse, "lse", torch.float32, q.shape[:2])
     rest = _segments(q, k, v, q_offsets, k_offsets, causal, scale)
     _check(lib().fgms_segment_attention_bwd(_p(out_grad), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(q_grad), _p(k_grad), _p(v_grad),
                                             _p(q_offsets), _p(k_offsets), *rest))
