@@ -240,7 +240,7 @@ __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_
   sum = ONES ? of_upper(o[W / 32 - 1][15]) : both_sum(sum);
   const bool none = sum == 0.f;      // no key for this row (here), or none with a score above -inf: the largest adds one or more
   const float inverse = none ? 0.f : 1.f / sum;
-  if (__builtin_amdgcn_ballot_w64(none))      // (zeros, whatever values of the tile they were multiplied with)
+  if (a.causal && __builtin_amdgcn_ballot_w64(none))      // (zeros, whatever values of the tile they were multiplied with)
 #pragma unroll
     for (int db = 0; db < W / 32; ++db) o[db] = none ? float16v{} : o[db];
   const float lse = none ? -inf : (base + __builtin_log2f(sum)) * (1.f / kLog2e);
@@ -502,7 +502,7 @@ __device__ __forceinline__ bool query_grad_rows(const AttentionArgs &a, int4v *k
     else some_of(k_tile0, v_tile0, k_tile1, v_tile1, j);
     second = !second;
   }
-  if (__builtin_amdgcn_ballot_w64(lse == inf))      // (no keys: as the forward pass)
+  if (a.causal && __builtin_amdgcn_ballot_w64(lse == inf))      // (no keys: as the forward pass)
 #pragma unroll
     for (int db = 0; db < W / 32; ++db) dq[db] = lse == inf ? float16v{} : dq[db];
   const bool fits = !ds_shifted<T>() || shift <= kLeastShift || __builtin_fabsf(dq[0][0]) < inf, ends = mine && open && fits;
