@@ -125,7 +125,7 @@ def norm_rotary(q, k, q_scale, k_scale, coords, freqs, sections, eps=1e-6, inter
     q ``[N, heads, D]``, k ``[N, key heads, D]`` (slices of one projection are read as they lie), scales ``[D]`` or None,
     coords int32 ``[N, axes]``.  The first ``sections[0]`` pairs of channels turn by ``coords[:, 0] * freqs[pair]``, the next
     ``sections[1]`` with the second axis, ...; pairs behind the last section stay.  Pair p is channels (p, p + D / 2), with
-    ``interleaved`` (2p, 2p + 1)."""
+    ``interleaved`` (2p, 2p + 1).  coords and freqs must not be written to before the backward pass."""
     return backend.norm_rotary(q, k, q_scale, k_scale, coords, freqs, list(sections), float(eps), bool(interleaved))
 
 
@@ -135,8 +135,9 @@ def segment_attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=No
     q ``[Nq, heads, D]``, k and v ``[Nk, key heads, D]``, heads a multiple of key heads.  Segment s is rows
     ``q_offsets[s]`` to ``q_offsets[s + 1]`` of q and likewise of k and v (``k_offsets``; None: the same): int32 tensors on
     the device, from which no size has to come back.  ``causal``: ends of queries and keys aligned, keys behind a query not
-    seen.  A row that sees no key comes out as zeros.  ``k_lengths`` (int32, one a segment; no gradients): how much of each
-    segment of k and v is in use, for caches with room left.  ``scale`` is positive, None: ``1 / sqrt(D)``."""
+    seen.  A row that sees no key comes out as zeros.  Offsets must not be written to before the backward pass.  ``k_lengths``
+    (int32, one a segment; no gradients): how much of each segment of k and v is in use, for caches with room left.  ``scale`` is
+    positive, None: ``1 / sqrt(D)``."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return backend.segment_attention(q, k, v, q_offsets, q_offsets if k_offsets is None else k_offsets, k_lengths, bool(causal), float(scale))

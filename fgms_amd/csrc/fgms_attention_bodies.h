@@ -95,9 +95,9 @@ __device__ __forceinline__ Place place_of(unsigned block, int kv_heads, int part
 // two pairs of buffers: the next one is on its way while this one is worked on.  ONES: a head has fewer channels than the tile (16-bit types);
 // the values' last column then holds ones, and the rows' sums come out of the second product, a sixth of the vector instructions less
 // (of the probabilities as rounded for it, so that a row's weights add up to one).
-// 16/4 heads of 128, two causal scans of 24 k rows together, bf16: 1.38 ms, 1.10 PFLOP/s where a large library product reaches 1.14; 16
-// heads of 64 over 12 k rows 142 us, 815 TFLOP/s: the vector pipe is busy 75 % of the time, the matrix pipe 46 % (heads of 128: 54 % and
-// 64 %; an exponential takes two turns).  Windows of 160 voxels on average, 4 heads of 16, 200 k voxels: 62 us, 20 for its bytes.
+// 16/4 heads of 128, two causal scans of 24 k rows together, bf16: 1.33 to 1.38 ms, 1.10 to 1.14 PFLOP/s where a large library product has 1.14; 16
+// heads of 64 over three of 12 k together 142 us, 815 TFLOP/s: the vector pipe is busy 75 % of the time, the matrix pipe 46 % (heads of 128: 54 %
+// and 65 %; an exponential takes two turns).  Windows of 160 voxels on average, 4 heads of 16, 200 k voxels: 64 us, 20 for its bytes.
 template <typename T, int DP, int NW, bool PARTS, bool ONES>
 __global__ __launch_bounds__(NW * 64, (waves_of_queries<T, DP>())) void segment_attention_kernel(const AttentionArgs a) {
   constexpr int W = tile_width<DP>(), NK = tile_rows<T, DP, NW>(), STEPS = DP / (32 / (int)sizeof(T)), T_ROWS = 32 * NW;
@@ -351,7 +351,7 @@ __device__ __forceinline__ bool any_lane(bool mine, int4v *tile) {
 }
 
 // A round that forms rows again is a function of its own, so that nothing of it is kept while the first one runs (as a loop around that one
-// it took 8 to 23 % of the gradients' time, in registers).  It is given the kernel's arguments where they lie; what a call passes is the
+// it took 8 to 23 % of the gradients' time, in registers; as it is, 0 to 4).  It is given the kernel's arguments where they lie; what a call passes is the
 // same for all lanes here, which the compiler has to be told again.
 typedef __attribute__((address_space(4))) const AttentionArgs args_in_place;
 template <typename E> using Lds = __attribute__((address_space(3))) E;
@@ -647,7 +647,8 @@ __device__ __forceinline__ bool key_grad_rows(const AttentionArgs &a, int4v *q_t
   const auto take = [&](auto masked, const int4v *q_tile, const int4v *g_tile, const float4v *lse_tile, const float4v *delta_tile, int qb,
                         int r0) __attribute__((always_inline)) {
     float16v p = {}, ds = {};
-    // (heads of 96: what one step reads is not fetched during the one before, which the registers have no room for: 836 -> 775 us over 9 k rows)
+    // (heads of 96: what one step reads is not fetched during the one before, which the registers have no room for: both gradients of
+    // two scans of 9 k rows together, 16/4 heads, bf16, 1278 -> 1228 us)
     const auto phase = []() __attribute__((always_inline)) { if constexpr (DP == 96) __builtin_amdgcn_sched_barrier(0); };
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)

@@ -18,7 +18,8 @@ template <typename T, int V> using Vec = T __attribute__((ext_vector_type(V)));
 
 // sin and cos of coordinate * frequency.  The angle of a far voxel has thousands of turns, of which 32 bits would leave the fraction a
 // few digits only: the product and the reduction to an eighth of a turn are taken in 64 (a handful of operations a pair of
-// channels, shared by all heads), the Taylor sums of the rest in 32 (last terms below 2^-25).
+// channels, shared by all heads), the Taylor sums of the rest in 32 (up to pi / 4; the first terms left out are x^11 / 11!, below
+// 2^-29, and x^12 / 12!, below 2^-33).
 __device__ __forceinline__ void sine_cosine(int coordinate, float frequency, float &sine, float &cosine) {
   const double turns = (double)coordinate * (double)frequency * 0.15915494309189535;
   const double quarters = __builtin_rint(turns * 4.0);

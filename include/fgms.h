@@ -294,7 +294,7 @@ int fgms_build_map_end(fgms_map_build_t *build, int32_t *host_nnz, int64_t *n_pa
  *   - coords: int32 [n, axes], device; freqs: fp32 [sum of sections], device; sections: HOST int [axes],
  *     1 to 4 axes.  Any 32-bit coordinate: the angle is reduced in 64 bits.
  * The backward call writes the gradients of q, k and the scales; NULL: not wanted.  The scales' gradients
- * are summed in a fixed order.
+ * are summed in a fixed order (k_heads = 0: k_scale's is zero).
  */
 int fgms_norm_rotary_fwd(const void *q, const void *k, const void *q_scale, const void *k_scale,
                          const int32_t *coords, const float *freqs, void *q_out, void *k_out,
@@ -320,16 +320,21 @@ int fgms_norm_rotary_bwd(const void *q_out_grad, const void *k_out_grad,
  *   - k_lengths: NULL, or int32 [segments], device: only the first k_lengths[s] rows of segment s are keys
  *     (caches with room left; what lies behind is not read)
  *   - causal != 0: the last query of a segment sees all of its keys, the one before it one less, ...
- *   - a row that sees no key: out 0 (and lse -infinity, gradients 0)
+ *   - a row that sees no key, or whose scores are all -infinity: out 0 (and lse -infinity); one that sees none: gradient 0
  *   - lse: fp32 [n_q, heads], the log of each row's sum of exponentials, for the backward call; may be NULL
  *   - scale: positive
- * Few queries over many keys (a new row and its cache) are cut along the keys, in a workspace of the stream.
+ * Few queries over many keys (a new row and its cache) are cut along the keys, in a workspace of the stream, which the call has to itself
+ * until its last launch.
  * The backward call forms the probabilities again from q, k and lse; it writes the gradients whose pointers
  * are not NULL, sums over the heads of a group included.  No atomics: the same bits every time.
- * Infinities and NaN in v reach the rows that see them, and with `causal` may turn up to 63 rows before those into NaN;
- * keys that a row does not see may hold anything.
- * Rows of k and v must not overlap, rows of any tensor lie at most 16 MB and the heads of a group 512 MB apart; n_k, and n_q
- * times the heads of a group, at most 2^31 - 2^25.
+ * Infinities and NaN, out: those in v reach the rows that see them, and with `causal` may turn up to 63 rows before those into
+ * NaN (rows that see no key stay 0); keys that a row does not see may hold anything.  Gradients: with `causal` a row of q, k, v or
+ * out_grad that holds one may turn gradients of rows of its segment into NaN that it does not see or that do not see it.  Nothing of one
+ * segment reaches another's rows.
+ * FGMS_F16: weights down to 2^-32 of a row's largest count; scores' gradients of any size are formed (those beyond 4094 in a second round
+ * over their rows).
+ * Rows of k and v must not overlap (the stride of a single one does not matter), rows of any tensor lie at most 16 MB and the heads of a
+ * group 512 MB apart; n_k, and n_q times the heads of a group, at most 2^31 - 2^25.
  */
 int fgms_segment_attention_fwd(const void *q, const void *k, const void *v, void *out, float *lse,
                                const int32_t *q_offsets, const int32_t *k_offsets, const int32_t *k_lengths,
