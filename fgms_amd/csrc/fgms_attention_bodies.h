@@ -365,7 +365,7 @@ __device__ __forceinline__ AttentionArgs same_args(args_in_place *args) {
 }
 template <typename E>
 __device__ __forceinline__ E *same_tile(Lds<E> *p) {
-  return (E *)(Lds<E> *)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)p);
+  return (E *)(Lds<E> *)(uintptr_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)p);
 }
 
 // delta = g_out . out of a lane's row, shared with its partner.
