@@ -12,6 +12,7 @@ repeat by hand before every call: the padded offset table ``qkpos``
 layer, pass and iteration that shares a map shares its plan through ``FGMS.backend``'s
 cache, which is keyed on these tensors.
 """
+import copy
 import math
 import threading
 
@@ -201,8 +202,8 @@ class VoxelAttention(torch.nn.Module):
     def _heads(self, feats, coords):
         h, hk, d = self.heads, self.kv_heads, self.dim
         q, k, v = (t.unflatten(-1, (-1, d)) for t in self.qkv(feats).split((h * d, hk * d, hk * d), -1))
-        if self._freqs.device != feats.device:
-            self._freqs = self._freqs.to(feats.device)
+        if self._freqs.device != q.device:
+            self._freqs = self._freqs.to(q.device)
         q, k = norm_rotary(q, k, self.q_scale, self.k_scale, coords, self._freqs, self.sections)
         return q, k, v
 
@@ -213,10 +214,130 @@ class VoxelAttention(torch.nn.Module):
     def step(self, feats, coords, cache):
         """One new row of every scan: its keys and values join the cache, its query sees all of them.  There are no gradients over
         caches: call it under ``torch.no_grad()`` where the layer or the rows ask for some."""
-        if torch.is_grad_enabled() and (feats.requires_grad or any(p.requires_grad for p in self.parameters())):
+        rows = feats[0] if isinstance(feats, tuple) else feats      # (in 8 bits, with their scales)
+        if torch.is_grad_enabled() and (rows.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise ValueError("a step over a cache has no gradients: call it under torch.no_grad()")
         q, k, v = self._heads(feats, coords)
         cache.append(k, v)
-        ones = torch.arange(feats.shape[0] + 1, dtype=torch.int32, device=feats.device)
+        ones = torch.arange(q.shape[0] + 1, dtype=torch.int32, device=q.device)
         y = segment_attention(q, cache.k, cache.v, ones, cache.offsets, k_lengths=cache.lengths)
         return self.out(y.flatten(1))
+
+    def to_int8(self):
+        """This layer with its projections' weights in 8 bits (:class:`Int8Linear`), for inference on the device that it is on: a new module
+        without gradients.  Its features may be in 8 bits too, as (q, scales)."""
+        layer = copy.deepcopy(self).requires_grad_(False).eval()
+        layer.qkv, layer.out = Int8Linear(layer.qkv), Int8Linear(layer.out)
+        return layer
+
+
+# ------------------------------------------------------------------------------- around attention
+def _seed_for(p, seed, x):
+    return torch.randint(-1 << 63, (1 << 63) - 1, (2,), device=x.device) if p > 0 and seed is None else seed
+
+
+def add_norm(x, residual=None, scale=None, eps=1e-6, p=0.0, seed=None):
+    """(y, h): h = residual + dropout(x), y = h * scale / sqrt(mean(h ** 2) + eps) over a row's channels, in one pass; differentiable in x,
+    residual and scale.
+
+    x and residual ``[N, channels]`` of one shape and type (rows of a wider tensor are read as they lie), scale ``[channels]`` or None.
+    h is rounded to the type before its norm is taken; where there is neither a residual nor dropout it is x itself.  ``p``: the share of
+    elements that is dropped (in steps of 2 ** -16), the others of x grow by 1 / (1 - p).  Which ones follows from ``seed``, two int64 numbers on
+    the device (None: drawn from torch's generator), and no mask is stored: seed must not be written to before the backward pass.  A
+    captured call replays with what stands in it then."""
+    return backend.add_norm(x, residual, scale, float(eps), float(p), _seed_for(p, seed, x))
+
+
+def dropout_add(x, residual=None, p=0.1, seed=None):
+    """residual + dropout(x), as :func:`add_norm` forms it; differentiable in x and residual."""
+    return backend.dropout_add(x, residual, float(p), _seed_for(p, seed, x))
+
+
+def quantize_rows(x, gated=False):
+    """Rows in 8 bits: (q int8 ``[N, channels]``, scales float32 ``[N]``), scales the largest magnitude of a row / 127 and q = x / scale
+    rounded.  ``gated``: of silu(a) * b, rows (a, b) of x.  Rows of q begin on 16 bytes.  No gradients.  A row with an infinity or NaN stands
+    for NaN."""
+    return backend.quantize_rows(x, bool(gated))
+
+
+def add_norm_int8(x, residual=None, scale=None, eps=1e-6):
+    """(q, scales, h): :func:`add_norm` without dropout with its norm in 8 bits, as :func:`quantize_rows` leaves it.  No gradients."""
+    return backend.add_norm_int8(x, residual, scale, float(eps))
+
+
+def int8_linear(x, x_scales, weight, weight_scales, bias=None, dtype=torch.float16):
+    """``x_scales[i] * weight_scales[o] * sum(x[i] * weight[o]) + bias[o]`` for int8 x ``[N, channels]`` and weight ``[outputs, channels]``; the
+    result and bias have type ``dtype``.  The sums are exact.  Rows that do not begin on 16 bytes are copied.  No gradients."""
+    return backend.int8_linear(x, x_scales, weight, weight_scales, bias, dtype)
+
+
+class Int8Linear(torch.nn.Module):
+    """A linear layer for inference with its weights in 8 bits and a scale for each output; its rows are brought to 8 bits on the way in:
+    ``y = layer(x)``, or ``y = layer((q, scales))`` of rows that are there already."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.in_features, self.out_features, self.dtype = linear.in_features, linear.out_features, linear.weight.dtype
+        with torch.no_grad():
+            q, scales = quantize_rows(linear.weight)
+            self.register_buffer("weight", q)
+            self.register_buffer("weight_scales", scales)
+            self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+
+    def _apply(self, fn, recurse=True):
+        scales = self.weight_scales
+        super()._apply(fn, recurse)
+        # (scales stay fp32 whatever the layer is cast to; its results are of the type)
+        self.weight_scales = scales.to(self.weight.device)
+        self.dtype = fn(torch.empty(0, dtype=self.dtype, device=scales.device)).dtype
+        return self
+
+    def forward(self, x):
+        q, scales = x if isinstance(x, tuple) else quantize_rows(x)
+        return int8_linear(q, scales, self.weight, self.weight_scales, self.bias, self.dtype)
+
+
+class VoxelBlock(torch.nn.Module):
+    """:class:`VoxelAttention` and a gated product pair, each behind a norm and with dropout ``p`` on its way back to the features:
+    ``y = block(feats, coords, offsets)``, ``y = block.step(feats, coords, cache)``; ``block.to_int8()`` for inference in 8 bits."""
+
+    def __init__(self, channels, heads, kv_heads=None, hidden=None, sections=None, base=100.0, causal=False, p=0.0, eps=1e-6, dtype=None,
+                 device=None):
+        super().__init__()
+        self.hidden = 2 * channels if hidden is None else hidden
+        if self.hidden < 1:
+            raise ValueError("a block needs hidden channels")
+        if not 0 <= p < 1:
+            raise ValueError("p must be at least 0 and less than 1")
+        self.p, self.eps = p, eps
+        self.norm1 = torch.nn.Parameter(torch.ones(channels, dtype=dtype, device=device))
+        self.attention = VoxelAttention(channels, heads, kv_heads, sections, base, causal, dtype, device)
+        self.norm2 = torch.nn.Parameter(torch.ones(channels, dtype=dtype, device=device))
+        self.up = torch.nn.Linear(channels, 2 * self.hidden, bias=False, dtype=dtype, device=device)
+        self.down = torch.nn.Linear(self.hidden, channels, bias=False, dtype=dtype, device=device)
+
+    def _through(self, feats, attend):
+        p = self.p if self.training else 0.0
+        if isinstance(self.up, Int8Linear):
+            q, scales, h = add_norm_int8(feats, None, self.norm1, self.eps)
+            q, scales, h = add_norm_int8(attend((q, scales)), h, self.norm2, self.eps)
+            return dropout_add(self.down(quantize_rows(self.up((q, scales)), gated=True)), h, 0.0)
+        y, h = add_norm(feats, None, self.norm1, self.eps)
+        y, h = add_norm(attend(y), h, self.norm2, self.eps, p)
+        a, b = self.up(y).chunk(2, -1)
+        return dropout_add(self.down(torch.nn.functional.silu(a) * b), h, p)
+
+    def forward(self, feats, coords, offsets):
+        return self._through(feats, lambda y: self.attention(y, coords, offsets))
+
+    def step(self, feats, coords, cache):
+        """One new row of every scan (:meth:`VoxelAttention.step`)."""
+        return self._through(feats, lambda y: self.attention.step(y, coords, cache))
+
+    def to_int8(self):
+        """This block with its projections' weights in 8 bits, for inference on the device that it is on: a new module without dropout or
+        gradients."""
+        block = copy.deepcopy(self).requires_grad_(False).eval()
+        block.attention = block.attention.to_int8()
+        block.up, block.down = Int8Linear(block.up), Int8Linear(block.down)
+        return block

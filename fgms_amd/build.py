@@ -21,9 +21,10 @@ OBJ_DIR = os.path.join(ROOT, "build", "obj")
 
 HIP_SOURCES = ["fgms_api.hip", "fgms_generic.hip", "fgms_plan.hip", "fgms_mfma.hip", "fgms_small.hip", "fgms_narrow.hip", "fgms_wgrad.hip",
                "fgms_probe.hip", "fgms_kmap.hip", "fgms_wide.hip", "fgms_pad.hip", "fgms_brief.hip",
-               "fgms_norm_rotary.hip", "fgms_attention.hip", "fgms_attention_f16.hip", "fgms_attention_bf16.hip", "fgms_attention_f32.hip"]
+               "fgms_norm_rotary.hip", "fgms_attention.hip", "fgms_attention_f16.hip", "fgms_attention_bf16.hip", "fgms_attention_f32.hip",
+               "fgms_block.hip", "fgms_rows.hip", "fgms_int8_linear.hip"]
 
-TORCH_SOURCES = ["fgms_torch.cpp", "fgms_torch_attention.cpp"]
+TORCH_SOURCES = ["fgms_torch.cpp", "fgms_torch_attention.cpp", "fgms_torch_block.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")

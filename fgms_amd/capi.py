@@ -20,6 +20,8 @@ SYMBOLS = [
     "fgms_profile_reset", "fgms_probe_gather", "fgms_build_kernel_map", "fgms_build_map_begin", "fgms_build_map_end", "fgms_allocation_count",
     "fgms_weights_pin", "fgms_weights_unpin", "fgms_relaid_weights_hits",
     "fgms_norm_rotary_fwd", "fgms_norm_rotary_bwd", "fgms_segment_attention_fwd", "fgms_segment_attention_bwd",
+    "fgms_add_norm_fwd", "fgms_add_norm_bwd_sums", "fgms_add_norm_bwd", "fgms_dropout_add", "fgms_quantize_rows", "fgms_add_norm_int8",
+    "fgms_int8_linear",
 ]
 
 _lib = None
@@ -85,6 +87,14 @@ def lib():
     attention = [i64, i64, i32, i32, i32, i32] + [i64] * 6 + [i32, f32, i32, vp]
     L.fgms_segment_attention_fwd.argtypes = [vp] * 8 + attention
     L.fgms_segment_attention_bwd.argtypes = [vp] * 11 + attention
+    L.fgms_add_norm_fwd.argtypes = [vp] * 5 + [i64, i32, i64, i64, f32, f32, vp, i32, vp]
+    L.fgms_add_norm_bwd_sums.argtypes = [i64, i32]
+    L.fgms_add_norm_bwd_sums.restype = i64
+    L.fgms_add_norm_bwd.argtypes = [vp] * 8 + [i64, i32, i64, f32, f32, vp, i32, vp]
+    L.fgms_dropout_add.argtypes = [vp] * 3 + [i64, i32, i64, i64, f32, vp, i32, vp]
+    L.fgms_quantize_rows.argtypes = [vp] * 3 + [i64, i32, i64, i64, i32, i32, vp]
+    L.fgms_add_norm_int8.argtypes = [vp] * 6 + [i64, i32, i64, i64, i64, f32, i32, vp]
+    L.fgms_int8_linear.argtypes = [vp] * 6 + [i64, i32, i32, i64, i64, i32, vp]
     L.fgms_profile_enable.argtypes = [i32]
     L.fgms_profile_enable.restype = None
     L.fgms_profile_reset.restype = None
@@ -376,9 +386,9 @@ def wgrad_static(in_feats, out_grad, kernel_grad, kpos, in_map, out_map, plan=No
 _ATTENTION_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
-def _attention_dtype(t):
+def _attention_dtype(t, of="FGMS attention"):
     if t.dtype not in _ATTENTION_DTYPES:
-        raise ValueError("FGMS attention handles float32, float16 and bfloat16 tensors")
+        raise ValueError(of + " handles float32, float16 and bfloat16 tensors")
     return _ATTENTION_DTYPES[t.dtype]
 
 
@@ -456,3 +466,102 @@ def segment_attention_bwd(out_grad, q, k, v, out, lse, q_grad, k_grad, v_grad, q
     rest = _segments(q, k, v, q_offsets, k_offsets, causal, scale)
     _check(lib().fgms_segment_attention_bwd(_p(out_grad), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(q_grad), _p(k_grad), _p(v_grad),
                                             _p(q_offsets), _p(k_offsets), *rest))
+
+
+def _need_features(t, name, like=None, channels=None):
+    """[rows, channels] with the channels of a row side by side."""
+    if not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("%s must be [rows, channels] on the GPU, channels side by side" % name)
+    if like is not None and (t.dtype != like.dtype or t.shape != like.shape):
+        raise ValueError("%s must have the dtype and the shape of x" % name)
+    _attention_dtype(t, "FGMS rows: " + name)
+
+
+def _row(t):
+    return t.stride(0) if t is not None and t.shape[0] > 1 else 0
+
+
+def _seed(seed):
+    _need_shaped(seed, "seed", torch.int64, (2,))
+    return _p(seed)
+
+
+def add_norm_fwd(x, residual, scale, sum, out, eps=1e-6, p=0.0, seed=None):
+    """``fgms_add_norm_fwd``; residual, scale and sum may be None."""
+    _need_features(x, "x")
+    if residual is not None:
+        _need_features(residual, "residual", x)
+    for t, n, like in ((scale, "scale", x.shape[1:]), (sum, "sum", x.shape), (out, "out", x.shape)):
+        _need_shaped(t, n, x.dtype, like)
+    _check(lib().fgms_add_norm_fwd(_p(x), _p(residual), _p(scale), _p(sum), _p(out), x.shape[0], x.shape[1], _row(x), _row(residual), float(eps),
+                                   float(p), _seed(seed), _attention_dtype(x), _stream()))
+
+
+def add_norm_bwd(out_grad, sum_grad, sum, scale, x_grad, residual_grad, scale_grad=None, eps=1e-6, p=0.0, seed=None):
+    """``fgms_add_norm_bwd``: gradients are written; None: not wanted."""
+    _need_features(sum, "sum")
+    for t, n, like in ((out_grad, "out_grad", sum.shape), (sum_grad, "sum_grad", sum.shape), (scale, "scale", sum.shape[1:]),
+                       (x_grad, "x_grad", sum.shape), (residual_grad, "residual_grad", sum.shape), (scale_grad, "scale_grad", sum.shape[1:])):
+        _need_shaped(t, n, sum.dtype, like)
+    n, channels = sum.shape
+    room = torch.empty(lib().fgms_add_norm_bwd_sums(n, channels), device=sum.device) if scale_grad is not None else None
+    _check(lib().fgms_add_norm_bwd(_p(out_grad), _p(sum_grad), _p(sum), _p(scale), _p(x_grad), _p(residual_grad), _p(scale_grad), _p(room), n, channels,
+                                   _row(sum), float(eps), float(p), _seed(seed), _attention_dtype(sum), _stream()))
+
+
+def dropout_add(x, residual, out, p=0.0, seed=None):
+    """``fgms_dropout_add``; residual may be None."""
+    _need_features(x, "x")
+    if residual is not None:
+        _need_features(residual, "residual", x)
+    _need_shaped(out, "out", x.dtype, x.shape)
+    _check(lib().fgms_dropout_add(_p(x), _p(residual), _p(out), x.shape[0], x.shape[1], _row(x), _row(residual), float(p), _seed(seed),
+                                  _attention_dtype(x), _stream()))
+
+
+def _need_eighths(t, name, rows, channels):
+    if not t.is_cuda or t.dtype != torch.int8 or tuple(t.shape) != (rows, channels) or (channels > 1 and t.stride(1) != 1):
+        raise ValueError("%s must be int8 [%d, %d] on the GPU, channels side by side" % (name, rows, channels))
+
+
+def quantize_rows(x, out, scales, gated=False):
+    """``fgms_quantize_rows``: out int8 with rows as far apart as they are, scales fp32."""
+    _need_features(x, "x")
+    n, channels = x.shape[0], x.shape[1] // 2 if gated else x.shape[1]
+    if gated and x.shape[1] % 2:
+        raise ValueError("gated rows hold two halves")
+    _need_eighths(out, "out", n, channels)
+    _need_shaped(scales, "scales", torch.float32, (n,))
+    _check(lib().fgms_quantize_rows(_p(x), _p(out), _p(scales), n, channels, _row(x), max(_row(out), channels), int(gated), _attention_dtype(x), _stream()))
+
+
+def add_norm_int8(x, residual, scale, sum, out, scales, eps=1e-6):
+    """``fgms_add_norm_int8``; residual, scale and sum may be None."""
+    _need_features(x, "x")
+    if residual is not None:
+        _need_features(residual, "residual", x)
+    n, channels = x.shape
+    for t, name, like in ((scale, "scale", x.shape[1:]), (sum, "sum", x.shape)):
+        _need_shaped(t, name, x.dtype, like)
+    _need_eighths(out, "out", n, channels)
+    _need_shaped(scales, "scales", torch.float32, (n,))
+    _check(lib().fgms_add_norm_int8(_p(x), _p(residual), _p(scale), _p(sum), _p(out), _p(scales), n, channels, _row(x), _row(residual),
+                                    max(_row(out), channels), float(eps), _attention_dtype(x), _stream()))
+
+
+def int8_linear(x, x_scales, weight, weight_scales, bias, out):
+    """``fgms_int8_linear``: rows of x and weight on 16 bytes, and the last one's 16 bytes in which its channels end in its storage."""
+    n, channels = x.shape
+    outputs = weight.shape[0]
+    _need_eighths(x, "x", n, channels)
+    _need_eighths(weight, "weight", outputs, channels)
+    least = (channels + 15) // 16 * 16
+    for t, name in ((x, "x"), (weight, "weight")):
+        if t.numel() and t.untyped_storage().nbytes() - t.storage_offset() - (t.shape[0] - 1) * t.stride(0) < least:
+            raise ValueError("the storage of %s ends in front of its last row's 16 bytes" % name)
+    _need_shaped(x_scales, "x_scales", torch.float32, (n,))
+    _need_shaped(weight_scales, "weight_scales", torch.float32, (outputs,))
+    _need_shaped(bias, "bias", out.dtype, (outputs,))
+    _need_shaped(out, "out", out.dtype, (n, outputs))
+    _check(lib().fgms_int8_linear(_p(x), _p(x_scales), _p(weight), _p(weight_scales), _p(bias), _p(out), n, outputs, channels, _row(x) or least,
+                                  _row(weight) or least, _attention_dtype(out, "FGMS rows: out"), _stream()))

@@ -1,0 +1,436 @@
+// Rows of features on their way from one branch of a block to the next:
+//
+//   h = x factor + residual          factor: 1, or with dropout 0 or 1 / (1 - p), from a generator that counts the elements
+//   y = h r w,  r = 1 / sqrt(mean h^2 + eps)
+//   s = max |v| / 127, q = round(v / s)      of a row v: the norm, x itself or silu(a) b
+//   backward:  gs = g_h + r (w g_y - h r^2 mean(w g_y h));  g_residual = gs;  g_x = gs factor;  g_w = sum g_y h r
+//
+// A dozen operations an element: memory is what the kernels have to wait for.  h is rounded to the type before its norm is taken: it is a
+// result, and the backward pass, which reads it, then forms the gradient of the very values that were computed.
+#include "fgms_rows.h"
+
+#include "fgms_internal.h"
+#include "fgms_mma.h"
+
+namespace fgms {
+namespace {
+
+// (an array, whose elements the compiler keeps apart)
+struct Eight {
+  float v[8];
+  __device__ __forceinline__ float &operator[](int e) { return v[e]; }
+  __device__ __forceinline__ float operator[](int e) const { return v[e]; }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f(v[e], e);
+  }
+};
+typedef int8_t byte8v __attribute__((ext_vector_type(8)));
+
+// Sixteen random bits for each of eight neighbouring elements: Philox4x32 with ten rounds (Salmon, Moraes, Dror, Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", SC 2011), counter (chunk, seed[1]), key seed[0].  Word e of a chunk is half e % 2 of the call's number e / 2.
+// (16 bits a word: a call of ten rounds takes some 90 instructions, half of them at a quarter of the rate; with a call for four elements
+// the multiplier, and not memory, would set the pace of 16-bit tensors.  p is met to 2^-17.)
+struct Words {
+  unsigned v[4];
+  __device__ __forceinline__ bool falls(int e, unsigned below) const { return (v[e / 2] >> (16 * (e % 2)) & 0xffffu) < below; }
+};
+__device__ __forceinline__ Words words_of(int64_t chunk, const int64_t *__restrict__ seed) {
+  unsigned k0 = (unsigned)seed[0], k1 = (unsigned)((uint64_t)seed[0] >> 32);
+  unsigned c0 = (unsigned)chunk, c1 = (unsigned)((uint64_t)chunk >> 32), c2 = (unsigned)seed[1], c3 = (unsigned)((uint64_t)seed[1] >> 32);
+#pragma unroll
+  for (int round = 0; round < 10; ++round) {
+    const uint64_t p = (uint64_t)0xD2511F53u * c0, q = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (unsigned)(q >> 32) ^ c1 ^ k0;
+    c1 = (unsigned)q;
+    c2 = (unsigned)(p >> 32) ^ c3 ^ k1;
+    c3 = (unsigned)p;
+    k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
+  }
+  return Words{{c0, c1, c2, c3}};
+}
+
+// Eight channels of a row from `c` on, zeros behind the last.  WHOLE: there are eight, and they begin on 16 bytes.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ Eight load8(const T *__restrict__ row, int c, int channels) {
+  if constexpr (WHOLE) {
+    constexpr int N = 16 / (int)sizeof(T);
+    typedef T Tn __attribute__((ext_vector_type(N)));
+    Eight to;
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+      const Tn from = reinterpret_cast<const Tn *>(row + c)[i];
+#pragma unroll
+      for (int e = 0; e < N; ++e) to[i * N + e] = (float)from[e];
+    }
+    return to;
+  } else {
+    Eight v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < channels ? (float)row[c + e] : 0.f;
+    return v;
+  }
+}
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void store8(T *__restrict__ row, int c, int channels, const Eight &v) {
+  if constexpr (WHOLE) {
+    constexpr int N = 16 / (int)sizeof(T);
+    typedef T Tn __attribute__((ext_vector_type(N)));
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+      Tn to;
+#pragma unroll
+      for (int e = 0; e < N; ++e) to[e] = (T)v[i * N + e];
+      reinterpret_cast<Tn *>(row + c)[i] = to;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < channels) row[c + e] = (T)v[e];
+  }
+}
+__device__ __forceinline__ void add(Eight &to, const Eight &v) {
+  to.each([&](float &t, int e) { t += v[e]; });
+}
+
+// How a row lies on its lanes: lane l of `lanes` (a power of two) has chunks l, l + lanes, ... of eight channels, CHUNKS of them.  A row
+// on a wave or less is summed by exchanges between lanes alone.
+struct Share {
+  int lanes, chunks, threads;
+};
+inline Share share_of(int channels) {
+  const int all = (channels + 7) / 8;
+  if (all > 256) return Share{all > 1024 ? 512 : 256, all > 512 ? 4 : 2, all > 1024 ? 512 : 256};
+  int lanes = 1;
+  while (lanes < 64 && lanes < all) lanes *= 2;
+  return Share{lanes, all > 128 ? 4 : all > 64 ? 2 : 1, 256};
+}
+
+// Sum over / largest of the lanes of a row.  `part`: a number for each wave, not in use by another exchange.
+template <typename V, typename F>
+__device__ __forceinline__ V over_row(V v, int lanes, V *part, F join) {
+  for (int d = 1; d < lanes && d < 64; d *= 2) v = join(v, __shfl_xor(v, d));
+  if (lanes > 64) {
+    const int wave = threadIdx.x / 64, waves = lanes / 64, first = wave / waves * waves;
+    if (threadIdx.x % 64 == 0) part[wave] = v;
+    __syncthreads();
+    v = part[first];
+    for (int w = 1; w < waves; ++w) v = join(v, part[first + w]);
+  }
+  return v;
+}
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+// (of the bits of numbers without their sign, which are in the numbers' order, infinity and then NaN behind the others)
+__device__ __forceinline__ unsigned larger_of(unsigned a, unsigned b) { return a > b ? a : b; }
+
+template <typename T, int CHUNKS, int THREADS, bool WHOLE, int WHAT>
+__global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lanes) {
+  constexpr bool NORM = WHAT == kRowsNorm || WHAT == kRowsNormEighths;
+  __shared__ float sums[THREADS / 64];
+  __shared__ unsigned tops[THREADS / 64];
+  const int lane = threadIdx.x & (lanes - 1);
+  const int64_t row = (int64_t)blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes;
+  const bool there = row < a.n;
+  const int per_row = (a.channels + 7) / 8;
+  const T *const x = (const T *)a.x + row * a.x_row;
+  Eight v[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = 8 * (lane + i * lanes);
+    v[i] = there && c < a.channels ? load8<T, WHOLE>(x, c, a.channels) : Eight{};
+  }
+  if constexpr (WHAT == kRowsGatedEighths) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = 8 * (lane + i * lanes);
+      const Eight b = there && c < a.channels ? load8<T, WHOLE>(x + a.channels, c, a.channels) : Eight{};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] / (1.f + __expf(-v[i][e])) * b[e];
+    }
+  }
+  if constexpr (NORM) {
+    float square = 0.f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = 8 * (lane + i * lanes);
+      if (!there || c >= a.channels) continue;
+      if (a.dropped) {
+        const Words words = words_of(row * per_row + c / 8, a.seed);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = words.falls(e, a.dropped) ? 0.f : v[i][e] * a.back;
+      }
+      if (a.residual) add(v[i], load8<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels));
+      v[i].each([](float &t, int) { t = (float)(T)t; });      // (x itself stays what it is)
+      if (a.sum) store8<T, WHOLE>((T *)a.sum + row * a.channels, c, a.channels, v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) square = __builtin_fmaf(v[i][e], v[i][e], square);
+    }
+    square = over_row(square, lanes, sums, sum_of);
+    const float r = 1.f / __builtin_sqrtf(square / (float)a.channels + a.eps);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = 8 * (lane + i * lanes);
+      if (!there || c >= a.channels) continue;
+      v[i].each([&](float &t, int) { t *= r; });
+      if (a.scale) {
+        const Eight w = load8<T, WHOLE>((const T *)a.scale, c, a.channels);
+        v[i].each([&](float &t, int e) { t *= w[e]; });
+      }
+      if constexpr (WHAT == kRowsNorm) store8<T, WHOLE>((T *)a.out + row * a.channels, c, a.channels, v[i]);
+    }
+  }
+  if constexpr (WHAT != kRowsNorm) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float value = v[i][e];
+        top = larger_of(top, __builtin_bit_cast(unsigned, value) & 0x7fffffffu);
+      }
+    top = over_row(top, lanes, tops, larger_of);
+    // A row with an infinity or NaN stands for NaN in every channel, one whose step would be no normal number for zeros.
+    const bool finite = top < 0x7f800000u;
+    const float most = __builtin_bit_cast(float, top), step = most / 127.f;
+    const bool some = finite && step >= 0x1p-126f;
+    const float by = some ? 1.f / step : 0.f;
+    if (there && lane == 0) a.scales[row] = some ? step : finite ? 0.f : __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = 8 * (lane + i * lanes);
+      if (!there || c >= a.channels) continue;
+      byte8v q;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // (the quotient to its last bit: halves are met where they are meant)
+        const float value = v[i][e], near = value * by, quotient = __builtin_fmaf(__builtin_fmaf(-near, step, value), by, near);
+        q[e] = some ? (int8_t)(int)__builtin_rintf(quotient) : (int8_t)0;
+      }
+      int8_t *const to = a.eighths + row * a.eighths_row + c;
+      if constexpr (WHOLE) {
+        *reinterpret_cast<byte8v *>(to) = q;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < a.channels) to[e] = q[e];
+      }
+    }
+  }
+}
+
+// A workgroup goes through the rows in steps of the grid and keeps its lanes' sums of the scale's gradient in registers.
+template <typename T, int CHUNKS, int THREADS, bool WHOLE>
+__global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a, int lanes) {
+  __shared__ float parts[2][2][THREADS / 64];
+  __shared__ Eight all[THREADS == 256 ? CHUNKS * 256 : 1];
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = THREADS / lanes, per_row = (a.channels + 7) / 8;
+  Eight w[CHUNKS], gw[CHUNKS] = {};
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = 8 * (lane + i * lanes);
+    w[i] = a.scale && c < a.channels ? load8<T, WHOLE>((const T *)a.scale, c, a.channels) : Eight{{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f}};
+  }
+  int turn = 0;      // (a row's exchanges and the next one's do not share their places)
+  for (int64_t first = (int64_t)blockIdx.x * groups; first < a.n; first += (int64_t)gridDim.x * groups, turn ^= 1) {
+    const int64_t row = first + group;
+    const bool there = row < a.n;
+    Eight h[CHUNKS], g[CHUNKS];
+    float square = 0.f, along = 0.f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = 8 * (lane + i * lanes);
+      const bool here = there && c < a.channels;
+      h[i] = here ? load8<T, WHOLE>((const T *)a.sum + row * a.x_row, c, a.channels) : Eight{};
+      g[i] = here ? load8<T, WHOLE>((const T *)a.g_out + row * a.channels, c, a.channels) : Eight{};
+    }
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        square = __builtin_fmaf(h[i][e], h[i][e], square);
+        along = __builtin_fmaf(w[i][e] * g[i][e], h[i][e], along);
+      }
+    square = over_row(square, lanes, parts[turn][0], sum_of);
+    along = over_row(along, lanes, parts[turn][1], sum_of);
+    const float r = 1.f / __builtin_sqrtf(square / (float)a.channels + a.eps), back = r * r * (along / (float)a.channels);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = 8 * (lane + i * lanes);
+      if (!there || c >= a.channels) continue;
+      Eight gs;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        gw[i][e] = __builtin_fmaf(g[i][e] * r, h[i][e], gw[i][e]);
+        gs[e] = r * (w[i][e] * g[i][e] - h[i][e] * back);
+      }
+      if (a.g_sum) add(gs, load8<T, WHOLE>((const T *)a.g_sum + row * a.channels, c, a.channels));
+      if (a.g_residual) store8<T, WHOLE>((T *)a.g_residual + row * a.channels, c, a.channels, gs);
+      if (a.gx) {
+        if (a.dropped) {
+          const Words words = words_of(row * per_row + c / 8, a.seed);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) gs[e] = words.falls(e, a.dropped) ? 0.f : gs[e] * a.back;
+        }
+        store8<T, WHOLE>((T *)a.gx + row * a.channels, c, a.channels, gs);
+      }
+    }
+  }
+  if (!a.scale_sums) return;
+  // the groups of lanes, in their order
+  float *const to = a.scale_sums + (int64_t)blockIdx.x * a.channels;
+  if (groups > 1) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) all[i * 256 + threadIdx.x] = gw[i];
+    __syncthreads();
+    if (group) return;
+    for (int other = 1; other < groups; ++other)
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) add(gw[i], all[i * 256 + other * lanes + lane]);
+  }
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int c = 8 * (lane + i * lanes);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < a.channels) to[c + e] = gw[i][e];
+  }
+}
+
+// out[channel] = the workgroups' sums, eight channels a workgroup, 32 threads each, in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_kernel(const float *__restrict__ sums, int64_t groups, int channels, T *__restrict__ out) {
+  __shared__ float part[4][8];
+  const int c = threadIdx.x % 8, column = blockIdx.x * 8 + c;
+  float sum = 0.f;
+  if (column < channels)
+#pragma unroll 8
+    for (int64_t b = threadIdx.x / 8; b < groups; b += 32) sum += sums[b * channels + column];
+  for (int d = 8; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if (threadIdx.x % 64 < 8) part[threadIdx.x / 64][c] = sum;
+  __syncthreads();
+  if (threadIdx.x < 8 && column < channels) out[column] = (T)(part[0][c] + part[1][c] + part[2][c] + part[3][c]);
+}
+
+// Eight elements a thread, counted through the rows.
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void dropout_add_kernel(const RowsArgs a, int64_t chunks) {
+  const int per_row = (a.channels + 7) / 8;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= chunks) return;
+  const int64_t row = at / per_row;
+  const int c = 8 * (int)(at - row * per_row);
+  Eight v = load8<T, WHOLE>((const T *)a.x + row * a.x_row, c, a.channels);
+  if (a.dropped) {
+    const Words words = words_of(at, a.seed);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = words.falls(e, a.dropped) ? 0.f : v[e] * a.back;
+  }
+  if (a.residual) add(v, load8<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels));
+  store8<T, WHOLE>((T *)a.out + row * a.channels, c, a.channels, v);
+}
+
+// --- launches --------------------------------------------------------------------------------------------------
+template <int N> struct Number { static constexpr int value = N; };
+template <int CHUNKS, int THREADS> struct Shape {
+  static constexpr int chunks = CHUNKS, threads = THREADS;
+};
+template <typename F>
+int by_share(const Share &s, F f) {
+  if (s.threads == 512) return f(Shape<4, 512>());
+  return s.chunks == 1 ? f(Shape<1, 256>()) : s.chunks == 2 ? f(Shape<2, 256>()) : f(Shape<4, 256>());
+}
+template <typename F>
+int by_type(int dtype, F f) {
+  return dtype == FGMS_F32 ? f(float()) : dtype == FGMS_F16 ? f((_Float16)0) : f((__bf16)0);
+}
+
+inline int grid_of(int64_t blocks, unsigned *grid) {
+  if (blocks > 0x7fffffff) {
+    set_error("%lld workgroups are more than one launch takes", (long long)blocks);
+    return FGMS_E_INVALID;
+  }
+  *grid = (unsigned)blocks;
+  return FGMS_OK;
+}
+
+// Rows that all begin on 16 bytes and are whole chunks of eight channels are read and written 16 bytes at a time, others element by element.
+bool whole(const void *p, int64_t row, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0; }
+bool whole_rows(const RowsArgs &a) {
+  const int size = a.dtype == FGMS_F32 ? 4 : 2;
+  bool ok = a.channels % 8 == 0 && whole(a.x, a.x_row, size) && whole(a.sum, a.x_row, size) && (!a.residual || whole(a.residual, a.residual_row, size));
+  for (const void *p : {a.scale, (const void *)a.out, a.g_out, a.g_sum, (const void *)a.gx, (const void *)a.g_residual}) ok = ok && whole(p, 0, size);
+  return ok && reinterpret_cast<uintptr_t>(a.eighths) % 8 == 0 && a.eighths_row % 8 == 0;
+}
+
+}  // namespace
+
+int launch_rows(const RowsArgs &a, int what) {
+  const Share s = share_of(a.channels);
+  const int at_once = s.threads / s.lanes;
+  unsigned grid;
+  const int rc = grid_of((a.n + at_once - 1) / at_once, &grid);
+  if (rc != FGMS_OK) return rc;
+  const bool w = whole_rows(a);
+  by_type(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_share(s, [&](auto shape) {
+      constexpr int K = decltype(shape)::chunks, N = decltype(shape)::threads;
+      const auto launch = [&](auto kind) {
+        constexpr int WHAT = decltype(kind)::value;
+        if (w) rows_kernel<T, K, N, true, WHAT><<<grid, N, 0, a.stream>>>(a, s.lanes);
+        else rows_kernel<T, K, N, false, WHAT><<<grid, N, 0, a.stream>>>(a, s.lanes);
+      };
+      if (what == kRowsNorm) launch(Number<kRowsNorm>());
+      else if (what == kRowsNormEighths) launch(Number<kRowsNormEighths>());
+      else if (what == kRowsEighths) launch(Number<kRowsEighths>());
+      else launch(Number<kRowsGatedEighths>());
+      return FGMS_OK;
+    });
+  });
+  FGMS_HIP_TRY(hipGetLastError());
+  return FGMS_OK;
+}
+
+int64_t scale_grad_groups(int64_t n, int channels) {
+  const Share s = share_of(channels);
+  const int at_once = s.threads / s.lanes;
+  const int64_t all = (n + at_once - 1) / at_once, most = 1024;
+  return all < most ? all : most;
+}
+
+int launch_add_norm_bwd(const RowsArgs &a) {
+  const Share s = share_of(a.channels);
+  const unsigned grid = (unsigned)scale_grad_groups(a.n, a.channels);
+  const bool w = whole_rows(a);
+  by_type(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_share(s, [&](auto shape) {
+      constexpr int K = decltype(shape)::chunks, N = decltype(shape)::threads;
+      if (w) add_norm_grad_kernel<T, K, N, true><<<grid, N, 0, a.stream>>>(a, s.lanes);
+      else add_norm_grad_kernel<T, K, N, false><<<grid, N, 0, a.stream>>>(a, s.lanes);
+      if (a.g_scale) column_sums_kernel<T><<<(a.channels + 7) / 8, 256, 0, a.stream>>>(a.scale_sums, grid, a.channels, (T *)a.g_scale);
+      return FGMS_OK;
+    });
+  });
+  FGMS_HIP_TRY(hipGetLastError());
+  return FGMS_OK;
+}
+
+int launch_dropout_add(const RowsArgs &a) {
+  const int64_t chunks = a.n * ((a.channels + 7) / 8);
+  unsigned grid;
+  const int rc = grid_of((chunks + 255) / 256, &grid);
+  if (rc != FGMS_OK) return rc;
+  const bool w = whole_rows(a);
+  by_type(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    if (w) dropout_add_kernel<T, true><<<grid, 256, 0, a.stream>>>(a, chunks);
+    else dropout_add_kernel<T, false><<<grid, 256, 0, a.stream>>>(a, chunks);
+    return FGMS_OK;
+  });
+  FGMS_HIP_TRY(hipGetLastError());
+  return FGMS_OK;
+}
+
+}  // namespace fgms

@@ -44,6 +44,7 @@
 #include "fgms.h"
 #include "fgms_diag.h"
 #include "fgms_torch_attention.h"
+#include "fgms_torch_block.h"
 
 namespace {
 
@@ -545,6 +546,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sparse_conv", &sparse_conv);
   m.def("norm_rotary", &norm_rotary);
   m.def("segment_attention", &segment_attention);
+  m.def("add_norm", &add_norm);
+  m.def("dropout_add", &dropout_add);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("add_norm_int8", &add_norm_int8);
+  m.def("int8_linear", &int8_linear);
   m.def("fgms_fusion_fwd_cuda", &ConvolutionForwardFused);
   m.def("fgms_fwd_cuda", &ConvolutionForward);
   m.def("fgms_bwd_cuda", &ConvolutionBackward);

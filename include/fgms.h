@@ -348,6 +348,57 @@ int fgms_segment_attention_bwd(const void *out_grad, const void *q, const void *
                                int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                                int64_t v_row, int64_t v_head, int causal, float scale, int dtype, void *stream);
 
+/*
+ * What goes around attention in a block: a branch joins the residual stream, and the sum's norm goes into the next branch; at inference the
+ * rows go there in 8 bits, with a scale each.  No counterpart in the reference.  Types: FGMS_F32, FGMS_F16, FGMS_BF16.  Rows of 1 to 16384 channels,
+ * which lie side by side; row strides in ELEMENTS; results and gradients are contiguous unless they have a stride.  Rows that all begin
+ * on 16 bytes and hold a multiple of 8 channels are read 16 bytes at a time, any others element by element.  Sums, norms and maxima are fp32.
+ */
+
+/*
+ *   h = x f + residual, rounded to the type;  y = h scale / sqrt(mean(h^2) + eps), of h as rounded
+ * f: 1, or with p > 0 (dropout) 0 for a share p of the elements and 1 / (1 - p) for the others (p in steps of 2^-16).
+ *   - x, residual [n, channels] (residual NULL: none), scale [channels] (NULL: ones); sum: h (NULL: not wanted), out: y
+ *   - seed: int64 [2], device, read by the kernels (a captured call replays with what stands there then); unused where p is 0.  Which
+ *     elements fall follows from seed and their places alone: Philox4x32-10 (Salmon, Moraes, Dror, Shaw, SC 2011), key seed[0], counter
+ *     (row * ceil(channels / 8) + channel / 8, seed[1]); half e % 2 of word e / 2 of the result is channel e = channel % 8's, which falls if
+ *     it is below rint(p * 65536).  No mask is stored; the backward call takes the same seed.
+ * The backward call reads sum (sum_row apart; x itself where there is neither a residual nor dropout) and the gradients of y (out_grad)
+ * and of h (sum_grad, NULL: none), and writes those that are not NULL: x_grad, residual_grad (without dropout x's too: ask for one of
+ * them), scale_grad, which needs scale_sums, fp32, fgms_add_norm_bwd_sums(n, channels) of them.  The same bits every time.
+ */
+int fgms_add_norm_fwd(const void *x, const void *residual, const void *scale, void *sum, void *out, int64_t n, int channels,
+                      int64_t x_row, int64_t residual_row, float eps, float p, const int64_t *seed, int dtype, void *stream);
+int64_t fgms_add_norm_bwd_sums(int64_t n, int channels);
+int fgms_add_norm_bwd(const void *out_grad, const void *sum_grad, const void *sum, const void *scale, void *x_grad,
+                      void *residual_grad, void *scale_grad, float *scale_sums, int64_t n, int channels, int64_t sum_row,
+                      float eps, float p, const int64_t *seed, int dtype, void *stream);
+
+/* out = x f + residual, as above.  Its gradients are the call on the gradient without a residual, and the gradient itself. */
+int fgms_dropout_add(const void *x, const void *residual, void *out, int64_t n, int channels, int64_t x_row,
+                     int64_t residual_row, float p, const int64_t *seed, int dtype, void *stream);
+
+/*
+ * Rows in 8 bits: scales[i] = max |v| / 127, out[i][c] = v[c] / scales[i] to the nearest whole number, even ones first, of
+ *   fgms_quantize_rows: v = x, or with gated != 0 v = silu(a) b of rows (a, b) of 2 * channels
+ *   fgms_add_norm_int8: v = y of fgms_add_norm_fwd (before it is rounded to the type), without dropout
+ * out_row: bytes, channels at least; what lies between the rows stays.  A row with an infinity or NaN has scale NaN and zeros, one
+ * whose scale would be below 2^-126 scale 0 and zeros.
+ */
+int fgms_quantize_rows(const void *x, int8_t *out, float *scales, int64_t n, int channels, int64_t x_row, int64_t out_row,
+                       int gated, int dtype, void *stream);
+int fgms_add_norm_int8(const void *x, const void *residual, const void *scale, void *sum, int8_t *out, float *scales, int64_t n,
+                       int channels, int64_t x_row, int64_t residual_row, int64_t out_row, float eps, int dtype, void *stream);
+
+/*
+ *   out[i][o] = x_scales[i] weight_scales[o] sum_k x[i][k] weight[o][k] + bias[o]
+ * x [n, channels], weight [outputs, channels], int8, 1 to 131071 channels; out [n, outputs] and bias (NULL: none) of `dtype`.  The sums are
+ * exact.  x_row, weight_row: bytes, a multiple of 16 and at least the channels, 4 MB at most; rows begin on 16 bytes, and the last one's
+ * 16 bytes in which its channels end belong to the tensor (what stands behind the channels does not count).
+ */
+int fgms_int8_linear(const int8_t *x, const float *x_scales, const int8_t *weight, const float *weight_scales, const void *bias,
+                     void *out, int64_t n, int outputs, int channels, int64_t x_row, int64_t weight_row, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
