@@ -46,7 +46,8 @@ struct Stager {
     for (int i = 0; i < PER; ++i) offset[i] = (unsigned)(row + i * (THREADS / kChunks)) * (unsigned)stride + chunk * 16;
   }
   __device__ __forceinline__ void load(int4v *tile, int k, int depth) const {
-    const __amdgpu_buffer_rsrc_t rows = rows_resource(base + k, range > (unsigned)k ? range - k : 0);
+    // (a range that the compiler does not know to be the wave's would have every load looped over lane by lane)
+    const __amdgpu_buffer_rsrc_t rows = rows_resource(base + k, (unsigned)__builtin_amdgcn_readfirstlane(max((int)range - k, 0)));
     const bool there = k + chunk * 16 < depth;
 #pragma unroll
     for (int i = 0; i < PER; ++i) load_to_lds(rows, tile + wave * 64 + i * THREADS, there ? offset[i] : kAbsentRow);
@@ -109,21 +110,51 @@ __device__ __forceinline__ void store_block(T *to, const int16v &acc, float by, 
   }
 }
 
-// acc += the products of a tile, 32 NB outputs by 32 MB rows.  at: where a lane reads its chunks of the first 32 rows.
+// A lane's chunks of 32 of a tile's 128 bytes, for 32 MB rows of x and 32 NB outputs.
 template <int MB, int NB>
-__device__ __forceinline__ void multiply(int16v (&acc)[NB][MB], const int4v *x_tile, const int4v *w_tile, const int (&at)[kDepth / 32]) {
+struct Fragments {
+  int4v x[MB], w[NB];
+  __device__ __forceinline__ void read(const int4v *x_tile, const int4v *w_tile, int at) {
 #pragma unroll
-  for (int s = 0; s < kDepth / 32; ++s) {
-    int4v xf[MB], wf[NB];
+    for (int i = 0; i < MB; ++i) x[i] = x_tile[32 * i * kChunks + at];
 #pragma unroll
-    for (int i = 0; i < MB; ++i) xf[i] = x_tile[32 * i * kChunks + at[s]];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) wf[j] = w_tile[32 * j * kChunks + at[s]];
+    for (int j = 0; j < NB; ++j) w[j] = w_tile[32 * j * kChunks + at];
+  }
+  __device__ __forceinline__ void multiply(int16v (&acc)[NB][MB]) const {
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+      for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[j], x[i], acc[j][i], 0, 0, 0);
   }
+};
+
+// The next chunks are read while these are multiplied, a read between every few products.
+template <int MB, int NB>
+__device__ __forceinline__ void step(int16v (&acc)[NB][MB], const Fragments<MB, NB> &now, Fragments<MB, NB> &next, const int4v *x_tile, const int4v *w_tile,
+                                     int at) {
+  next.read(x_tile, w_tile, at);
+  now.multiply(acc);
+#pragma unroll
+  for (int i = 0; i < MB + NB; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                  // a read of LDS
+    __builtin_amdgcn_sched_group_barrier(0x008, MB * NB > 8 ? 2 : 1, 0);                // products
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A tile of 128 bytes of depth, whose first chunks are in `first` already, and the next one's first chunks; `load` asks for the one after, into
+// this one's place, as soon as all waves have read theirs.
+template <int MB, int NB, typename L>
+__device__ __forceinline__ void turn(int16v (&acc)[NB][MB], Fragments<MB, NB> &first, const int4v *x_now, const int4v *w_now, const int4v *x_next,
+                                     const int4v *w_next, const int (&at)[kDepth / 32], const L &load) {
+  Fragments<MB, NB> other;
+  step(acc, first, other, x_now, w_now, at[1]);
+  step(acc, other, first, x_now, w_now, at[2]);
+  step(acc, first, other, x_now, w_now, at[3]);
+  tiles_ready();
+  load();
+  __builtin_amdgcn_sched_barrier(0);
+  step(acc, other, first, x_next, w_next, at[0]);
 }
 
 // 64 MB rows of x by 64 NB outputs to a workgroup of four waves, 32 MB by 32 NB to a wave.
@@ -159,19 +190,32 @@ __global__ __launch_bounds__(256, (MB * NB >= 16 ? 1 : 2)) void int8_linear_kern
     __syncthreads();
   }
   // (no choice in the loop: the accumulators would be moved from registers to registers)
+  const int4v *const x0_now = x_tile0 + x0 * kChunks, *const w0_now = w_tile0 + w0 * kChunks;
+  const int4v *const x1_now = x_tile1 + x0 * kChunks, *const w1_now = w_tile1 + w0 * kChunks;
+  const auto k_of = [&](int tile) { return tile < tiles ? (tile - 1) * kDepth : a.depth; };
+  x.load(x_tile1, k_of(1), a.depth);
+  w.load(w_tile1, k_of(1), a.depth);
+  Fragments<MB, NB> first;
+  first.read(x0_now, w0_now, at[0]);
   int i = 0;
   for (; i + 1 < tiles; i += 2) {
-    x.load(x_tile1, i * kDepth, a.depth);
-    w.load(w_tile1, i * kDepth, a.depth);
-    multiply<MB, NB>(acc, x_tile0 + x0 * kChunks, w_tile0 + w0 * kChunks, at);
-    tiles_ready();
-    const int k = i + 2 < tiles ? (i + 1) * kDepth : a.depth;
-    x.load(x_tile0, k, a.depth);
-    w.load(w_tile0, k, a.depth);
-    multiply<MB, NB>(acc, x_tile1 + x0 * kChunks, w_tile1 + w0 * kChunks, at);
-    tiles_ready();
+    turn(acc, first, x0_now, w0_now, x1_now, w1_now, at, [&] {
+      x.load(x_tile0, k_of(i + 2), a.depth);
+      w.load(w_tile0, k_of(i + 2), a.depth);
+    });
+    turn(acc, first, x1_now, w1_now, x0_now, w0_now, at, [&] {
+      x.load(x_tile1, k_of(i + 3), a.depth);
+      w.load(w_tile1, k_of(i + 3), a.depth);
+    });
   }
-  if (i < tiles) multiply<MB, NB>(acc, x_tile0 + x0 * kChunks, w_tile0 + w0 * kChunks, at);
+  if (i < tiles) {
+    Fragments<MB, NB> other;
+    step(acc, first, other, x0_now, w0_now, at[1]);
+    step(acc, other, first, x0_now, w0_now, at[2]);
+    step(acc, first, other, x0_now, w0_now, at[3]);
+    other.multiply(acc);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);      // (the zeros asked for behind the last tile: their place is used again)
   // scales and bias of the workgroup's outputs by way of LDS
   __syncthreads();
   float *const scales = (float *)w_tile0, *const biases = scales + WR;
