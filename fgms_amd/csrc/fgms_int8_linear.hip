@@ -45,12 +45,14 @@ struct Stager {
 #pragma unroll
     for (int i = 0; i < PER; ++i) offset[i] = (unsigned)(row + i * (THREADS / kChunks)) * (unsigned)stride + chunk * 16;
   }
-  __device__ __forceinline__ void load(int4v *tile, int k, int depth) const {
+  // shares [from, to) of PER
+  __device__ __forceinline__ void load(int4v *tile, int k, int depth, int from = 0, int to = PER) const {
     // (a range that the compiler does not know to be the wave's would have every load looped over lane by lane)
     const __amdgpu_buffer_rsrc_t rows = rows_resource(base + k, (unsigned)__builtin_amdgcn_readfirstlane(max((int)range - k, 0)));
     const bool there = k + chunk * 16 < depth;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) load_to_lds(rows, tile + wave * 64 + i * THREADS, there ? offset[i] : kAbsentRow);
+    for (int i = 0; i < PER; ++i)
+      if (i >= from && i < to) load_to_lds(rows, tile + wave * 64 + i * THREADS, there ? offset[i] : kAbsentRow);
   }
 };
 
@@ -128,33 +130,36 @@ struct Fragments {
   }
 };
 
-// The next chunks are read while these are multiplied, a read between every few products.
-template <int MB, int NB>
+// The next chunks are read while these are multiplied, and LOADS loads asked for: one of each between every few products.
+template <int LOADS, int MB, int NB, typename L>
 __device__ __forceinline__ void step(int16v (&acc)[NB][MB], const Fragments<MB, NB> &now, Fragments<MB, NB> &next, const int4v *x_tile, const int4v *w_tile,
-                                     int at) {
+                                     int at, const L &load) {
   next.read(x_tile, w_tile, at);
+  load();
   now.multiply(acc);
 #pragma unroll
   for (int i = 0; i < MB + NB; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                  // a read of LDS
-    __builtin_amdgcn_sched_group_barrier(0x008, MB * NB > 8 ? 2 : 1, 0);                // products
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                              // a read of LDS
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                              // a product
+    if (i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);               // a load
+    if (MB * NB > 8) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
   }
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// A tile of 128 bytes of depth, whose first chunks are in `first` already, and the next one's first chunks; `load` asks for the one after, into
-// this one's place, as soon as all waves have read theirs.
-template <int MB, int NB, typename L>
+// A tile of 128 bytes of depth, whose first chunks are in `first` already, and the next one's first chunks.  load(0) and load(1) ask for the
+// halves of the one after the next: x's rows into this one's place as soon as all waves have read theirs, the weights' during the next one's first step.
+template <int MB, int NB, typename L0, typename L1>
 __device__ __forceinline__ void turn(int16v (&acc)[NB][MB], Fragments<MB, NB> &first, const int4v *x_now, const int4v *w_now, const int4v *x_next,
-                                     const int4v *w_next, const int (&at)[kDepth / 32], const L &load) {
+                                     const int4v *w_next, const int (&at)[kDepth / 32], const L0 &load_rest, const L1 &load) {
+  const auto none = [] {};
   Fragments<MB, NB> other;
-  step(acc, first, other, x_now, w_now, at[1]);
-  step(acc, other, first, x_now, w_now, at[2]);
-  step(acc, first, other, x_now, w_now, at[3]);
+  step<2 * NB>(acc, first, other, x_now, w_now, at[1], load_rest);
+  step<0>(acc, other, first, x_now, w_now, at[2], none);
+  step<0>(acc, first, other, x_now, w_now, at[3], none);
   tiles_ready();
-  load();
   __builtin_amdgcn_sched_barrier(0);
-  step(acc, other, first, x_next, w_next, at[0]);
+  step<2 * MB>(acc, other, first, x_next, w_next, at[0], load);
 }
 
 // 64 MB rows of x by 64 NB outputs to a workgroup of four waves, 32 MB by 32 NB to a wave.
@@ -194,25 +199,19 @@ __global__ __launch_bounds__(256, (MB * NB >= 16 ? 1 : 2)) void int8_linear_kern
   const int4v *const x1_now = x_tile1 + x0 * kChunks, *const w1_now = w_tile1 + w0 * kChunks;
   const auto k_of = [&](int tile) { return tile < tiles ? (tile - 1) * kDepth : a.depth; };
   x.load(x_tile1, k_of(1), a.depth);
-  w.load(w_tile1, k_of(1), a.depth);
   Fragments<MB, NB> first;
   first.read(x0_now, w0_now, at[0]);
   int i = 0;
   for (; i + 1 < tiles; i += 2) {
-    turn(acc, first, x0_now, w0_now, x1_now, w1_now, at, [&] {
-      x.load(x_tile0, k_of(i + 2), a.depth);
-      w.load(w_tile0, k_of(i + 2), a.depth);
-    });
-    turn(acc, first, x1_now, w1_now, x0_now, w0_now, at, [&] {
-      x.load(x_tile1, k_of(i + 3), a.depth);
-      w.load(w_tile1, k_of(i + 3), a.depth);
-    });
+    turn(acc, first, x0_now, w0_now, x1_now, w1_now, at, [&] { w.load(w_tile1, k_of(i + 1), a.depth); }, [&] { x.load(x_tile0, k_of(i + 2), a.depth); });
+    turn(acc, first, x1_now, w1_now, x0_now, w0_now, at, [&] { w.load(w_tile0, k_of(i + 2), a.depth); }, [&] { x.load(x_tile1, k_of(i + 3), a.depth); });
   }
   if (i < tiles) {
+    const auto none = [] {};
     Fragments<MB, NB> other;
-    step(acc, first, other, x0_now, w0_now, at[1]);
-    step(acc, other, first, x0_now, w0_now, at[2]);
-    step(acc, first, other, x0_now, w0_now, at[3]);
+    step<0>(acc, first, other, x0_now, w0_now, at[1], none);
+    step<0>(acc, other, first, x0_now, w0_now, at[2], none);
+    step<0>(acc, first, other, x0_now, w0_now, at[3], none);
     other.multiply(acc);
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);      // (the zeros asked for behind the last tile: their place is used again)
