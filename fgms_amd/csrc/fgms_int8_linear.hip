@@ -13,12 +13,12 @@ namespace {
 
 typedef int int16v __attribute__((ext_vector_type(16)));
 
-constexpr int kDepth = 128, kChunks = kDepth / 16;      // bytes of a row, and 16-byte chunks, to a tile in LDS
-
-// Where chunk c of a tile's row lies.  A fragment is read by 32 lanes that ask 32 rows for the same chunk: this way they cover all banks.  (The
-// same for rows 32 apart.)
-__device__ __forceinline__ int swizzle(int row) { return ((row & 2) << 1) | ((row >> 2) & 3); }
-__device__ __forceinline__ int chunk_at(int row, int c) { return row * kChunks + (c ^ swizzle(row)); }
+// Where chunk c of a tile's row of DEPTH bytes lies.  A fragment is read by 32 lanes that ask 32 rows for the same chunk: this way they cover all
+// banks.  (The same for rows 32 apart.)
+template <int DEPTH>
+__device__ __forceinline__ int swizzle(int row) { return DEPTH == 128 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3; }
+template <int DEPTH>
+__device__ __forceinline__ int chunk_at(int row, int c) { return row * (DEPTH / 16) + (c ^ swizzle<DEPTH>(row)); }
 
 // 16 bytes a lane from a buffer to LDS, one lane's behind the other's from `to` on (the same for all lanes).
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *to, unsigned offset) {
@@ -28,31 +28,29 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, int4v *
 
 // Rows of a tensor on their way to a tile in LDS, past the registers: every lane asks for the chunk that belongs where its 16 bytes land; rows
 // behind the last are out of the buffer's range and arrive as zeros, and so do chunks behind the channels, which are asked for out of range.
-template <int ROWS, int THREADS>
+template <int ROWS, int DEPTH>
 struct Stager {
-  static constexpr int PER = ROWS * kChunks / THREADS;
+  static constexpr int THREADS = 256, kChunks = DEPTH / 16, PER = ROWS * kChunks / THREADS;
   const int8_t *base;
   unsigned range, offset[PER];
   int wave, chunk;      // (rows of a lane lie THREADS / kChunks apart, a multiple of 16: their chunks are the same)
   __device__ __forceinline__ void open(const int8_t *from, int64_t first, int64_t count, int64_t stride, int depth) {
     static_assert(THREADS / kChunks % 16 == 0, "");
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % (THREADS / 64));
     base = from + first * stride;
     const int there = (int)min((int64_t)ROWS, count - first);
     range = (unsigned)(there - 1) * (unsigned)stride + (unsigned)((depth + 15) & ~15);
-    const int row = threadIdx.x / kChunks;
-    chunk = (threadIdx.x % kChunks) ^ swizzle(row);
+    const int row = threadIdx.x % THREADS / kChunks;
+    chunk = (threadIdx.x % kChunks) ^ swizzle<DEPTH>(row);
 #pragma unroll
     for (int i = 0; i < PER; ++i) offset[i] = (unsigned)(row + i * (THREADS / kChunks)) * (unsigned)stride + chunk * 16;
   }
-  // shares [from, to) of PER
-  __device__ __forceinline__ void load(int4v *tile, int k, int depth, int from = 0, int to = PER) const {
+  __device__ __forceinline__ void load(int4v *tile, int k, int depth) const {
     // (a range that the compiler does not know to be the wave's would have every load looped over lane by lane)
     const __amdgpu_buffer_rsrc_t rows = rows_resource(base + k, (unsigned)__builtin_amdgcn_readfirstlane(max((int)range - k, 0)));
     const bool there = k + chunk * 16 < depth;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i >= from && i < to) load_to_lds(rows, tile + wave * 64 + i * THREADS, there ? offset[i] : kAbsentRow);
+    for (int i = 0; i < PER; ++i) load_to_lds(rows, tile + wave * 64 + i * THREADS, there ? offset[i] : kAbsentRow);
   }
 };
 
@@ -79,48 +77,52 @@ __device__ __forceinline__ void swap_halves(int &a, int &b) {
   a = (int)r[0], b = (int)r[1];
 }
 
-// Results of a block of 32 outputs by 32 rows of x (register 4 p + e of lane l: output 8 p + 4 (l / 32) + e, row l % 32).
+// Results of a block of 32 outputs by 32 rows of x (register 4 p + e of lane l: output 8 p + 4 (l / 32) + e, row l % 32), `there` of the outputs, 16
+// bytes at a time wherever these begin.
 template <typename T>
-__device__ __forceinline__ void store_block(T *to, const int16v &acc, float by, const float4v (&w)[4], const float4v (&b)[4], int there, bool whole, int lane) {
+__device__ __forceinline__ void store_block(T *to, const int16v &acc, float by, const float4v (&w)[4], const float4v (&b)[4], int there, int lane) {
+  constexpr int N = 16 / (int)sizeof(T);
+  typedef T Tn __attribute__((ext_vector_type(N)));
+  typedef Tn Anywhere __attribute__((aligned(sizeof(T))));
   float4v v[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[p][e] = (float)acc[4 * p + e] * by * w[p][e] + b[p][e];
-  if (!whole) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (8 * p + 4 * (lane / 32) + e < there) to[8 * p + 4 * (lane / 32) + e] = (T)v[p][e];
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-      if (8 * p + 4 * (lane / 32) < there) *reinterpret_cast<float4v *>(to + 8 * p + 4 * (lane / 32)) = v[p];
-  } else {
-    // eight outputs side by side: a lane takes its partner's four for one pair of p, and gives it four of the other
-    typedef T T4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int p = 0; p < 4; p += 2) {
+  for (int p = 0; p < 4; p += N / 4) {
+    Tn all;
+    int at;
+    if constexpr (N == 4) {
+      all = v[p], at = 8 * p + 4 * (lane / 32);
+    } else {
+      // eight outputs side by side: a lane takes its partner's four for one p, and gives it four of the other
+      typedef T T4 __attribute__((ext_vector_type(4)));
       const int2v lo = __builtin_bit_cast(int2v, __builtin_convertvector(v[p], T4)), hi = __builtin_bit_cast(int2v, __builtin_convertvector(v[p + 1], T4));
       int a = lo[0], b = lo[1], c = hi[0], d = hi[1];
       swap_halves(a, c);
       swap_halves(b, d);
-      const int at = 8 * p + 8 * (lane / 32);
-      if (at < there) *reinterpret_cast<int4v *>(to + at) = int4v{a, b, c, d};
+      all = __builtin_bit_cast(Tn, int4v{a, b, c, d}), at = 8 * p + 8 * (lane / 32);
+    }
+    if (at + N <= there) {
+      *reinterpret_cast<Anywhere *>(to + at) = all;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (at + e < there) to[at + e] = all[e];
     }
   }
 }
 
-// A lane's chunks of 32 of a tile's 128 bytes, for 32 MB rows of x and 32 NB outputs.
-template <int MB, int NB>
+// A lane's chunks of 32 bytes of a tile's depth, for 32 MB rows of x and 32 NB outputs.
+template <int MB, int NB, int DEPTH>
 struct Fragments {
   int4v x[MB], w[NB];
   __device__ __forceinline__ void read(const int4v *x_tile, const int4v *w_tile, int at) {
 #pragma unroll
-    for (int i = 0; i < MB; ++i) x[i] = x_tile[32 * i * kChunks + at];
+    for (int i = 0; i < MB; ++i) x[i] = x_tile[2 * i * DEPTH + at];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) w[j] = w_tile[32 * j * kChunks + at];
+    for (int j = 0; j < NB; ++j) w[j] = w_tile[2 * j * DEPTH + at];
   }
   __device__ __forceinline__ void multiply(int16v (&acc)[NB][MB]) const {
 #pragma unroll
@@ -130,10 +132,15 @@ struct Fragments {
   }
 };
 
-// The next chunks are read while these are multiplied, and LOADS loads asked for: one of each between every few products.
-template <int LOADS, int MB, int NB, typename L>
-__device__ __forceinline__ void step(int16v (&acc)[NB][MB], const Fragments<MB, NB> &now, Fragments<MB, NB> &next, const int4v *x_tile, const int4v *w_tile,
-                                     int at, const L &load) {
+struct Nothing {
+  __device__ __forceinline__ void operator()() const {}
+};
+
+// The next chunks are read while these are multiplied, and LOADS loads asked for: one of each between every few products.  (All 16 loads of a tile
+// in a row keep the wave from its products: 8192^3 478 us, this way 443.)
+template <int LOADS, int MB, int NB, int DEPTH, typename L>
+__device__ __forceinline__ void step(int16v (&acc)[NB][MB], const Fragments<MB, NB, DEPTH> &now, Fragments<MB, NB, DEPTH> &next, const int4v *x_tile,
+                                     const int4v *w_tile, int at, const L &load) {
   next.read(x_tile, w_tile, at);
   load();
   now.multiply(acc);
@@ -147,90 +154,120 @@ __device__ __forceinline__ void step(int16v (&acc)[NB][MB], const Fragments<MB, 
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// A tile of 128 bytes of depth, whose first chunks are in `first` already, and the next one's first chunks.  load(0) and load(1) ask for the
-// halves of the one after the next: x's rows into this one's place as soon as all waves have read theirs, the weights' during the next one's first step.
-template <int MB, int NB, typename L0, typename L1>
-__device__ __forceinline__ void turn(int16v (&acc)[NB][MB], Fragments<MB, NB> &first, const int4v *x_now, const int4v *w_now, const int4v *x_next,
-                                     const int4v *w_next, const int (&at)[kDepth / 32], const L0 &load_rest, const L1 &load) {
-  const auto none = [] {};
-  Fragments<MB, NB> other;
-  step<2 * NB>(acc, first, other, x_now, w_now, at[1], load_rest);
-  step<0>(acc, other, first, x_now, w_now, at[2], none);
-  step<0>(acc, first, other, x_now, w_now, at[3], none);
-  tiles_ready();
-  __builtin_amdgcn_sched_barrier(0);
-  step<2 * MB>(acc, other, first, x_next, w_next, at[0], load);
+// The chunks of a tile behind its first two, of which the second are in `other`, to its last (in `other` then), whose products are left.
+template <int MB, int NB, int DEPTH>
+__device__ __forceinline__ void rest_of(int16v (&acc)[NB][MB], Fragments<MB, NB, DEPTH> &first, Fragments<MB, NB, DEPTH> &other, const int4v *x_tile,
+                                        const int4v *w_tile, const int (&at)[DEPTH / 32]) {
+  if constexpr (DEPTH == 128) {
+    step<0>(acc, other, first, x_tile, w_tile, at[2], Nothing());
+    step<0>(acc, first, other, x_tile, w_tile, at[3], Nothing());
+  }
 }
 
-// 64 MB rows of x by 64 NB outputs to a workgroup of four waves, 32 MB by 32 NB to a wave.
-template <typename T, int MB, int NB>
-__global__ __launch_bounds__(256, (MB * NB >= 16 ? 1 : 2)) void int8_linear_kernel(const Int8LinearArgs a, unsigned x_tiles, unsigned w_tiles) {
-  constexpr int XR = 64 * MB, WR = 64 * NB;
-  __shared__ int4v x_tile0[XR * kChunks], w_tile0[WR * kChunks], x_tile1[XR * kChunks], w_tile1[WR * kChunks];
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+// ... and the first two of the next one.  load_x and load_w ask for the tile after that, into this one's place, as soon as all waves have read theirs.
+template <int MB, int NB, int DEPTH, typename L0, typename L1>
+__device__ __forceinline__ void turn(int16v (&acc)[NB][MB], Fragments<MB, NB, DEPTH> &first, Fragments<MB, NB, DEPTH> &other, const int4v *x_now,
+                                     const int4v *w_now, const int4v *x_next, const int4v *w_next, const int (&at)[DEPTH / 32], const L0 &load_x,
+                                     const L1 &load_w) {
+  rest_of(acc, first, other, x_now, w_now, at);
+  tiles_ready();
+  __builtin_amdgcn_sched_barrier(0);
+  step<MB * DEPTH / 64>(acc, other, first, x_next, w_next, at[0], load_x);
+  step<NB * DEPTH / 64>(acc, first, other, x_next, w_next, at[1], load_w);
+}
+
+// 64 MB rows of x by 64 NB outputs to a workgroup, 32 MB by 32 NB to a wave.  Four waves have a tile of LDS after another, from the last on; with KW
+// above one, as many fours take turns at the tiles and add their sums up at the end.
+template <typename T, int MB, int NB, int KW, int DEPTH>
+__global__ __launch_bounds__(256 * KW, (MB * NB >= 16 ? 1 : KW > 1 ? KW : DEPTH == 128 ? 2 : 4)) void int8_linear_kernel(const Int8LinearArgs a, unsigned x_tiles, unsigned w_tiles) {
+  constexpr int XR = 64 * MB, WR = 64 * NB, CH = DEPTH / 16;
+  __shared__ int4v x_tiles0[KW * XR * CH], w_tiles0[KW * WR * CH], x_tiles1[KW * XR * CH], w_tiles1[KW * WR * CH];
+  __shared__ float scales[WR], biases[WR], row_scales[XR];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4), four = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
   unsigned xt, wt;
   place_of(blockIdx.x, x_tiles, w_tiles, xt, wt);
   const int64_t row0 = (int64_t)xt * XR;
   const int out0 = (int)wt * WR;
-  Stager<XR, 256> x;
-  Stager<WR, 256> w;
+  const int x0 = wave % 2 * 32 * MB, w0 = wave / 2 * 32 * NB;
+  int4v *const x_tile0 = x_tiles0 + four * XR * CH, *const w_tile0 = w_tiles0 + four * WR * CH;
+  int4v *const x_tile1 = x_tiles1 + four * XR * CH, *const w_tile1 = w_tiles1 + four * WR * CH;
+  Stager<XR, DEPTH> x;
+  Stager<WR, DEPTH> w;
   x.open(a.x, row0, a.n, a.x_row, a.depth);
   w.open(a.weight, out0, a.outputs, a.weight_row, a.depth);
-  // The last tile goes first: what lies behind a row in its last 16 bytes is not known (zeros on one side are enough), and is out of the way
-  // then.  Tiles behind the last are zeros.
-  const int tiles = (a.depth + kDepth - 1) / kDepth, last = (tiles - 1) * kDepth;
-  x.load(x_tile0, last, a.depth);
-  w.load(w_tile0, last, a.depth);
-  const int x0 = wave % 2 * 32 * MB, w0 = wave / 2 * 32 * NB;
-  int at[kDepth / 32];
+  // Tile i of this four: the last goes first.  (What lies behind a row in its last 16 bytes is not known, and is out of the way then: zeros on
+  // one side are enough.)  Tiles in front of the first are zeros.
+  const int all = (a.depth + DEPTH - 1) / DEPTH, tiles = (all + KW - 1) / KW;
+  const auto k_of = [&](int i) {
+    const int tile = all - 1 - four - i * KW;
+    return tile < 0 ? a.depth : tile * DEPTH;
+  };
+  x.load(x_tile0, k_of(0), a.depth);
+  w.load(w_tile0, k_of(0), a.depth);
+  x.load(x_tile1, k_of(1), a.depth);
+  w.load(w_tile1, k_of(1), a.depth);
+  // scales and bias of the workgroup's outputs, scales of its rows: to LDS when all products are done
+  static_assert(XR == WR && 256 * KW >= WR, "");
+  const int mine = min(out0 + (int)threadIdx.x, a.outputs - 1);
+  const float scale = a.weight_scales[mine], row_scale = a.x_scales[min(row0 + (int)threadIdx.x, a.n - 1)];
+  const T bias = a.bias ? ((const T *)a.bias)[mine] : (T)0.f;
+  int at[DEPTH / 32];
 #pragma unroll
-  for (int s = 0; s < kDepth / 32; ++s) at[s] = chunk_at(lane % 32, 2 * s + lane / 32);
+  for (int s = 0; s < DEPTH / 32; ++s) at[s] = chunk_at<DEPTH>(lane % 32, 2 * s + lane / 32);
   int16v acc[NB][MB] = {};
-  tiles_ready();
+  // the first tile is there, the second may be on its way
+  constexpr int kBehind = x.PER + w.PER;
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (kBehind & 15) | (kBehind & 48) << 10);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();      // (__syncthreads waits for all loads)
+  asm volatile("" ::: "memory");
   if (a.depth % 16) {
-    for (int row = threadIdx.x; row < XR; row += 256) {
-      int8_t *const end = (int8_t *)&x_tile0[chunk_at(row, (a.depth - last) / 16)];
+    for (int row = threadIdx.x; row < XR; row += 256 * KW) {
+      int8_t *const end = (int8_t *)&x_tiles0[chunk_at<DEPTH>(row, a.depth % DEPTH / 16)];
       for (int b = a.depth % 16; b < 16; ++b) end[b] = 0;
     }
     __syncthreads();
   }
   // (no choice in the loop: the accumulators would be moved from registers to registers)
-  const int4v *const x0_now = x_tile0 + x0 * kChunks, *const w0_now = w_tile0 + w0 * kChunks;
-  const int4v *const x1_now = x_tile1 + x0 * kChunks, *const w1_now = w_tile1 + w0 * kChunks;
-  const auto k_of = [&](int tile) { return tile < tiles ? (tile - 1) * kDepth : a.depth; };
-  x.load(x_tile1, k_of(1), a.depth);
-  Fragments<MB, NB> first;
+  const int4v *const x0_now = x_tile0 + x0 * CH, *const w0_now = w_tile0 + w0 * CH, *const x1_now = x_tile1 + x0 * CH, *const w1_now = w_tile1 + w0 * CH;
+  Fragments<MB, NB, DEPTH> first, other;
   first.read(x0_now, w0_now, at[0]);
+  step<0>(acc, first, other, x0_now, w0_now, at[1], Nothing());
   int i = 0;
-  for (; i + 1 < tiles; i += 2) {
-    turn(acc, first, x0_now, w0_now, x1_now, w1_now, at, [&] { w.load(w_tile1, k_of(i + 1), a.depth); }, [&] { x.load(x_tile0, k_of(i + 2), a.depth); });
-    turn(acc, first, x1_now, w1_now, x0_now, w0_now, at, [&] { w.load(w_tile0, k_of(i + 2), a.depth); }, [&] { x.load(x_tile1, k_of(i + 3), a.depth); });
+  for (; i + 2 < tiles; i += 2) {
+    turn(acc, first, other, x0_now, w0_now, x1_now, w1_now, at, [&] { x.load(x_tile0, k_of(i + 2), a.depth); }, [&] { w.load(w_tile0, k_of(i + 2), a.depth); });
+    turn(acc, first, other, x1_now, w1_now, x0_now, w0_now, at, [&] { x.load(x_tile1, k_of(i + 3), a.depth); }, [&] { w.load(w_tile1, k_of(i + 3), a.depth); });
   }
-  if (i < tiles) {
-    const auto none = [] {};
-    Fragments<MB, NB> other;
-    step<0>(acc, first, other, x0_now, w0_now, at[1], none);
-    step<0>(acc, other, first, x0_now, w0_now, at[2], none);
-    step<0>(acc, first, other, x0_now, w0_now, at[3], none);
-    other.multiply(acc);
+  rest_of(acc, first, other, x0_now, w0_now, at);
+  if (i + 1 < tiles) {
+    tiles_ready();
+    step<0>(acc, other, first, x1_now, w1_now, at[0], Nothing());
+    step<0>(acc, first, other, x1_now, w1_now, at[1], Nothing());
+    rest_of(acc, first, other, x1_now, w1_now, at);
   }
-  __builtin_amdgcn_s_waitcnt(0x0f70);      // (the zeros asked for behind the last tile: their place is used again)
-  // scales and bias of the workgroup's outputs by way of LDS
-  __syncthreads();
-  float *const scales = (float *)w_tile0, *const biases = scales + WR;
-  for (int o = threadIdx.x; o < WR; o += 256) {
-    const bool there = out0 + o < a.outputs;
-    scales[o] = there ? a.weight_scales[out0 + o] : 0.f;
-    biases[o] = there && a.bias ? (float)((const T *)a.bias)[out0 + o] : 0.f;
-  }
-  float by[MB];
+  other.multiply(acc);
+  tiles_ready();      // (zeros asked for behind the last tile have landed before their place or the workgroup's LDS is used again)
+  if (threadIdx.x < WR) scales[threadIdx.x] = scale, biases[threadIdx.x] = (float)bias, row_scales[threadIdx.x] = row_scale;
+  if constexpr (KW == 1) __syncthreads();
+  if constexpr (KW > 1) {
+    // (what was asked for behind the last tile has landed before its place is used again)
+    static_assert(MB == 1 && NB == 1 && KW <= 4 && DEPTH == 128, "");
+    // 16 KB a four: two in x's first tiles, the third in the weights'
+    const auto place = [&](int f) { return (f < 3 ? x_tiles0 : w_tiles0) + (f - 1) % 2 * 1024 + threadIdx.x % 256; };
+    if (four > 0)
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int64_t row = row0 + x0 + 32 * i + lane % 32;
-    by[i] = row < a.n ? a.x_scales[row] : 0.f;
+      for (int q = 0; q < 4; ++q) place(four)[q * 256] = int4v{acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
+    __syncthreads();
+    if (four > 0) return;
+#pragma unroll
+    for (int f = 1; f < KW; ++f)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int4v more = place(f)[q * 256];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][0][4 * q + e] += more[e];
+      }
   }
-  __syncthreads();
-  const bool whole = a.outputs % (16 / (int)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int o = w0 + 32 * j;
@@ -246,7 +283,7 @@ __global__ __launch_bounds__(256, (MB * NB >= 16 ? 1 : 2)) void int8_linear_kern
       const int64_t row = row0 + x0 + 32 * i + lane % 32;
       __builtin_amdgcn_sched_barrier(0);      // (block by block: there are no registers for two)
       // (a lane whose row is not there keeps its partner company in the exchange)
-      store_block<T>((T *)a.out + row * a.outputs + out0 + o, acc[j][i], by[i], wb, bb, row < a.n ? there : 0, whole, lane);
+      store_block<T>((T *)a.out + row * a.outputs + out0 + o, acc[j][i], row_scales[x0 + 32 * i + lane % 32], wb, bb, row < a.n ? there : 0, lane);
     }
   }
 }
@@ -260,8 +297,7 @@ __global__ __launch_bounds__(512) void int8_linear_few_kernel(const Int8LinearAr
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int out0 = blockIdx.x * 16;
   // (rows behind the last are read as the last one, and left)
-  const int8_t *const w = a.weight + min(out0 + lane % 16, a.outputs - 1) * a.weight_row + lane / 16 * 16;
-  const int8_t *x[MB];
+  const int8_t *const w = a.weight + min(out0 + lane % 16, a.outputs - 1) * a.weight_row + lane / 16 * 16, *x[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) x[i] = a.x + min((int64_t)(16 * i + lane % 16), a.n - 1) * a.x_row + lane / 16 * 16;
   int4v acc[MB] = {};
@@ -308,14 +344,14 @@ __global__ __launch_bounds__(512) void int8_linear_few_kernel(const Int8LinearAr
   }
 }
 
-template <typename T, int MB, int NB>
+template <typename T, int MB, int NB, int KW, int DEPTH>
 int launch_tiles(const Int8LinearArgs &a) {
   const int64_t x_tiles = (a.n + 64 * MB - 1) / (64 * MB), w_tiles = (a.outputs + 64 * NB - 1) / (64 * NB);
   if (x_tiles * w_tiles > 0x7fffffff) {
     set_error("products in eight bits: more results than one launch takes");
     return FGMS_E_INVALID;
   }
-  int8_linear_kernel<T, MB, NB><<<(unsigned)(x_tiles * w_tiles), 256, 0, a.stream>>>(a, (unsigned)x_tiles, (unsigned)w_tiles);
+  int8_linear_kernel<T, MB, NB, KW, DEPTH><<<(unsigned)(x_tiles * w_tiles), 256 * KW, 0, a.stream>>>(a, (unsigned)x_tiles, (unsigned)w_tiles);
   return FGMS_OK;
 }
 
@@ -325,15 +361,21 @@ int launch_few(const Int8LinearArgs &a) {
   return FGMS_OK;
 }
 
+// Up to 32 rows: sixteen outputs a workgroup where that leaves a CU no more than two (32 rows of 4096 to 4096 outputs 8.0 us, tiles of 64 by four
+// fours 9.9; to 11008 outputs 17 to 19 and 11.5).  Otherwise the widest tiles that fill the chip: 256 in lives of more than eight tiles (24000 rows, 4096
+// outputs, 1024 deep: 128 us with 256 as with 128, 2048 deep 201 and 220, 512 deep 104 and 85), 128, and 64 with two fours along the depth, or four
+// where the tiles are not even one a CU (256 x 4096 x 4096: 12.7 us with two, 11.1 with four, 21.6 with tiles of 128; 512 rows 14.9, 21.3, 22.3).  Up to 128
+// deep a tile has 64 bytes of depth and a CU twice the workgroups, which hide each other's ends (120000 rows of 128 to 384: 25.6 -> 22.9 us; 50000
+// of 256 to 768 the other way, 25.9 -> 29.4), up to 64 outputs in tiles that these fill (200000 rows of 64 to 64: 11.5 -> 10.1).
 template <typename T>
 int launch(const Int8LinearArgs &a) {
-  if (a.n <= 16) return launch_few<T, 1>(a);
-  if (a.n <= 32) return launch_few<T, 2>(a);
-  if (a.n <= 64) return launch_few<T, 4>(a);
   const auto tiles = [&](int64_t side) { return ((a.n + side - 1) / side) * ((a.outputs + side - 1) / side); };
-  if (tiles(256) >= num_cus()) return launch_tiles<T, 4, 4>(a);
-  if (tiles(128) >= num_cus()) return launch_tiles<T, 2, 2>(a);
-  return launch_tiles<T, 1, 1>(a);
+  const int64_t cus = num_cus();
+  if (a.n <= 32 && a.outputs <= 32 * cus) return a.n <= 16 ? launch_few<T, 1>(a) : launch_few<T, 2>(a);
+  if (a.depth <= 128) return a.outputs <= 64 || tiles(128) < cus ? launch_tiles<T, 1, 1, 1, 64>(a) : launch_tiles<T, 2, 2, 1, 64>(a);
+  if (a.depth > 1024 && tiles(256) >= cus) return launch_tiles<T, 4, 4, 1, 128>(a);
+  if (tiles(128) >= cus) return launch_tiles<T, 2, 2, 1, 128>(a);
+  return a.depth >= 2048 && tiles(64) <= cus ? launch_tiles<T, 1, 1, 4, 128>(a) : launch_tiles<T, 1, 1, 2, 128>(a);
 }
 
 }  // namespace

@@ -27,6 +27,7 @@ struct Eight {
   }
 };
 typedef int8_t byte8v __attribute__((ext_vector_type(8)));
+typedef byte8v Byte8Anywhere __attribute__((aligned(1)));
 
 // Sixteen random bits for each of eight neighbouring elements: Philox4x32 with ten rounds (Salmon, Moraes, Dror, Shaw, "Parallel random
 // numbers: as easy as 1, 2, 3", SC 2011), counter (chunk, seed[1]), key seed[0].  Word e of a chunk is half e % 2 of the call's number e / 2.
@@ -51,38 +52,41 @@ __device__ __forceinline__ Words words_of(int64_t chunk, const int64_t *__restri
   return Words{{c0, c1, c2, c3}};
 }
 
-// Eight channels of a row from `c` on, zeros behind the last.  WHOLE: there are eight, and they begin on 16 bytes.
+// Eight channels of a row from `c` on, zeros behind the last.  WHOLE: there are eight, and they begin on 16 bytes; other rows are read and written
+// 16 bytes at a time too, wherever these begin, and by elements where they end.
+template <typename T, bool WHOLE>
+struct Chunk {
+  static constexpr int N = 16 / (int)sizeof(T);
+  typedef T Aligned __attribute__((ext_vector_type(N)));
+  typedef Aligned Vector __attribute__((aligned(WHOLE ? 16 : sizeof(T))));
+};
 template <typename T, bool WHOLE>
 __device__ __forceinline__ Eight load8(const T *__restrict__ row, int c, int channels) {
-  if constexpr (WHOLE) {
-    constexpr int N = 16 / (int)sizeof(T);
-    typedef T Tn __attribute__((ext_vector_type(N)));
-    Eight to;
+  typedef Chunk<T, WHOLE> C;
+  Eight to;
+  if (WHOLE || c + 8 <= channels) {
 #pragma unroll
-    for (int i = 0; i < 8 / N; ++i) {
-      const Tn from = reinterpret_cast<const Tn *>(row + c)[i];
+    for (int i = 0; i < 8 / C::N; ++i) {
+      const typename C::Aligned from = reinterpret_cast<const typename C::Vector *>(row + c)[i];
 #pragma unroll
-      for (int e = 0; e < N; ++e) to[i * N + e] = (float)from[e];
+      for (int e = 0; e < C::N; ++e) to[i * C::N + e] = (float)from[e];
     }
-    return to;
   } else {
-    Eight v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < channels ? (float)row[c + e] : 0.f;
-    return v;
+    for (int e = 0; e < 8; ++e) to[e] = c + e < channels ? (float)row[c + e] : 0.f;
   }
+  return to;
 }
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void store8(T *__restrict__ row, int c, int channels, const Eight &v) {
-  if constexpr (WHOLE) {
-    constexpr int N = 16 / (int)sizeof(T);
-    typedef T Tn __attribute__((ext_vector_type(N)));
+  typedef Chunk<T, WHOLE> C;
+  if (WHOLE || c + 8 <= channels) {
 #pragma unroll
-    for (int i = 0; i < 8 / N; ++i) {
-      Tn to;
+    for (int i = 0; i < 8 / C::N; ++i) {
+      typename C::Aligned to;
 #pragma unroll
-      for (int e = 0; e < N; ++e) to[e] = (T)v[i * N + e];
-      reinterpret_cast<Tn *>(row + c)[i] = to;
+      for (int e = 0; e < C::N; ++e) to[e] = (T)v[i * C::N + e];
+      reinterpret_cast<typename C::Vector *>(row + c)[i] = to;
     }
   } else {
 #pragma unroll
@@ -208,8 +212,8 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
         q[e] = some ? (int8_t)(int)__builtin_rintf(quotient) : (int8_t)0;
       }
       int8_t *const to = a.eighths + row * a.eighths_row + c;
-      if constexpr (WHOLE) {
-        *reinterpret_cast<byte8v *>(to) = q;
+      if (WHOLE || c + 8 <= a.channels) {
+        *reinterpret_cast<Byte8Anywhere *>(to) = q;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -354,13 +358,13 @@ inline int grid_of(int64_t blocks, unsigned *grid) {
   return FGMS_OK;
 }
 
-// Rows that all begin on 16 bytes and are whole chunks of eight channels are read and written 16 bytes at a time, others element by element.
+// Whether all rows begin on 16 bytes and are whole chunks of eight channels.
 bool whole(const void *p, int64_t row, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0; }
 bool whole_rows(const RowsArgs &a) {
   const int size = a.dtype == FGMS_F32 ? 4 : 2;
   bool ok = a.channels % 8 == 0 && whole(a.x, a.x_row, size) && whole(a.sum, a.x_row, size) && (!a.residual || whole(a.residual, a.residual_row, size));
   for (const void *p : {a.scale, (const void *)a.out, a.g_out, a.g_sum, (const void *)a.gx, (const void *)a.g_residual}) ok = ok && whole(p, 0, size);
-  return ok && reinterpret_cast<uintptr_t>(a.eighths) % 8 == 0 && a.eighths_row % 8 == 0;
+  return ok;
 }
 
 }  // namespace
