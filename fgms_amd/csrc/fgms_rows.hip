@@ -60,20 +60,39 @@ struct Chunk {
   typedef T Aligned __attribute__((ext_vector_type(N)));
   typedef Aligned Vector __attribute__((aligned(WHOLE ? 16 : sizeof(T))));
 };
+// ... as they come from memory, in half the registers of their values where these have 16 bits.
+template <typename T>
+struct Raw {
+  int4v part[sizeof(T) / 2];
+  __device__ __forceinline__ Eight values() const {
+    constexpr int N = 16 / (int)sizeof(T);
+    typedef T Tn __attribute__((ext_vector_type(N)));
+    Eight to;
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+      const Tn from = __builtin_bit_cast(Tn, part[i]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) to[i * N + e] = (float)from[e];
+    }
+    return to;
+  }
+};
 template <typename T, bool WHOLE>
-__device__ __forceinline__ Eight load8(const T *__restrict__ row, int c, int channels) {
+__device__ __forceinline__ Raw<T> load_raw(const T *__restrict__ row, int c, int channels, bool there = true) {
   typedef Chunk<T, WHOLE> C;
-  Eight to;
+  Raw<T> to = {};
+  if (!there || c >= channels) return to;
   if (WHOLE || c + 8 <= channels) {
 #pragma unroll
-    for (int i = 0; i < 8 / C::N; ++i) {
-      const typename C::Aligned from = reinterpret_cast<const typename C::Vector *>(row + c)[i];
-#pragma unroll
-      for (int e = 0; e < C::N; ++e) to[i * C::N + e] = (float)from[e];
-    }
+    for (int i = 0; i < 8 / C::N; ++i) to.part[i] = __builtin_bit_cast(int4v, (typename C::Aligned)reinterpret_cast<const typename C::Vector *>(row + c)[i]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) to[e] = c + e < channels ? (float)row[c + e] : 0.f;
+    for (int i = 0; i < 8 / C::N; ++i) {
+      typename C::Aligned v;
+#pragma unroll
+      for (int e = 0; e < C::N; ++e) v[e] = c + i * C::N + e < channels ? row[c + i * C::N + e] : (T)0.f;
+      to.part[i] = __builtin_bit_cast(int4v, v);
+    }
   }
   return to;
 }
@@ -98,17 +117,19 @@ __device__ __forceinline__ void add(Eight &to, const Eight &v) {
   to.each([&](float &t, int e) { t += v[e]; });
 }
 
-// How a row lies on its lanes: lane l of `lanes` (a power of two) has chunks l, l + lanes, ... of eight channels, CHUNKS of them.  A row
-// on a wave or less is summed by exchanges between lanes alone.
+// How a row lies on its lanes: lane l of `lanes` (a power of two) has chunks l, l + lanes, ... of eight channels, `chunks` of them.  Up to 2048
+// channels a row is a wave's or less and is summed by exchanges between lanes alone; the widest take 1024 threads, whose registers
+// hold two chunks.
 struct Share {
   int lanes, chunks, threads;
 };
 inline Share share_of(int channels) {
   const int all = (channels + 7) / 8;
-  if (all > 256) return Share{all > 1024 ? 512 : 256, all > 512 ? 4 : 2, all > 1024 ? 512 : 256};
+  if (all > 1024) return Share{1024, 2, 1024};
+  if (all > 256) return Share{256, all > 512 ? 4 : 2, 256};
   int lanes = 1;
   while (lanes < 64 && lanes < all) lanes *= 2;
-  return Share{lanes, all > 128 ? 4 : all > 64 ? 2 : 1, 256};
+  return Share{lanes, (all + lanes - 1) / lanes, 256};
 }
 
 // Sum over / largest of the lanes of a row.  `part`: a number for each wave, not in use by another exchange.
@@ -137,23 +158,31 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
   const int64_t row = (int64_t)blockIdx.x * (THREADS / lanes) + threadIdx.x / lanes;
   const bool there = row < a.n;
   const int per_row = (a.channels + 7) / 8;
+  // (all that is read, before any of it is waited for)
   const T *const x = (const T *)a.x + row * a.x_row;
-  Eight v[CHUNKS];
+  Raw<T> x_raw[CHUNKS], other[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) x_raw[i] = load_raw<T, WHOLE>(x, 8 * (lane + i * lanes), a.channels, there);
 #pragma unroll
   for (int i = 0; i < CHUNKS; ++i) {
     const int c = 8 * (lane + i * lanes);
-    v[i] = there && c < a.channels ? load8<T, WHOLE>(x, c, a.channels) : Eight{};
+    if constexpr (WHAT == kRowsGatedEighths) other[i] = load_raw<T, WHOLE>(x + a.channels, c, a.channels, there);
+    if constexpr (NORM) other[i] = load_raw<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels, there && a.residual);
   }
+  Eight v[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) v[i] = x_raw[i].values();
   if constexpr (WHAT == kRowsGatedEighths) {
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
-      const int c = 8 * (lane + i * lanes);
-      const Eight b = there && c < a.channels ? load8<T, WHOLE>(x + a.channels, c, a.channels) : Eight{};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] / (1.f + __expf(-v[i][e])) * b[e];
+      const Eight b = other[i].values();
+      v[i].each([&](float &t, int e) { t = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)) * b[e]; });
     }
   }
   if constexpr (NORM) {
+    Raw<T> w[CHUNKS];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) w[i] = load_raw<T, WHOLE>((const T *)a.scale, 8 * (lane + i * lanes), a.channels, a.scale);
     float square = 0.f;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
@@ -161,14 +190,12 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
       if (!there || c >= a.channels) continue;
       if (a.dropped) {
         const Words words = words_of(row * per_row + c / 8, a.seed);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = words.falls(e, a.dropped) ? 0.f : v[i][e] * a.back;
+        v[i].each([&](float &t, int e) { t = words.falls(e, a.dropped) ? 0.f : t * a.back; });
       }
-      if (a.residual) add(v[i], load8<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels));
+      add(v[i], other[i].values());
       v[i].each([](float &t, int) { t = (float)(T)t; });      // (x itself stays what it is)
       if (a.sum) store8<T, WHOLE>((T *)a.sum + row * a.channels, c, a.channels, v[i]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) square = __builtin_fmaf(v[i][e], v[i][e], square);
+      v[i].each([&](float &t, int) { square = __builtin_fmaf(t, t, square); });
     }
     square = over_row(square, lanes, sums, sum_of);
     const float r = 1.f / __builtin_sqrtf(square / (float)a.channels + a.eps);
@@ -178,8 +205,8 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
       if (!there || c >= a.channels) continue;
       v[i].each([&](float &t, int) { t *= r; });
       if (a.scale) {
-        const Eight w = load8<T, WHOLE>((const T *)a.scale, c, a.channels);
-        v[i].each([&](float &t, int e) { t *= w[e]; });
+        const Eight wv = w[i].values();
+        v[i].each([&](float &t, int e) { t *= wv[e]; });
       }
       if constexpr (WHAT == kRowsNorm) store8<T, WHOLE>((T *)a.out + row * a.channels, c, a.channels, v[i]);
     }
@@ -223,38 +250,49 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
   }
 }
 
-// A workgroup goes through the rows in steps of the grid and keeps its lanes' sums of the scale's gradient in registers.
+// A workgroup goes through the rows in steps of the grid and keeps its lanes' sums of the scale's gradient in registers.  The next row is asked for
+// before this one is worked on.
 template <typename T, int CHUNKS, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a, int lanes) {
   __shared__ float parts[2][2][THREADS / 64];
   __shared__ Eight all[THREADS == 256 ? CHUNKS * 256 : 1];
   const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = THREADS / lanes, per_row = (a.channels + 7) / 8;
-  Eight w[CHUNKS], gw[CHUNKS] = {};
+  Raw<T> w[CHUNKS];
+  Eight gw[CHUNKS] = {};
 #pragma unroll
-  for (int i = 0; i < CHUNKS; ++i) {
-    const int c = 8 * (lane + i * lanes);
-    w[i] = a.scale && c < a.channels ? load8<T, WHOLE>((const T *)a.scale, c, a.channels) : Eight{{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f}};
-  }
-  int turn = 0;      // (a row's exchanges and the next one's do not share their places)
-  for (int64_t first = (int64_t)blockIdx.x * groups; first < a.n; first += (int64_t)gridDim.x * groups, turn ^= 1) {
-    const int64_t row = first + group;
-    const bool there = row < a.n;
-    Eight h[CHUNKS], g[CHUNKS];
-    float square = 0.f, along = 0.f;
+  for (int i = 0; i < CHUNKS; ++i) w[i] = load_raw<T, WHOLE>((const T *)a.scale, 8 * (lane + i * lanes), a.channels, a.scale);
+  Raw<T> next_h[CHUNKS], next_g[CHUNKS], next_gs[CHUNKS];
+  const auto ask = [&](int64_t row) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const int c = 8 * (lane + i * lanes);
-      const bool here = there && c < a.channels;
-      h[i] = here ? load8<T, WHOLE>((const T *)a.sum + row * a.x_row, c, a.channels) : Eight{};
-      g[i] = here ? load8<T, WHOLE>((const T *)a.g_out + row * a.channels, c, a.channels) : Eight{};
+      next_h[i] = load_raw<T, WHOLE>((const T *)a.sum + row * a.x_row, c, a.channels, row < a.n);
+      next_g[i] = load_raw<T, WHOLE>((const T *)a.g_out + row * a.channels, c, a.channels, row < a.n);
+      next_gs[i] = load_raw<T, WHOLE>((const T *)a.g_sum + row * a.channels, c, a.channels, row < a.n && a.g_sum);
     }
+  };
+  int64_t row = (int64_t)blockIdx.x * groups + group;
+  const int64_t stride = (int64_t)gridDim.x * groups;
+  constexpr bool kAhead = THREADS == 256;      // (1024 threads have no registers for it)
+  if (kAhead) ask(row);
+  int turn = 0;      // (a row's exchanges and the next one's do not share their places)
+  for (int64_t first = (int64_t)blockIdx.x * groups; first < a.n; first += stride, row += stride, turn ^= 1) {
+    if (!kAhead) ask(row);
+    Raw<T> h[CHUNKS], g[CHUNKS], gs_raw[CHUNKS];
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i)
+    for (int i = 0; i < CHUNKS; ++i) h[i] = next_h[i], g[i] = next_g[i], gs_raw[i] = next_gs[i];
+    if (kAhead) ask(row + stride);
+    const bool there = row < a.n;
+    float square = 0.f, along = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        square = __builtin_fmaf(h[i][e], h[i][e], square);
-        along = __builtin_fmaf(w[i][e] * g[i][e], h[i][e], along);
-      }
+    for (int i = 0; i < CHUNKS; ++i) {
+      const Eight hv = h[i].values(), gv = g[i].values();
+      Eight wv = w[i].values();
+      wv.each([&](float &t, int e) {
+        square = __builtin_fmaf(hv[e], hv[e], square);
+        along = __builtin_fmaf((a.scale ? t : 1.f) * gv[e], hv[e], along);
+      });
+    }
     square = over_row(square, lanes, parts[turn][0], sum_of);
     along = over_row(along, lanes, parts[turn][1], sum_of);
     const float r = 1.f / __builtin_sqrtf(square / (float)a.channels + a.eps), back = r * r * (along / (float)a.channels);
@@ -262,19 +300,15 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a
     for (int i = 0; i < CHUNKS; ++i) {
       const int c = 8 * (lane + i * lanes);
       if (!there || c >= a.channels) continue;
+      const Eight hv = h[i].values(), gv = g[i].values(), wv = w[i].values(), more = gs_raw[i].values();
+      gw[i].each([&](float &t, int e) { t = __builtin_fmaf(gv[e] * r, hv[e], t); });
       Eight gs;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        gw[i][e] = __builtin_fmaf(g[i][e] * r, h[i][e], gw[i][e]);
-        gs[e] = r * (w[i][e] * g[i][e] - h[i][e] * back);
-      }
-      if (a.g_sum) add(gs, load8<T, WHOLE>((const T *)a.g_sum + row * a.channels, c, a.channels));
+      gs.each([&](float &t, int e) { t = __builtin_fmaf(r, (a.scale ? wv[e] : 1.f) * gv[e] - hv[e] * back, more[e]); });
       if (a.g_residual) store8<T, WHOLE>((T *)a.g_residual + row * a.channels, c, a.channels, gs);
       if (a.gx) {
         if (a.dropped) {
           const Words words = words_of(row * per_row + c / 8, a.seed);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) gs[e] = words.falls(e, a.dropped) ? 0.f : gs[e] * a.back;
+          gs.each([&](float &t, int e) { t = words.falls(e, a.dropped) ? 0.f : t * a.back; });
         }
         store8<T, WHOLE>((T *)a.gx + row * a.channels, c, a.channels, gs);
       }
@@ -324,13 +358,13 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const RowsArgs a, int6
   if (at >= chunks) return;
   const int64_t row = at / per_row;
   const int c = 8 * (int)(at - row * per_row);
-  Eight v = load8<T, WHOLE>((const T *)a.x + row * a.x_row, c, a.channels);
-  if (a.dropped) {
-    const Words words = words_of(at, a.seed);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = words.falls(e, a.dropped) ? 0.f : v[e] * a.back;
-  }
-  if (a.residual) add(v, load8<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels));
+  const Raw<T> x = load_raw<T, WHOLE>((const T *)a.x + row * a.x_row, c, a.channels);
+  const Raw<T> residual = load_raw<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels, a.residual);
+  Words words = {};
+  if (a.dropped) words = words_of(at, a.seed);      // (while the rows are on their way)
+  Eight v = x.values();
+  if (a.dropped) v.each([&](float &t, int e) { t = words.falls(e, a.dropped) ? 0.f : t * a.back; });
+  if (a.residual) add(v, residual.values());
   store8<T, WHOLE>((T *)a.out + row * a.channels, c, a.channels, v);
 }
 
@@ -341,8 +375,8 @@ template <int CHUNKS, int THREADS> struct Shape {
 };
 template <typename F>
 int by_share(const Share &s, F f) {
-  if (s.threads == 512) return f(Shape<4, 512>());
-  return s.chunks == 1 ? f(Shape<1, 256>()) : s.chunks == 2 ? f(Shape<2, 256>()) : f(Shape<4, 256>());
+  if (s.threads == 1024) return f(Shape<2, 1024>());
+  return s.chunks == 1 ? f(Shape<1, 256>()) : s.chunks == 2 ? f(Shape<2, 256>()) : s.chunks == 3 ? f(Shape<3, 256>()) : f(Shape<4, 256>());
 }
 template <typename F>
 int by_type(int dtype, F f) {
