@@ -277,6 +277,8 @@ class Int8Linear(torch.nn.Module):
 
     def __init__(self, linear):
         super().__init__()
+        if not isinstance(linear, torch.nn.Linear):
+            raise ValueError("Int8Linear is made of a torch.nn.Linear")
         self.in_features, self.out_features, self.dtype = linear.in_features, linear.out_features, linear.weight.dtype
         with torch.no_grad():
             q, scales = quantize_rows(linear.weight)

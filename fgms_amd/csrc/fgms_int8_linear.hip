@@ -250,7 +250,6 @@ __global__ __launch_bounds__(256 * KW, (MB * NB >= 16 ? 1 : KW > 1 ? KW : DEPTH 
   if (threadIdx.x < WR) scales[threadIdx.x] = scale, biases[threadIdx.x] = (float)bias, row_scales[threadIdx.x] = row_scale;
   if constexpr (KW == 1) __syncthreads();
   if constexpr (KW > 1) {
-    // (what was asked for behind the last tile has landed before its place is used again)
     static_assert(MB == 1 && NB == 1 && KW <= 4 && DEPTH == 128, "");
     // 16 KB a four: two in x's first tiles, the third in the weights'
     const auto place = [&](int f) { return (f < 3 ? x_tiles0 : w_tiles0) + (f - 1) % 2 * 1024 + threadIdx.x % 256; };

@@ -192,6 +192,50 @@ def test_values_that_are_no_numbers():
         assert (y == 0).all() and torch.autograd.grad(y, zero, torch.ones_like(y))[0].isfinite().all()
 
 
+def test_far_rows():
+    """Rows behind 2^32 bytes and 2^31 elements, and their words."""
+    from FGMS import nn
+    n, c = 140000, 16384
+    seed = torch.tensor([11, 12], device="cuda")
+    x = torch.zeros(n, c, dtype=torch.float16, device="cuda")
+    x[-1] = 1
+    y, h = nn.add_norm(x, None, None, p=0.5, seed=seed)
+    per = c // 8
+    words = B.philox([torch.arange((n - 1) * per, n * per), torch.zeros(per, dtype=torch.int64), torch.full((per,), 12), torch.zeros(per, dtype=torch.int64)], [11, 0])
+    words = torch.stack([w >> shift & 0xFFFF for w in words for shift in (0, 16)], 1).reshape(1, c)
+    want = 2.0 * (words >= 32768)
+    assert torch.equal(h[-1:].cpu().double(), want.double()) and not h[:-1].any() and not y[:-1].any()
+    B.within(y[-1:], *B.normed(h[-1:], None, 1e-6), "norm")
+    assert torch.equal(nn.dropout_add(x, None, 0.5, seed)[-1], h[-1])
+    del y, h
+    q, scales, _ = nn.add_norm_int8(x)
+    assert (q[-1] == 127).all() and not q[-2].any() and not scales[:-1].any()
+    g = torch.ones(n, c, dtype=torch.float16, device="cuda")
+    x[-1, ::2] = 3
+    leaf = x.requires_grad_()
+    got = torch.autograd.grad(nn.add_norm(leaf, None, None)[0], leaf, g)[0]
+    row = x[-1:].detach()
+    gs, off, *_ = B.norm_grads(row, None, 1e-6, g[-1:], None, torch.ones(1, c, dtype=torch.float64))
+    B.within(got[-1:], gs, off, "gradient")
+
+
+def test_captured_seeds():
+    """Seeds that a captured call draws are new ones at every replay."""
+    from FGMS import nn
+    x = torch.ones(100, 64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    nn.dropout_add(x, None, 0.5)
+    with torch.cuda.graph(graph):
+        y = nn.dropout_add(x, None, 0.5)
+    seen = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        seen.append(y.clone())
+        assert ((y == 0) | (y == 2)).all() and abs(float(y.mean()) - 1) < 0.2
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
 def test_no_rows():
     from FGMS import nn
     x = torch.zeros(0, 24, device="cuda", requires_grad=True)

@@ -107,6 +107,48 @@ def test_products(shape, dtype):
             assert torch.equal(nn.int8_linear(u, sx, v, sw, bias, B.DTYPES[dtype]), y)
 
 
+@pytest.mark.parametrize("dtype", list(B.DTYPES))
+@pytest.mark.parametrize("shape", [(4200, 4100, 1111), (4097, 4352, 2048), (9000, 1025, 130), (20000, 200, 72), (8300, 64, 40)], ids=str)
+def test_wide_products(shape, dtype):
+    """The widest tiles, and rows behind their last; sums of whole numbers in 64 bits on the card, where they are exact too."""
+    from FGMS import nn
+    n, outputs, c = shape
+    gen = torch.Generator().manual_seed(n)
+    x, sx = eighths(n, c, gen, 55)
+    w, sw = eighths(outputs, c, gen, 66)
+    bias = torch.randn(outputs, generator=gen).to(B.DTYPES[dtype]).cuda()
+    y = nn.int8_linear(x, sx, w, sw / c, bias, B.DTYPES[dtype]).double()
+    want = x.double() @ w.double().t().contiguous() * sx.double()[:, None] * (sw / c).double()
+    off = 4 * B.SUM * want.abs()
+    want += bias.double()
+    off += (B.SUM + B.UNIT[B.DTYPES[dtype]]) * want.abs() + B.TINY[B.DTYPES[dtype]]
+    assert ((y - want).abs() <= off).all()
+
+
+def test_far_rows():
+    """Rows behind 2^32 bytes of x, and results behind 2^32 elements."""
+    from FGMS import nn
+    gen = torch.Generator().manual_seed(2)
+    w, sw = eighths(24, 16000, gen, 1)
+    x = torch.zeros(270000, 16000, dtype=torch.int8, device="cuda")
+    at = torch.tensor([0, 1, 134217, 134218, 268435, 268436, 269998, 269999], device="cuda")
+    few, _ = eighths(8, 16000, gen, 0)
+    x[at] = few
+    scales = torch.ones(270000, device="cuda") / 16000
+    y = nn.int8_linear(x, scales, w, sw, None, torch.float32)
+    B.within(y[at], *B.product(few, scales[:8], w, sw, None, torch.float32), "far rows")
+    y[at] = 0
+    assert not y.any()
+    del x, y
+    w, sw = eighths(8000, 24, gen, 1)
+    x = torch.zeros(600000, 32, dtype=torch.int8, device="cuda")[:, :24]
+    few, _ = eighths(3, 24, gen, 0)
+    x[[7, 536870, 599999]] = few
+    y = nn.int8_linear(x, torch.ones(600000, device="cuda"), w, sw, None, torch.float16)
+    B.within(y[[7, 536870, 599999]], *B.product(few, torch.ones(3), w, sw, None, torch.float16), "far results")
+    assert not y[536871:599999].any()
+
+
 def test_largest_sums():
     """Sums at the ends of 32 bits."""
     from FGMS import nn
