@@ -291,6 +291,10 @@ class Int8Linear(torch.nn.Module):
         super()._apply(fn, recurse)
         # (scales stay fp32 whatever the layer is cast to; its results are of the type)
         self.weight_scales = scales.to(self.weight.device)
+        if self.weight.stride(0) % 16:      # (a copy's rows lie next to each other: on 16 bytes again, or every call would copy them)
+            held = self.weight.new_zeros(self.out_features, (self.in_features + 15) // 16 * 16)
+            held[:, :self.in_features] = self.weight
+            self.weight = held[:, :self.in_features]
         self.dtype = fn(torch.empty(0, dtype=self.dtype, device=scales.device)).dtype
         return self
 

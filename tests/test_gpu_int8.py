@@ -49,6 +49,20 @@ def test_halves_go_to_even_numbers():
     assert q.tolist() == [[127, 0, 2, 2, 0, -2, -2, 64, -126, 0, -127, 3, 0, -1, 100, 100]]
 
 
+def test_quotients_are_those_of_a_division():
+    """Of 16-bit values, half of a row's largest and its odd multiples of 1/254 among them, and of 32-bit ones."""
+    from FGMS import nn
+    for t in B.DTYPES.values():
+        gen = torch.Generator().manual_seed(4)
+        x = torch.randn(2000, 2072, generator=gen).to(t)
+        x[:, :64] = (x.abs().amax(1, keepdim=True).double() * (2 * torch.arange(64) + 1) / 254).to(t)
+        x = x.cuda()
+        q, scales = nn.quantize_rows(x)
+        want = x.cpu().float().abs().amax(1) / 127      # (on the CPU, whose divisions are rounded as they should be)
+        assert torch.equal(scales.cpu(), want)
+        assert torch.equal(q.cpu(), torch.round(x.cpu().float() / want[:, None]).to(torch.int8))
+
+
 @pytest.mark.parametrize("channels", [24, 72, 1096, 4100])
 def test_rows_without_values(channels):
     """Zeros, numbers too small for a scale, infinities and NaN."""

@@ -108,6 +108,29 @@ def test_row_by_row(eight):
                 assert float(off.max()) < 4096 * 2.0 ** -24, i
 
 
+def test_moved_layers_keep_their_rows_on_sixteen_bytes():
+    from FGMS import nn
+    torch.manual_seed(6)
+    linear = torch.nn.Linear(40, 7, device="cuda")
+    layer = nn.Int8Linear(linear)
+    x = torch.randn(9, 40, device="cuda")
+    with torch.no_grad():
+        want = layer(x)
+        assert layer.weight.shape == (7, 40) and layer.weight.stride(0) == 48
+        back = layer.cpu().cuda()
+        assert back.weight.stride(0) == 48 and torch.equal(back(x), want)
+        fresh = nn.Int8Linear(torch.nn.Linear(40, 7, device="cuda"))
+        fresh.load_state_dict(layer.state_dict())
+        assert torch.equal(fresh(x), want) and layer.half()(x.half()).dtype == torch.float16
+        with pytest.raises(ValueError, match="Linear"):
+            nn.Int8Linear(layer)
+        # 8 bits of x and of the weights, each off by up to half a step of 1/127 of a row's largest
+        exact = x.double() @ linear.weight.double().t() + linear.bias.double()
+        off = (x.abs().amax(1, keepdim=True) / 254 * 1.01).double() * linear.weight.double().abs().sum(1) \
+            + x.double().abs().sum(1, keepdim=True) * (linear.weight.abs().amax(1) / 254 * 1.02).double() + 1e-5
+        assert ((want.double() - exact).abs() <= off).all()
+
+
 def test_block_without_gradients_over_caches():
     from FGMS import nn
     block = nn.VoxelBlock(64, 4, device="cuda")
