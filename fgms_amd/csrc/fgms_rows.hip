@@ -176,6 +176,7 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const Eight b = other[i].values();
+      // (the exponential and the reciprocal as the unit gives them: of 2 M values two fall to the other side of a border, as many as with divisions)
       v[i].each([&](float &t, int e) { t = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)) * b[e]; });
     }
   }
