@@ -481,6 +481,11 @@ def _row(t):
     return t.stride(0) if t is not None and t.shape[0] > 1 else 0
 
 
+def _row_of_result(t, least):
+    """(rows that lie on top of each other are refused by the call)"""
+    return t.stride(0) if t.shape[0] > 1 else least
+
+
 def _seed(seed):
     _need_shaped(seed, "seed", torch.int64, (2,))
     return _p(seed)
@@ -504,7 +509,7 @@ def add_norm_bwd(out_grad, sum_grad, sum, scale, x_grad, residual_grad, scale_gr
                        (x_grad, "x_grad", sum.shape), (residual_grad, "residual_grad", sum.shape), (scale_grad, "scale_grad", sum.shape[1:])):
         _need_shaped(t, n, sum.dtype, like)
     n, channels = sum.shape
-    room = torch.empty(lib().fgms_add_norm_bwd_sums(n, channels), device=sum.device) if scale_grad is not None else None
+    room = torch.empty(lib().fgms_add_norm_bwd_sums(n, channels), dtype=torch.float32, device=sum.device) if scale_grad is not None else None
     _check(lib().fgms_add_norm_bwd(_p(out_grad), _p(sum_grad), _p(sum), _p(scale), _p(x_grad), _p(residual_grad), _p(scale_grad), _p(room), n, channels,
                                    _row(sum), float(eps), float(p), _seed(seed), _attention_dtype(sum), _stream()))
 
@@ -532,7 +537,7 @@ def quantize_rows(x, out, scales, gated=False):
         raise ValueError("gated rows hold two halves")
     _need_eighths(out, "out", n, channels)
     _need_shaped(scales, "scales", torch.float32, (n,))
-    _check(lib().fgms_quantize_rows(_p(x), _p(out), _p(scales), n, channels, _row(x), max(_row(out), channels), int(gated), _attention_dtype(x), _stream()))
+    _check(lib().fgms_quantize_rows(_p(x), _p(out), _p(scales), n, channels, _row(x), _row_of_result(out, channels), int(gated), _attention_dtype(x), _stream()))
 
 
 def add_norm_int8(x, residual, scale, sum, out, scales, eps=1e-6):
@@ -546,7 +551,7 @@ def add_norm_int8(x, residual, scale, sum, out, scales, eps=1e-6):
     _need_eighths(out, "out", n, channels)
     _need_shaped(scales, "scales", torch.float32, (n,))
     _check(lib().fgms_add_norm_int8(_p(x), _p(residual), _p(scale), _p(sum), _p(out), _p(scales), n, channels, _row(x), _row(residual),
-                                    max(_row(out), channels), float(eps), _attention_dtype(x), _stream()))
+                                    _row_of_result(out, channels), float(eps), _attention_dtype(x), _stream()))
 
 
 def int8_linear(x, x_scales, weight, weight_scales, bias, out):
@@ -563,5 +568,5 @@ def int8_linear(x, x_scales, weight, weight_scales, bias, out):
     _need_shaped(weight_scales, "weight_scales", torch.float32, (outputs,))
     _need_shaped(bias, "bias", out.dtype, (outputs,))
     _need_shaped(out, "out", out.dtype, (n, outputs))
-    _check(lib().fgms_int8_linear(_p(x), _p(x_scales), _p(weight), _p(weight_scales), _p(bias), _p(out), n, outputs, channels, _row(x) or least,
-                                  _row(weight) or least, _attention_dtype(out, "FGMS rows: out"), _stream()))
+    _check(lib().fgms_int8_linear(_p(x), _p(x_scales), _p(weight), _p(weight_scales), _p(bias), _p(out), n, outputs, channels, _row_of_result(x, least),
+                                  _row_of_result(weight, least), _attention_dtype(out, "FGMS rows: out"), _stream()))
