@@ -149,6 +149,8 @@ __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 // (of the bits of numbers without their sign, which are in the numbers' order, infinity and then NaN behind the others)
 __device__ __forceinline__ unsigned larger_of(unsigned a, unsigned b) { return a > b ? a : b; }
 
+// A row to each group of lanes, once: what a launch of any kind (WHAT) reads and writes is all that memory moves.  (50000 rows of 256, fp32: 205 MB in
+// 41 us, 5.0 TB/s; 120000 of 128, fp16, with dropout: 123 MB in 25 us; 200000 of 64 to eight bits: 90 MB in 18 to 19 us; 16 gated rows of 11008: 5 us.)
 template <typename T, int CHUNKS, int THREADS, bool WHOLE, int WHAT>
 __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lanes) {
   constexpr bool NORM = WHAT == kRowsNorm || WHAT == kRowsNormEighths;
@@ -255,7 +257,8 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
 }
 
 // A workgroup goes through the rows in steps of the grid and keeps its lanes' sums of the scale's gradient in registers.  The next row is asked for
-// before this one is worked on.
+// before this one is worked on: the registers of three chunks leave two waves a SIMD, whose loads alone would not keep memory busy.  (120000 rows of 128,
+// fp16, with dropout: 154 MB in 32 us; 10007 of 1096, bf16: 88 MB in 21 us.)
 template <typename T, int CHUNKS, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a, int lanes) {
   __shared__ float parts[2][2][THREADS / 64];
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a
   }
 }
 
-// out[channel] = the workgroups' sums, eight channels a workgroup, 32 threads each, in a fixed order.
+// out[channel] = the workgroups' sums, eight channels a workgroup, 32 threads each, in a fixed order.  (1250 sums of 128, or 501 of 1096: 4 us.)
 template <typename T>
 __global__ __launch_bounds__(256) void column_sums_kernel(const float *__restrict__ sums, int64_t groups, int channels, T *__restrict__ out) {
   __shared__ float part[4][8];
@@ -354,7 +357,8 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float *__restric
   if (threadIdx.x < 8 && column < channels) out[column] = (T)(part[0][c] + part[1][c] + part[2][c] + part[3][c]);
 }
 
-// Eight elements a thread, counted through the rows.
+// Eight elements a thread, counted through the rows; their words while they are on their way.  (200000 rows of 64, fp32: 154 MB in 27 us; 16384 of 4096,
+// bf16: 403 MB in 74 us.)
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const RowsArgs a, int64_t chunks) {
   const int per_row = (a.channels + 7) / 8;
@@ -365,7 +369,7 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const RowsArgs a, int6
   const Raw<T> x = load_raw<T, WHOLE>((const T *)a.x + row * a.x_row, c, a.channels);
   const Raw<T> residual = load_raw<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels, a.residual);
   Words words = {};
-  if (a.dropped) words = words_of(at, a.seed);      // (while the rows are on their way)
+  if (a.dropped) words = words_of(at, a.seed);
   Eight v = x.values();
   if (a.dropped) v.each([&](float &t, int e) { t = words.falls(e, a.dropped) ? 0.f : t * a.back; });
   if (a.residual) add(v, residual.values());
