@@ -349,7 +349,7 @@ __global__ __launch_bounds__(512) void int8_linear_few_kernel(const Int8LinearAr
 template <typename T, int MB, int NB, int KW, int DEPTH>
 int launch_tiles(const Int8LinearArgs &a) {
   const int64_t x_tiles = (a.n + 64 * MB - 1) / (64 * MB), w_tiles = (a.outputs + 64 * NB - 1) / (64 * NB);
-  if (x_tiles * w_tiles > 0x7fffffff) {
+  if (x_tiles * w_tiles > 0xffffffffll / (256 * KW)) {
     set_error("products in eight bits: more results than one launch takes");
     return FGMS_E_INVALID;
   }

@@ -20,6 +20,7 @@ struct RowsArgs {
   unsigned dropped;
   float back;
   const int64_t *seed;                   // [2]: key, upper half of the counter
+  int64_t first;                         // which row of the caller's the first is (a launch may have a part of them)
   void *sum, *out;                       // [n, channels]; sum may be nullptr
   int8_t *eighths;                       // rows of `eighths_row`
   int64_t eighths_row;

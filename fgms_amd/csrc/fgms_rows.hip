@@ -192,7 +192,7 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
       const int c = 8 * (lane + i * lanes);
       if (!there || c >= a.channels) continue;
       if (a.dropped) {
-        const Words words = words_of(row * per_row + c / 8, a.seed);
+        const Words words = words_of((a.first + row) * per_row + c / 8, a.seed);
         v[i].each([&](float &t, int e) { t = words.falls(e, a.dropped) ? 0.f : t * a.back; });
       }
       add(v[i], other[i].values());
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const RowsArgs a, int6
   const Raw<T> x = load_raw<T, WHOLE>((const T *)a.x + row * a.x_row, c, a.channels);
   const Raw<T> residual = load_raw<T, WHOLE>((const T *)a.residual + row * a.residual_row, c, a.channels, a.residual);
   Words words = {};
-  if (a.dropped) words = words_of(at, a.seed);
+  if (a.dropped) words = words_of(a.first * per_row + at, a.seed);
   Eight v = x.values();
   if (a.dropped) v.each([&](float &t, int e) { t = words.falls(e, a.dropped) ? 0.f : t * a.back; });
   if (a.residual) add(v, residual.values());
@@ -382,22 +382,30 @@ template <int CHUNKS, int THREADS> struct Shape {
   static constexpr int chunks = CHUNKS, threads = THREADS;
 };
 template <typename F>
-int by_share(const Share &s, F f) {
+void by_share(const Share &s, F f) {
   if (s.threads == 1024) return f(Shape<2, 1024>());
   return s.chunks == 1 ? f(Shape<1, 256>()) : s.chunks == 2 ? f(Shape<2, 256>()) : s.chunks == 3 ? f(Shape<3, 256>()) : f(Shape<4, 256>());
 }
 template <typename F>
-int by_type(int dtype, F f) {
+void by_type(int dtype, F f) {
   return dtype == FGMS_F32 ? f(float()) : dtype == FGMS_F16 ? f((_Float16)0) : f((__bf16)0);
 }
 
-inline int grid_of(int64_t blocks, unsigned *grid) {
-  if (blocks > 0x7fffffff) {
-    set_error("%lld workgroups are more than one launch takes", (long long)blocks);
-    return FGMS_E_INVALID;
+// Launches over all rows, `rows` at most in one (a grid has fewer than 2^32 threads): f(the rows of one).
+constexpr int64_t kMostThreads = (int64_t)1 << 31;
+template <typename F>
+void by_parts(const RowsArgs &a, int64_t rows, F f) {
+  const int64_t size = a.dtype == FGMS_F32 ? 4 : 2;
+  for (int64_t first = 0; first < a.n; first += rows) {
+    const auto moved = [&](const void *p, int64_t row) { return p ? (const char *)p + first * row * size : nullptr; };
+    RowsArgs part = a;
+    part.first = first, part.n = a.n - first < rows ? a.n - first : rows;
+    part.x = moved(a.x, a.x_row), part.residual = moved(a.residual, a.residual_row);
+    part.sum = (void *)moved(a.sum, a.channels), part.out = (void *)moved(a.out, a.channels);
+    if (a.eighths) part.eighths = a.eighths + first * a.eighths_row;
+    if (a.scales) part.scales = a.scales + first;
+    f(part);
   }
-  *grid = (unsigned)blocks;
-  return FGMS_OK;
 }
 
 // Whether all rows begin on 16 bytes and are whole chunks of eight channels.
@@ -414,24 +422,23 @@ bool whole_rows(const RowsArgs &a) {
 int launch_rows(const RowsArgs &a, int what) {
   const Share s = share_of(a.channels);
   const int at_once = s.threads / s.lanes;
-  unsigned grid;
-  const int rc = grid_of((a.n + at_once - 1) / at_once, &grid);
-  if (rc != FGMS_OK) return rc;
   const bool w = whole_rows(a);
-  by_type(a.dtype, [&](auto t) {
-    using T = decltype(t);
-    return by_share(s, [&](auto shape) {
-      constexpr int K = decltype(shape)::chunks, N = decltype(shape)::threads;
-      const auto launch = [&](auto kind) {
-        constexpr int WHAT = decltype(kind)::value;
-        if (w) rows_kernel<T, K, N, true, WHAT><<<grid, N, 0, a.stream>>>(a, s.lanes);
-        else rows_kernel<T, K, N, false, WHAT><<<grid, N, 0, a.stream>>>(a, s.lanes);
-      };
-      if (what == kRowsNorm) launch(Number<kRowsNorm>());
-      else if (what == kRowsNormEighths) launch(Number<kRowsNormEighths>());
-      else if (what == kRowsEighths) launch(Number<kRowsEighths>());
-      else launch(Number<kRowsGatedEighths>());
-      return FGMS_OK;
+  by_parts(a, kMostThreads / s.lanes, [&](const RowsArgs &part) {
+    const unsigned grid = (unsigned)((part.n + at_once - 1) / at_once);
+    by_type(a.dtype, [&](auto t) {
+      using T = decltype(t);
+      by_share(s, [&](auto shape) {
+        constexpr int K = decltype(shape)::chunks, N = decltype(shape)::threads;
+        const auto launch = [&](auto kind) {
+          constexpr int WHAT = decltype(kind)::value;
+          if (w) rows_kernel<T, K, N, true, WHAT><<<grid, N, 0, a.stream>>>(part, s.lanes);
+          else rows_kernel<T, K, N, false, WHAT><<<grid, N, 0, a.stream>>>(part, s.lanes);
+        };
+        if (what == kRowsNorm) launch(Number<kRowsNorm>());
+        else if (what == kRowsNormEighths) launch(Number<kRowsNormEighths>());
+        else if (what == kRowsEighths) launch(Number<kRowsEighths>());
+        else launch(Number<kRowsGatedEighths>());
+      });
     });
   });
   FGMS_HIP_TRY(hipGetLastError());
@@ -454,12 +461,11 @@ int launch_add_norm_bwd(const RowsArgs &a) {
   const bool w = whole_rows(a);
   by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return by_share(s, [&](auto shape) {
+    by_share(s, [&](auto shape) {
       constexpr int K = decltype(shape)::chunks, N = decltype(shape)::threads;
       if (w) add_norm_grad_kernel<T, K, N, true><<<grid, N, 0, a.stream>>>(a, s.lanes);
       else add_norm_grad_kernel<T, K, N, false><<<grid, N, 0, a.stream>>>(a, s.lanes);
       if (a.g_scale) column_sums_kernel<T><<<(a.channels + 7) / 8, 256, 0, a.stream>>>(a.scale_sums, grid, a.channels, (T *)a.g_scale);
-      return FGMS_OK;
     });
   });
   FGMS_HIP_TRY(hipGetLastError());
@@ -467,16 +473,16 @@ int launch_add_norm_bwd(const RowsArgs &a) {
 }
 
 int launch_dropout_add(const RowsArgs &a) {
-  const int64_t chunks = a.n * ((a.channels + 7) / 8);
-  unsigned grid;
-  const int rc = grid_of((chunks + 255) / 256, &grid);
-  if (rc != FGMS_OK) return rc;
+  const int per_row = (a.channels + 7) / 8;
   const bool w = whole_rows(a);
-  by_type(a.dtype, [&](auto t) {
-    using T = decltype(t);
-    if (w) dropout_add_kernel<T, true><<<grid, 256, 0, a.stream>>>(a, chunks);
-    else dropout_add_kernel<T, false><<<grid, 256, 0, a.stream>>>(a, chunks);
-    return FGMS_OK;
+  by_parts(a, kMostThreads / per_row, [&](const RowsArgs &part) {
+    const int64_t chunks = part.n * per_row;
+    const unsigned grid = (unsigned)((chunks + 255) / 256);
+    by_type(a.dtype, [&](auto t) {
+      using T = decltype(t);
+      if (w) dropout_add_kernel<T, true><<<grid, 256, 0, a.stream>>>(part, chunks);
+      else dropout_add_kernel<T, false><<<grid, 256, 0, a.stream>>>(part, chunks);
+    });
   });
   FGMS_HIP_TRY(hipGetLastError());
   return FGMS_OK;

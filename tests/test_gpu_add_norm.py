@@ -219,6 +219,40 @@ def test_far_rows():
     B.within(got[-1:], gs, off, "gradient")
 
 
+def test_more_rows_than_a_launch_takes():
+    """Both sides of the row that the second launch begins with."""
+    from FGMS import nn
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GB")
+    n, c = (1 << 25) + 5, 512
+    at = torch.tensor([0, (1 << 25) - 1, 1 << 25, n - 1])
+    gen = torch.Generator().manual_seed(1)
+    rows = features(4, c, "fp16", gen)
+    x = torch.zeros(n, c, dtype=torch.float16, device="cuda")
+    x[at] = rows
+    per = c // 8
+    chunk = (at[:, None] * per + torch.arange(per)).flatten()
+    words = B.philox([chunk & B.MASK, chunk >> 32, torch.full_like(chunk, 12), torch.zeros_like(chunk)], [11, 0])
+    words = torch.stack([w >> shift & 0xFFFF for w in words for shift in (0, 16)], 1).reshape(4, c)
+    factor = 2.0 * (words >= 32768).double()
+    seed = torch.tensor([11, 12], device="cuda")
+    y, h = nn.add_norm(x, None, None, p=0.5, seed=seed)
+    B.within(h[at], *B.total(rows, None, factor), "sum")
+    B.within(y[at], *B.normed(h[at], None, 1e-6), "norm")
+    kept = h[at]
+    del y, h
+    out = nn.dropout_add(x, None, 0.5, seed)
+    assert torch.equal(out[at], kept)
+    out[at] = 0
+    assert not out.any()
+    del out
+    q, scales = nn.quantize_rows(x)
+    few = nn.quantize_rows(rows)
+    assert torch.equal(q[at], few[0]) and torch.equal(scales[at], few[1])
+    q[at] = 0
+    assert not q.any()
+
+
 def test_captured_seeds():
     """Seeds that a captured call draws are new ones at every replay."""
     from FGMS import nn
