@@ -119,12 +119,14 @@ __device__ __forceinline__ void add(Eight &to, const Eight &v) {
 
 // How a row lies on its lanes: lane l of `lanes` (a power of two) has chunks l, l + lanes, ... of eight channels, `chunks` of them.  Up to 2048
 // channels a row is a wave's or less and is summed by exchanges between lanes alone; the widest take 1024 threads, whose registers
-// hold two chunks.
+// hold two chunks.  Gradients have rows of 2049 to 8192 channels on a chunk a thread, which leaves room to ask for the next row (4096 rows of 8192, fp32: 121 us
+// on 256 threads, 110 so).
 struct Share {
   int lanes, chunks, threads;
 };
-inline Share share_of(int channels) {
+inline Share share_of(int channels, bool gradient = false) {
   const int all = (channels + 7) / 8;
+  if (gradient && all > 256 && all <= 1024) return all > 512 ? Share{1024, 1, 1024} : Share{512, 1, 512};
   if (all > 1024) return Share{1024, 2, 1024};
   if (all > 256) return Share{256, all > 512 ? 4 : 2, 256};
   int lanes = 1;
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a
   };
   int64_t row = (int64_t)blockIdx.x * groups + group;
   const int64_t stride = (int64_t)gridDim.x * groups;
-  constexpr bool kAhead = THREADS == 256;      // (1024 threads have no registers for it)
+  constexpr bool kAhead = THREADS * CHUNKS < 2048;      // (two chunks of 1024 threads have no registers for it)
   if (kAhead) ask(row);
   int turn = 0;      // (a row's exchanges and the next one's do not share their places)
   for (int64_t first = (int64_t)blockIdx.x * groups; first < a.n; first += stride, row += stride, turn ^= 1) {
@@ -387,6 +389,12 @@ void by_share(const Share &s, F f) {
   return s.chunks == 1 ? f(Shape<1, 256>()) : s.chunks == 2 ? f(Shape<2, 256>()) : s.chunks == 3 ? f(Shape<3, 256>()) : f(Shape<4, 256>());
 }
 template <typename F>
+void by_grad_share(const Share &s, F f) {
+  if (s.threads == 512) return f(Shape<1, 512>());
+  if (s.threads == 1024 && s.chunks == 1) return f(Shape<1, 1024>());
+  by_share(s, f);
+}
+template <typename F>
 void by_type(int dtype, F f) {
   return dtype == FGMS_F32 ? f(float()) : dtype == FGMS_F16 ? f((_Float16)0) : f((__bf16)0);
 }
@@ -448,20 +456,20 @@ int launch_rows(const RowsArgs &a, int what) {
 // As many as run at once on 256 CUs (their registers leave a SIMD five, three or two waves), or fewer that all have as many rows: the last round of
 // a grid is as long as the others.  (10007 rows of 1096, two at once: 1024 workgroups 24.8 us, 501 21.0.)
 int64_t scale_grad_groups(int64_t n, int channels) {
-  const Share s = share_of(channels);
+  const Share s = share_of(channels, true);
   const int at_once = s.threads / s.lanes;
-  const int64_t all = (n + at_once - 1) / at_once, most = 256 * (s.threads == 1024 ? 1 : s.chunks == 1 ? 5 : s.chunks == 2 ? 3 : 2);
+  const int64_t all = (n + at_once - 1) / at_once, most = 256 * (s.threads == 1024 ? 1 : s.threads == 512 ? 2 : s.chunks == 1 ? 5 : s.chunks == 2 ? 3 : 2);
   const int64_t rounds = (all + most - 1) / most;
   return rounds ? (all + rounds - 1) / rounds : 0;
 }
 
 int launch_add_norm_bwd(const RowsArgs &a) {
-  const Share s = share_of(a.channels);
+  const Share s = share_of(a.channels, true);
   const unsigned grid = (unsigned)scale_grad_groups(a.n, a.channels);
   const bool w = whole_rows(a);
   by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
-    by_share(s, [&](auto shape) {
+    by_grad_share(s, [&](auto shape) {
       constexpr int K = decltype(shape)::chunks, N = decltype(shape)::threads;
       if (w) add_norm_grad_kernel<T, K, N, true><<<grid, N, 0, a.stream>>>(a, s.lanes);
       else add_norm_grad_kernel<T, K, N, false><<<grid, N, 0, a.stream>>>(a, s.lanes);
