@@ -83,6 +83,26 @@ def test_results_stay_between_their_neighbours():
             assert (held[:3] == 5).all() and (held[3 + n * outputs:] == 5).all(), (n, outputs, c)
 
 
+def test_results_end_anywhere():
+    """Rows of results of every length over tiles of every size, that begin on four bytes, beside it, or in turns."""
+    from fgms_amd import capi
+    gen = torch.Generator().manual_seed(77)
+    for n, c, lengths in ((33, 64, range(1, 140)), (33, 300, range(50, 140)), (70, 2100, range(60, 75)), (16500, 80, range(225, 262)), (16500, 200, range(225, 262)),
+                          (33000, 1100, (511, 513, 523, 537, 549))):
+        x = torch.randint(-9, 10, (n, (c + 15) // 16 * 16), generator=gen).char().cuda()[:, :c]
+        w = torch.randint(-9, 10, (max(lengths), (c + 15) // 16 * 16), generator=gen).char().cuda()[:, :c]
+        sx, sw = (torch.full((k,), v, dtype=torch.float32, device="cuda") for k, v in ((n, 1.0), (max(lengths), 2.0 ** -8)))
+        sums = x.float() @ w.float().t() / 256      # (whole numbers under 2^24: exact)
+        for outputs in lengths:
+            for dtype in (torch.float16, torch.bfloat16):
+                held = torch.full((n * outputs + 9,), 5, dtype=dtype, device="cuda")
+                begin = 3 + outputs // 2 % 2
+                out = held[begin:begin + n * outputs].view(n, outputs)
+                capi.int8_linear(x, sx, w[:outputs], sw[:outputs], None, out)
+                assert torch.equal(out, sums[:, :outputs].to(dtype)), (n, c, outputs, dtype)
+                assert (held[:begin] == 5).all() and (held[begin + n * outputs:] == 5).all(), (n, c, outputs, dtype)
+
+
 def test_binding_refuses():
     from fgms_amd import capi
     x, q, s = torch.zeros(4, 24, device="cuda"), torch.zeros(4, 24, dtype=torch.int8, device="cuda"), torch.zeros(4, dtype=torch.float32, device="cuda")
