@@ -238,7 +238,7 @@ def _seed_for(p, seed, x):
 
 def add_norm(x, residual=None, scale=None, eps=1e-6, p=0.0, seed=None):
     """(y, h): h = residual + dropout(x), y = h * scale / sqrt(mean(h ** 2) + eps) over a row's channels, in one pass; differentiable in x,
-    residual and scale.
+    residual and scale (once: to differentiate a gradient raises NotImplementedError).
 
     x and residual ``[N, channels]`` of one shape and type (rows of a wider tensor are read as they lie), scale ``[channels]`` or None.
     h is rounded to the type before its norm is taken; where there is neither a residual nor dropout it is x itself.  ``p``: the share of

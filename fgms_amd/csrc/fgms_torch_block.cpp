@@ -65,6 +65,7 @@ struct AddNormBackward final : public torch::autograd::Node {
     const bool given = both && grads[1].defined();
     if (!grads[0].defined() && !given) return variable_list(3);
     refuse_receivers_outside_the_capture(*this, op);
+    const Once once(*this, op);
     const auto self = shared_from_this();
     const at::Tensor h = by_row(sum.unpack(self, op, "sum"));
     at::Tensor w = scale.unpack(self, op, "scale");
@@ -89,6 +90,10 @@ struct AddNormBackward final : public torch::autograd::Node {
     check(fgms_add_norm_bwd(data(g[0]), data(g[1]), data(h), data(w), data(gx), data(g_residual), data(gw), (float *)data(sums), h.size(0),
                             (int)h.size(1), row_stride(h), (float)eps, (float)dropout.p, dropout.unchanged(op),
                             dtype_of(h, kOf), current_stream()));
+    const at::Tensor &g_y = grads[0], &g_h = both ? grads[1] : grads[0];
+    once(g_residual, {&g_y, &g_h}, {0, 1, 2});
+    once(gx, {&g_y, &g_h}, {0, 1, 2});
+    once(gw, {&g_y}, {0, 1});
     if (!dropout.falls && wants_x) gx = g_residual;      // (the sum's own)
     return {gx, wants_residual ? g_residual : at::Tensor(), gw};
   }
@@ -152,6 +157,8 @@ at::Tensor drop(const at::Tensor &x, const at::Tensor &residual, const Dropout &
   return out;
 }
 
+at::Tensor dropout_add_node(const at::Tensor &x, const MaybeTensor &residual, double p, const MaybeTensor &seed);
+
 struct DropoutAddBackward final : public torch::autograd::Node {
   Dropout dropout;
 
@@ -161,11 +168,17 @@ struct DropoutAddBackward final : public torch::autograd::Node {
     if (!grads[0].defined()) return variable_list(2);
     refuse_receivers_outside_the_capture(*this, op);
     refuse_tangent(grads[0], op, "the output gradient");
-    at::NoGradGuard no_grad;
     c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[0].device());
     at::Tensor gx = grads[0];
-    if (!task_should_compute_output(0)) gx = at::Tensor();
-    else if (dropout.falls) gx = drop(by_row(gx), at::Tensor(), dropout, dropout.unchanged(op));
+    if (!task_should_compute_output(0)) {
+      gx = at::Tensor();
+    } else if (dropout.falls && at::GradMode::is_enabled() && gx.requires_grad()) {
+      (void)dropout.unchanged(op);
+      gx = dropout_add_node(gx, {}, dropout.p, dropout.seed.tensor);      // (the same map again, whose gradient is the same map)
+    } else if (dropout.falls) {
+      at::NoGradGuard no_grad;
+      gx = drop(by_row(gx), at::Tensor(), dropout, dropout.unchanged(op));
+    }
     return {gx, task_should_compute_output(1) ? grads[0] : at::Tensor()};
   }
 

@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/library.h>
 
@@ -12,6 +13,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -116,6 +118,41 @@ struct Index {
   const at::Tensor &unchanged(const char *op, const char *name) const {
     TORCH_CHECK(version_of(tensor) == version, op, ": ", name, " has been modified by an inplace operation between the forward and the backward pass");
     return tensor;
+  }
+};
+
+// Gradients are formed outside of any graph.  Where a graph of them is asked for (create_graph), one that depends on an input or an output gradient
+// that has a graph itself becomes the result of a node that refuses to be passed: without its part a second derivative would look right and not be.
+struct NoSecondDerivative final : public torch::autograd::Node {
+  const char *op;
+
+  explicit NoSecondDerivative(const char *op_) : op(op_) {}
+  variable_list apply(variable_list &&) override {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, op, " has no second derivatives");
+    return {};
+  }
+  std::string name() const override { return "NoSecondDerivative"; }
+};
+
+// (made before the gradients are, while the pass's own mode holds)
+struct Once {
+  const torch::autograd::Node &node;
+  const char *op;
+  bool graph = at::GradMode::is_enabled();
+
+  Once(const torch::autograd::Node &node_, const char *op_) : node(node_), op(op_) {}
+  // `grad`, a tensor of the node's own making, depends on these output gradients and on the node's inputs at these places.
+  void operator()(const at::Tensor &grad, std::initializer_list<const at::Tensor *> output_grads, std::initializer_list<size_t> inputs) const {
+    if (!graph || !grad.defined()) return;
+    torch::autograd::edge_list edges;
+    for (const at::Tensor *t : output_grads)
+      if (t->defined() && t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+    for (size_t i : inputs)
+      if (node.next_edge(i).is_valid()) edges.push_back(node.next_edge(i));
+    if (edges.empty()) return;
+    const std::shared_ptr<NoSecondDerivative> refusal(new NoSecondDerivative(op), torch::autograd::deleteNode);
+    refusal->set_next_edges(std::move(edges));
+    torch::autograd::set_history(grad, refusal);
   }
 };
 
