@@ -45,6 +45,7 @@
 #include "fgms_diag.h"
 #include "fgms_torch_attention.h"
 #include "fgms_torch_block.h"
+#include "fgms_torch_nodes.h"
 
 namespace {
 
@@ -380,6 +381,7 @@ struct SparseConvBackward final : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+    const fgms_nodes::Once once(*this, "sparse_conv");
     at::Tensor x = unpacked(feats, feats_shape, "feats"), w = unpacked(weight, weight_shape, "weight");
     refuse_tangent(grads[0], "the output gradient");
     at::NoGradGuard no_grad;
@@ -398,6 +400,8 @@ struct SparseConvBackward final : public torch::autograd::Node {
                         gw.defined() ? gw.data_ptr() : nullptr, i32(map.kpos), i32(map.in_map), i32(map.out_map), tf32,
                         map.n_in, map.n_out, (int)w.size(1), (int)w.size(2), k_vol, map.in_map.numel(), dtype_of(x), plan.get(),
                         stream));
+    once(gx, {&grads[0]}, {1});
+    once(gw, {&grads[0]}, {0});
     return {gx, gw};
   }
 

@@ -24,6 +24,7 @@ struct NormRotaryBackward final : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     static const char op[] = "norm_rotary";
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(4);
+    const Once once(*this, op);
     const auto self = shared_from_this();
     at::Tensor x[2] = {q.unpack(self, op, "q"), k.unpack(self, op, "k")};
     at::Tensor w[2] = {q_scale.unpack(self, op, "q_scale"), k_scale.unpack(self, op, "k_scale")};
@@ -45,6 +46,10 @@ struct NormRotaryBackward final : public torch::autograd::Node {
                                (int)x[0].size(1), (int)x[1].size(1), (int)x[0].size(2), x[0].stride(0), x[0].stride(1), x[1].stride(0),
                                x[1].stride(1), (int)turn.sections.size(), turn.sections.data(), turn.interleaved, (float)turn.eps,
                                dtype_of(x[0]), current_stream()));
+    for (size_t i = 0; i < 2; ++i) {
+      once(gx[i], {&grads[i]}, {i, 2 + i});
+      once(gw[i], {&grads[i]}, {i});
+    }
     return {gx[0], gx[1], gw[0], gw[1]};
   }
 
@@ -135,6 +140,7 @@ struct SegmentAttentionBackward final : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     static const char op[] = "segment_attention";
     if (!grads[0].defined()) return variable_list(3);
+    const Once once(*this, op);
     const auto self = shared_from_this();
     at::Tensor x[3] = {q.unpack(self, op, "q"), k.unpack(self, op, "k"), v.unpack(self, op, "v")};
     at::Tensor o = out.unpack(self, op, "result"), l = lse.unpack(self, op, "log-sums");
@@ -156,6 +162,9 @@ struct SegmentAttentionBackward final : public torch::autograd::Node {
                                      (int)q_offsets.numel() - 1, (int)x[0].size(1), (int)x[1].size(1), (int)x[0].size(2),
                                      x[0].stride(0), x[0].stride(1), x[1].stride(0), x[1].stride(1), x[2].stride(0), x[2].stride(1),
                                      segments.causal, (float)segments.scale, dtype_of(x[0]), current_stream()));
+    once(gx[0], {&grads[0]}, {0, 1, 2});
+    once(gx[1], {&grads[0]}, {0, 1, 2});
+    once(gx[2], {&grads[0]}, {0, 1});
     return {gx[0], gx[1], gx[2]};
   }
 

@@ -93,3 +93,53 @@ def test_blocks_still_train_with_a_graph_of_their_gradients():
     got = torch.autograd.grad(loss, list(block.parameters()), create_graph=True)
     for a, b in zip(want, got):
         assert float((a - b).detach().abs().max()) < 4096 * 2.0 ** -24 * float(a.abs().max())
+
+
+def refuses(grads, of):
+    """The gradients that depend on `of` refuse a second pass, also beside a path of torch's own."""
+    for g in grads:
+        with pytest.raises(NotImplementedError, match="second derivatives"):
+            torch.autograd.grad(g.sum() + (of ** 2).sum(), of, retain_graph=True)
+
+
+def test_attention_refuses():
+    from FGMS import nn
+    from tests import attention_util as U
+    gen = torch.Generator().manual_seed(4)
+    q, k, v, g, gk = (torch.randn(30, 2, 16, generator=gen).cuda().requires_grad_() for _ in range(5))
+    w, u = torch.randn(2, 16, generator=gen).cuda().unbind()
+    w, u = w.clone().requires_grad_(), u.clone().requires_grad_()
+    coords, freqs = torch.randint(0, 50, (30, 3), generator=gen, dtype=torch.int32).cuda(), nn.rotary_freqs((3, 3, 2)).cuda()
+    turned = nn.norm_rotary(q, k, w, u, coords, freqs, (3, 3, 2))
+    want = torch.autograd.grad(turned, (q, k, w, u), (g, gk), retain_graph=True)
+    gq_, gk_, gw, gu = torch.autograd.grad(turned, (q, k, w, u), (g, gk), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, (gq_, gk_, gw, gu)))
+    refuses((gq_, gw), q), refuses((gq_,), w), refuses((gq_, gw), g)
+    refuses((gk_, gu), k), refuses((gk_,), u), refuses((gk_, gu), gk)
+    # (neither side's gradients have a part of the other's)
+    extra = torch.autograd.grad(gq_.sum() + (k ** 2).sum(), k, retain_graph=True)[0]
+    assert torch.equal(extra, 2 * k)
+    out = nn.segment_attention(q, k, v, U.offsets([10, 20]))
+    want = torch.autograd.grad(out, (q, k, v), g, retain_graph=True)
+    got = torch.autograd.grad(out, (q, k, v), g, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    refuses(got, q), refuses(got, k), refuses(got, g), refuses(got[:2], v)
+    # values alone: a linear map, whose gradient by constants is one
+    got, = torch.autograd.grad(nn.segment_attention(q.detach(), k.detach(), v, U.offsets([10, 20])), v, g.detach(), create_graph=True)
+    assert not got.requires_grad
+
+
+def test_sparse_conv_refuses():
+    from fgms_amd import clouds
+    from FGMS import nn
+    from tests.test_gpu_voxel_attention import small_cloud
+    coords = small_cloud(1)
+    kmap = nn.KernelMap.from_coords(coords, coords, clouds.offsets_cube(3))
+    gen = torch.Generator().manual_seed(5)
+    x, w = torch.randn(len(coords), 32, generator=gen).cuda().requires_grad_(), torch.randn(27, 32, 32, generator=gen).cuda().requires_grad_()
+    g = torch.randn(len(coords), 32, generator=gen).cuda().requires_grad_()
+    gx, gw = torch.autograd.grad(nn.sparse_conv(x, w, kmap), (x, w), g, create_graph=True)
+    refuses((gx,), w), refuses((gw,), x), refuses((gx, gw), g)
+    assert torch.equal(torch.autograd.grad(gx.sum() + (x ** 2).sum(), x, retain_graph=True)[0], 2 * x)
+    gx, = torch.autograd.grad(nn.sparse_conv(x, w.detach(), kmap), x, g.detach(), create_graph=True)
+    assert not gx.requires_grad
