@@ -302,14 +302,39 @@ at::Tensor int8_linear_op(const at::Tensor &x_, const at::Tensor &x_scales, cons
 
 }  // namespace
 
-// Under torch.jit.trace all go through torch's dispatcher, as sparse_conv does.
+// Under torch.jit.trace all go through torch's dispatcher, as sparse_conv does.  An operator's results there are tensors of its own: where the sum is x itself,
+// the norm's own operators are recorded and x is handed on beside them; the others, called by name, leave a copy of it.
+namespace {
+
+std::tuple<at::Tensor, at::Tensor> add_norm_op(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &scale, double eps, double p,
+                                               const MaybeTensor &seed) {
+  const auto [y, h] = add_norm_node(x, residual, scale, eps, p, seed);
+  return {y, h.is_same(x) ? x.clone() : h};
+}
+at::Tensor norm_op(const at::Tensor &x, const MaybeTensor &scale, double eps) { return std::get<0>(add_norm_node(x, {}, scale, eps, 0, {})); }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_norm_int8_own(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &scale, double eps) {
+  const auto [q, scales, h] = add_norm_int8_op(x, residual, scale, eps);
+  return {q, scales, h.is_same(x) ? x.clone() : h};
+}
+std::tuple<at::Tensor, at::Tensor> norm_int8_op(const at::Tensor &x, const MaybeTensor &scale, double eps) {
+  const auto all = add_norm_int8_op(x, {}, scale, eps);
+  return {std::get<0>(all), std::get<1>(all)};
+}
+
+}  // namespace
+
 #define FGMS_TRACED(name, f) \
   static const auto traced = c10::Dispatcher::singleton().findSchemaOrThrow("fgms::" name, "").typed<decltype(f)>()
 
 std::tuple<at::Tensor, at::Tensor> add_norm(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &scale, double eps, double p,
                                             const MaybeTensor &seed) {
   if (!torch::jit::tracer::isTracing()) return add_norm_node(x, residual, scale, eps, p, seed);
-  FGMS_TRACED("add_norm", add_norm_node);
+  if (!or_none(residual).defined() && !Dropout(seed, p, x).falls) {
+    FGMS_TRACED("norm", norm_op);
+    return {traced.call(x, scale, eps), x};
+  }
+  FGMS_TRACED("add_norm", add_norm_op);
   return traced.call(x, residual, scale, eps, p, seed);
 }
 
@@ -327,7 +352,12 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor &x, bool gated
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_norm_int8(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &scale, double eps) {
   if (!torch::jit::tracer::isTracing()) return add_norm_int8_op(x, residual, scale, eps);
-  FGMS_TRACED("add_norm_int8", add_norm_int8_op);
+  if (!or_none(residual).defined()) {
+    FGMS_TRACED("norm_int8", norm_int8_op);
+    const auto [q, scales] = traced.call(x, scale, eps);
+    return {q, scales, x};
+  }
+  FGMS_TRACED("add_norm_int8", add_norm_int8_own);
   return traced.call(x, residual, scale, eps);
 }
 
@@ -339,9 +369,11 @@ at::Tensor int8_linear(const at::Tensor &x, const at::Tensor &x_scales, const at
 }
 
 TORCH_LIBRARY_FRAGMENT(fgms, m) {
-  m.def("add_norm(Tensor x, Tensor? residual, Tensor? scale, float eps, float p, Tensor? seed) -> (Tensor, Tensor)", &add_norm_node);
+  m.def("add_norm(Tensor x, Tensor? residual, Tensor? scale, float eps, float p, Tensor? seed) -> (Tensor, Tensor)", &add_norm_op);
+  m.def("norm(Tensor x, Tensor? scale, float eps) -> Tensor", &norm_op);
   m.def("dropout_add(Tensor x, Tensor? residual, float p, Tensor? seed) -> Tensor", &dropout_add_node);
   m.def("quantize_rows(Tensor x, bool gated) -> (Tensor, Tensor)", &quantize_rows_op);
-  m.def("add_norm_int8(Tensor x, Tensor? residual, Tensor? scale, float eps) -> (Tensor, Tensor, Tensor)", &add_norm_int8_op);
+  m.def("add_norm_int8(Tensor x, Tensor? residual, Tensor? scale, float eps) -> (Tensor, Tensor, Tensor)", &add_norm_int8_own);
+  m.def("norm_int8(Tensor x, Tensor? scale, float eps) -> (Tensor, Tensor)", &norm_int8_op);
   m.def("int8_linear(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype) -> Tensor", &int8_linear_op);
 }
