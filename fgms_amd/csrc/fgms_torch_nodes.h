@@ -158,7 +158,8 @@ struct Once {
 
 // A gradient that is handed on under stream capture is waited for on the stream that its receiver was made on, which joins the capture and
 // never leaves it if it is none of the capture's: the capture's end then takes the process with it.  That is so where an eager graph of the
-// same leaves is still alive (its nodes receive their gradients): refused before anything is queued.
+// same leaves is still alive (its nodes receive their gradients): refused before anything is queued.  (A gradient that the pass does not ask for is handed
+// to nobody.)
 inline void refuse_receivers_outside_the_capture(const torch::autograd::Node &node, const char *op) {
   const auto capturing = [](hipStream_t stream) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -166,6 +167,7 @@ inline void refuse_receivers_outside_the_capture(const torch::autograd::Node &no
   };
   if (!capturing(current_stream())) return;
   for (size_t i = 0; i < node.num_outputs(); ++i) {
+    if (!node.task_should_compute_output(i)) continue;
     const auto &receiver = node.next_edge(i).function;
     const auto stream = receiver ? receiver->stream() : std::nullopt;
     TORCH_CHECK(!stream || capturing(c10::hip::HIPStreamMasqueradingAsCUDA(*stream).stream()), op,
