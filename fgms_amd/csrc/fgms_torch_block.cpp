@@ -52,6 +52,18 @@ struct Dropout {
   const int64_t *unchanged(const char *op) const { return seed.tensor.defined() ? seed.unchanged(op, "seed").data_ptr<int64_t>() : nullptr; }
 };
 
+at::Tensor drop(const at::Tensor &x, const at::Tensor &residual, const Dropout &dropout, const int64_t *seed);
+at::Tensor dropout_add_node(const at::Tensor &x, const MaybeTensor &residual, double p, const MaybeTensor &seed);
+
+// The gradient of a sum on its way to the branch that was dropped from: the same map again, whose gradient is the same map.
+at::Tensor dropped_grad(const at::Tensor &g, const Dropout &dropout, const char *op) {
+  if (!dropout.falls) return g;
+  const int64_t *const seed = dropout.unchanged(op);
+  if (at::GradMode::is_enabled() && g.requires_grad()) return dropout_add_node(g, {}, dropout.p, dropout.seed.tensor);
+  at::NoGradGuard no_grad;
+  return drop(by_row(g), at::Tensor(), dropout, seed);
+}
+
 // ------------------------------------------------------------------------------------------------ sums and norms
 struct AddNormBackward final : public torch::autograd::Node {
   Saved sum, scale;
@@ -65,6 +77,13 @@ struct AddNormBackward final : public torch::autograd::Node {
     const bool given = both && grads[1].defined();
     if (!grads[0].defined() && !given) return variable_list(3);
     refuse_receivers_outside_the_capture(*this, op);
+    const bool wants_x = task_should_compute_output(0), wants_residual = task_should_compute_output(1);
+    if (!grads[0].defined()) {      // (the norm has no part in it, whatever its rows hold)
+      refuse_tangent(grads[1], op, "the output gradient");
+      c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[1].device());
+      return {wants_x ? dropped_grad(grads[1], dropout, op) : at::Tensor(), wants_residual ? grads[1] : at::Tensor(),
+              task_should_compute_output(2) ? at::zeros(scale.shape, scale.options.requires_grad(false)) : at::Tensor()};
+    }
     const Once once(*this, op);
     const auto self = shared_from_this();
     const at::Tensor h = by_row(sum.unpack(self, op, "sum"));
@@ -76,10 +95,8 @@ struct AddNormBackward final : public torch::autograd::Node {
     for (int i = 0; i < (both ? 2 : 1); ++i) {
       refuse_tangent(grads[i], op, "the output gradient");
       if (grads[i].defined()) g[i] = packed(grads[i]);
-      else if (i == 0) g[i] = at::zeros(h.sizes(), h.options().requires_grad(false));
       FGMS_NEED(!g[i].defined() || g[i].scalar_type() == h.scalar_type(), "the output gradient must have the dtype of x");
     }
-    const bool wants_x = task_should_compute_output(0), wants_residual = task_should_compute_output(1);
     at::Tensor gx, g_residual, gw, sums;
     if (dropout.falls && wants_x) gx = result(h.sizes(), h);
     if (wants_residual || (wants_x && !dropout.falls)) g_residual = result(h.sizes(), h);
@@ -157,8 +174,6 @@ at::Tensor drop(const at::Tensor &x, const at::Tensor &residual, const Dropout &
   return out;
 }
 
-at::Tensor dropout_add_node(const at::Tensor &x, const MaybeTensor &residual, double p, const MaybeTensor &seed);
-
 struct DropoutAddBackward final : public torch::autograd::Node {
   Dropout dropout;
 
@@ -169,16 +184,7 @@ struct DropoutAddBackward final : public torch::autograd::Node {
     refuse_receivers_outside_the_capture(*this, op);
     refuse_tangent(grads[0], op, "the output gradient");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(grads[0].device());
-    at::Tensor gx = grads[0];
-    if (!task_should_compute_output(0)) {
-      gx = at::Tensor();
-    } else if (dropout.falls && at::GradMode::is_enabled() && gx.requires_grad()) {
-      (void)dropout.unchanged(op);
-      gx = dropout_add_node(gx, {}, dropout.p, dropout.seed.tensor);      // (the same map again, whose gradient is the same map)
-    } else if (dropout.falls) {
-      at::NoGradGuard no_grad;
-      gx = drop(by_row(gx), at::Tensor(), dropout, dropout.unchanged(op));
-    }
+    const at::Tensor gx = task_should_compute_output(0) ? dropped_grad(grads[0], dropout, op) : at::Tensor();
     return {gx, task_should_compute_output(1) ? grads[0] : at::Tensor()};
   }
 
