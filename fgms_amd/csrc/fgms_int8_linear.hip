@@ -109,14 +109,15 @@ struct Results {
   static __device__ __forceinline__ int place(int i, int lane) { return 2 * N * i + N * (lane / 32); }
 };
 
-// `there` outputs of a row are there, from `to` on; those of a chunk at `at`, from its element `from` on.
+// `left` outputs from `to` on are there; those of a chunk from its element `from` on.  (Places are compared as what is left of a row against numbers that
+// the instruction holds: sums of a place and a number would each take a register.)
 template <typename T>
-__device__ __forceinline__ void store_elements(T *to, int at, int there, const int4v &chunk, int from) {
+__device__ __forceinline__ void store_elements(T *to, int left, const int4v &chunk, int from) {
   typedef T Tn __attribute__((ext_vector_type(16 / sizeof(T))));
   const Tn all = __builtin_bit_cast(Tn, chunk);
 #pragma unroll
   for (int e = 0; e < 16 / (int)sizeof(T); ++e)
-    if (e >= from && at + e < there) to[at + e] = all[e];
+    if (e >= from && e < left) to[e] = all[e];
 }
 
 // 16 bytes at a time, wherever an element or two begin.
@@ -131,8 +132,8 @@ __device__ __forceinline__ void store_row(T *to, const int16v (&acc)[NB][MB], in
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int at = 32 * j + r.place(c, lane);
-      if (at + r.N <= there) *reinterpret_cast<Anywhere *>(to + at) = r.chunk[c];
-      else store_elements<T>(to, at, there, r.chunk[c], 0);
+      if (r.N <= there - at) *reinterpret_cast<Anywhere *>(to + at) = r.chunk[c];
+      else store_elements<T>(to + at, there - at, r.chunk[c], 0);
     }
   }
 }
@@ -155,7 +156,7 @@ __device__ __forceinline__ void store_odd_row(T *to, const int16v (&acc)[NB][MB]
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int4v d = now.chunk[c];
-      const int at = 32 * j + now.place(c, lane);
+      const int at = 32 * j + now.place(c, lane), left = there - at;
       // the next chunk is the partner's: the same for the lower lanes, for the upper ones the one after
       int a = d[0], b = c == 0 ? now.chunk[1][0] : j + 1 < NB ? next.chunk[0][0] : 0;
       swap_halves(a, b);
@@ -163,13 +164,13 @@ __device__ __forceinline__ void store_odd_row(T *to, const int16v (&acc)[NB][MB]
       const bool last = c == 1 && j == NB - 1 && lane >= 32;      // (what follows is another wave's)
       const int4v s = {(int)__builtin_amdgcn_alignbit((unsigned)d[1], (unsigned)d[0], shift), (int)__builtin_amdgcn_alignbit((unsigned)d[2], (unsigned)d[1], shift),
                        (int)__builtin_amdgcn_alignbit((unsigned)d[3], (unsigned)d[2], shift), (int)__builtin_amdgcn_alignbit((unsigned)follows, (unsigned)d[3], shift)};
-      if (at + 8 + (int)odd <= there && !(last && odd)) {
+      if (8 + (int)odd <= left && !(last && odd)) {
         *reinterpret_cast<Four *>(to + at + odd) = s;
-      } else if (last && odd && at + 8 <= there) {
+      } else if (last && odd && 8 <= left) {
         *reinterpret_cast<Three *>(to + at + 1) = int3v{s[0], s[1], s[2]};
         to[at + 7] = __builtin_bit_cast(T, (unsigned short)((unsigned)d[3] >> 16));
       } else {
-        store_elements<T>(to, at, there, d, (int)odd);
+        store_elements<T>(to + at, left, d, (int)odd);
       }
     }
     now = next;
