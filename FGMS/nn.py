@@ -272,8 +272,8 @@ def int8_linear(x, x_scales, weight, weight_scales, bias=None, dtype=torch.float
 
 
 class Int8Linear(torch.nn.Module):
-    """A linear layer for inference with its weights in 8 bits and a scale for each output; its rows are brought to 8 bits on the way in:
-    ``y = layer(x)``, or ``y = layer((q, scales))`` of rows that are there already."""
+    """A linear layer for inference, of up to 16384 channels, with its weights in 8 bits and a scale for each output; its rows are brought to 8 bits on
+    the way in: ``y = layer(x)``, or ``y = layer((q, scales))`` of rows that are there already."""
 
     def __init__(self, linear):
         super().__init__()
