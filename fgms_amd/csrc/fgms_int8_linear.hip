@@ -139,7 +139,8 @@ __device__ __forceinline__ void store_row(T *to, const int16v (&acc)[NB][MB], in
 }
 
 // ... where rows may begin half-way through four bytes (an odd number of outputs): such a row's chunks are shifted by an element, whose place the next
-// chunk's first fills.  (50000 rows of 256 to 767, bf16: 34.8 us, with stores of 16 bytes beside four-byte boundaries 44.7; to 768 25.3.)
+// chunk's first fills.  (50000 rows of 256 to 767, bf16, from memory: 37.2 us over three sets of tensors, with stores of 16 bytes beside four-byte boundaries
+// 47.6; to 768 31.0.)
 template <typename T, int MB, int NB>
 __device__ __forceinline__ void store_odd_row(T *to, const int16v (&acc)[NB][MB], int i, float by, const float *scales, const float *biases, int there, int lane) {
   typedef int4v Four __attribute__((aligned(4)));
@@ -351,7 +352,8 @@ __global__ __launch_bounds__(256 * KW, (MB * NB >= 16 ? 1 : KW > 1 ? KW : DEPTH 
 }
 
 // Few rows of x: the weights' way from memory counts.  A workgroup has 16 outputs, its waves take turns along the depth, 256 bytes of each row at
-// a time, straight into registers, and add their sums up in LDS.  (16 rows of 11008 to 4096: 45 MB in 12 us; one of 4096 to 4096: 17 MB in 5.3.)
+// a time, straight into registers, and add their sums up in LDS.  (16 rows of 11008 to 4096: 45 MB in 14.6 us from memory, 12.8 where a cache holds
+// the weights; one of 4096 to 4096: 17 MB in 6.9 and 4.9.)
 template <typename T, int MB>
 __global__ __launch_bounds__(512) void int8_linear_few_kernel(const Int8LinearArgs a) {
   constexpr int kWaves = 8, kSteps = 4;
@@ -428,7 +430,10 @@ int launch_few(const Int8LinearArgs &a) {
 // outputs, 1024 deep: 128 us with 256 as with 128, 2048 deep 201 and 220, 512 deep 104 and 85), 128, and 64 with two fours along the depth, or four
 // where the tiles are not even one a CU (256 x 4096 x 4096: 12.7 us with two, 11.1 with four, 21.6 with tiles of 128; 512 rows 14.9, 21.3, 22.3).  Up to 128
 // deep a tile has 64 bytes of depth and a CU twice the workgroups, which hide each other's ends (120000 rows of 128 to 384: 25.6 -> 22.9 us; 50000
-// of 256 to 768 the other way, 25.9 -> 29.4), up to 64 outputs in tiles that these fill (200000 rows of 64 to 64: 11.5 -> 10.1).
+// of 256 to 768 the other way, 25.9 -> 29.4), up to 64 outputs in tiles that these fill (200000 rows of 64 to 64: 11.5 -> 10.1).  All of these with one set of
+// tensors, which the last-level cache holds where it can; from memory 256 x 4096 x 4096 takes 15.2 us, 120000 of 128 to 384 36, 50000 of 256 to 768 33, 200000 of
+// 64 to 64 14.  The rule goes by the number of tiles and not by how far rows fill them: one row of 4096 to 128256 outputs runs in tiles of 256 (526 MB of
+// weights in 136 us).
 template <typename T>
 int launch(const Int8LinearArgs &a) {
   const auto tiles = [&](int64_t side) { return ((a.n + side - 1) / side) * ((a.outputs + side - 1) / side); };

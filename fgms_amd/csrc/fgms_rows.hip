@@ -119,8 +119,8 @@ __device__ __forceinline__ void add(Eight &to, const Eight &v) {
 
 // How a row lies on its lanes: lane l of `lanes` (a power of two) has chunks l, l + lanes, ... of eight channels, `chunks` of them.  Up to 2048
 // channels a row is a wave's or less and is summed by exchanges between lanes alone; the widest take 1024 threads, whose registers
-// hold two chunks.  Gradients have rows of 2049 to 8192 channels on a chunk a thread, which leaves room to ask for the next row (4096 rows of 8192, fp32: 121 us
-// on 256 threads, 110 so).
+// hold two chunks.  Gradients have rows of 2049 to 8192 channels on a chunk a thread, which leaves room to ask for the next row (4096 rows of 8192, fp32, the
+// norm's gradient, the sum's, the sum and the result, 537 MB, with the scale's second launch: 121 us on 256 threads, 110 so; fp16 76 and 72).
 struct Share {
   int lanes, chunks, threads;
 };
@@ -152,7 +152,8 @@ __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 __device__ __forceinline__ unsigned larger_of(unsigned a, unsigned b) { return a > b ? a : b; }
 
 // A row to each group of lanes, once: what a launch of any kind (WHAT) reads and writes is all that memory moves.  (50000 rows of 256, fp32: 205 MB in
-// 41 us, 5.0 TB/s; 120000 of 128, fp16, with dropout: 123 MB in 25 us; 200000 of 64 to eight bits: 90 MB in 18 to 19 us; 16 gated rows of 11008: 5 us.)
+// 41 us, 5.0 TB/s; 16384 of 2048, fp16: 268 MB in 46 us, 5.8 TB/s; 120000 of 128, fp16, with dropout: 123 MB in 25 us; a norm of 200000 of 64 to eight bits:
+// 90 MB in 19 to 21 us; 200000 of 64 as they are, fp16 to eight bits: 39 MB in 12 us; 16 gated rows of 11008: 5.7 us.)
 template <typename T, int CHUNKS, int THREADS, bool WHOLE, int WHAT>
 __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lanes) {
   constexpr bool NORM = WHAT == kRowsNorm || WHAT == kRowsNormEighths;
@@ -180,7 +181,9 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const Eight b = other[i].values();
-      // (the exponential and the reciprocal as the unit gives them: of 2 M values two fall to the other side of a border, as many as with divisions)
+      // (the exponential and the reciprocal as the unit gives them: of 2 M values two fall to the other side of a border, as many as with divisions; where the
+      // exponential's reciprocal is no normal number, a below -87.3, silu counts as zero.  50000 rows of 256, fp16: 16.1 us, 18.3 with the argument's rest and a
+      // Newton step; fp32 21.6 and 22.0)
       v[i].each([&](float &t, int e) { t = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)) * b[e]; });
     }
   }
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
       for (int e = 0; e < 8; ++e) {
         // The quotient by the step, rounded as a division rounds it (halves are met where they are meant): its remainder is exact, the first correction
         // brings it within its last bit, the second is right with a reciprocal that is (P. Markstein, IBM J. Res. Dev. 34, 1990).  A division's own
-        // steps take 10 to 25 % longer (200000 rows of 64 12.4 us, this 10.5).
+        // steps take 10 to 25 % longer (200000 rows of 64 that a cache holds 12.4 us, this 10.5 to 10.8; from memory this takes 12.2).
         const float value = v[i][e], near = value * by, nearer = __builtin_fmaf(__builtin_fmaf(-near, step, value), by, near);
         const float quotient = __builtin_fmaf(__builtin_fmaf(-nearer, step, value), by, nearer);
         q[e] = some ? (int8_t)(int)__builtin_rintf(quotient) : (int8_t)0;
@@ -260,7 +263,8 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(const RowsArgs a, int lan
 
 // A workgroup goes through the rows in steps of the grid and keeps its lanes' sums of the scale's gradient in registers.  The next row is asked for
 // before this one is worked on: the registers of three chunks leave two waves a SIMD, whose loads alone would not keep memory busy.  (120000 rows of 128,
-// fp16, with dropout: 154 MB in 32 us; 10007 of 1096, bf16: 88 MB in 21 us.)
+// fp16, with dropout: 154 MB in 32 to 34 us; 10007 of 1096, bf16: 88 MB in 21 to 23 us; 50000 of 256, fp32: 205 MB in 42 us; 4096 of 16384, fp16, where
+// nothing is asked for ahead: 537 MB in 117 us.)
 template <typename T, int CHUNKS, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a, int lanes) {
   __shared__ float parts[2][2][THREADS / 64];
@@ -344,7 +348,8 @@ __global__ __launch_bounds__(THREADS) void add_norm_grad_kernel(const RowsArgs a
   }
 }
 
-// out[channel] = the workgroups' sums, eight channels a workgroup, 32 threads each, in a fixed order.  (1250 sums of 128, or 501 of 1096: 4 us.)
+// out[channel] = the workgroups' sums, eight channels a workgroup, 32 threads each, in a fixed order.  (1250 sums of 128: 5.5 us, 501 of 1096: 4.4, 256 of 16384:
+// 11.8.)
 template <typename T>
 __global__ __launch_bounds__(256) void column_sums_kernel(const float *__restrict__ sums, int64_t groups, int channels, T *__restrict__ out) {
   __shared__ float part[4][8];
@@ -359,8 +364,8 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float *__restric
   if (threadIdx.x < 8 && column < channels) out[column] = (T)(part[0][c] + part[1][c] + part[2][c] + part[3][c]);
 }
 
-// Eight elements a thread, counted through the rows; their words while they are on their way.  (200000 rows of 64, fp32: 154 MB in 27 us; 16384 of 4096,
-// bf16: 403 MB in 74 us.)
+// Eight elements a thread, counted through the rows; their words while they are on their way.  (200000 rows of 64, fp32: 154 MB in 28 us; 16384 of 4096,
+// bf16: 403 MB in 70 to 72 us, 5.7 TB/s.)
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const RowsArgs a, int64_t chunks) {
   const int per_row = (a.channels + 7) / 8;
@@ -453,8 +458,9 @@ int launch_rows(const RowsArgs &a, int what) {
   return FGMS_OK;
 }
 
-// As many as run at once on 256 CUs (their registers leave a SIMD five, three or two waves), or fewer that all have as many rows: the last round of
-// a grid is as long as the others.  (10007 rows of 1096, two at once: 1024 workgroups 24.8 us, 501 21.0.)
+// About as many as run at once on 256 CUs, or fewer that all have as many rows: the last round of a grid is as long as the others.  (10007 rows of 1096, two
+// at once: 1024 workgroups 24.8 us, 501 21.0.)  The counts are those of 16-bit rows of one to three chunks, whose registers leave a SIMD five, three or two
+// waves; fp32 rows on 16 bytes leave four, two and one, rows of four chunks one in every type, so that some of their workgroups start behind the others.
 int64_t scale_grad_groups(int64_t n, int channels) {
   const Share s = share_of(channels, true);
   const int at_once = s.threads / s.lanes;

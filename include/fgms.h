@@ -351,8 +351,8 @@ int fgms_segment_attention_bwd(const void *out_grad, const void *q, const void *
 /*
  * What goes around attention in a block: a branch joins the residual stream, and the sum's norm goes into the next branch; at inference the
  * rows go there in 8 bits, with a scale each.  No counterpart in the reference.  Types: FGMS_F32, FGMS_F16, FGMS_BF16.  Rows of 1 to 16384 channels,
- * which lie side by side; row strides in ELEMENTS; results and gradients are contiguous unless they have a stride.  Rows that all begin
- * on 16 bytes and hold a multiple of 8 channels are read 16 bytes at a time, any others element by element.  Sums, norms and maxima are fp32.
+ * which lie side by side; row strides in ELEMENTS; results and gradients are contiguous unless they have a stride.  Rows are read and written
+ * 16 bytes at a time, wherever they begin, but for what is left of them behind whole eights of channels.  Sums, norms and maxima are fp32.
  */
 
 /*
@@ -380,7 +380,7 @@ int fgms_dropout_add(const void *x, const void *residual, void *out, int64_t n, 
 
 /*
  * Rows in 8 bits: scales[i] = max |v| / 127, out[i][c] = v[c] / scales[i] to the nearest whole number, even ones first, of
- *   fgms_quantize_rows: v = x, or with gated != 0 v = silu(a) b of rows (a, b) of 2 * channels
+ *   fgms_quantize_rows: v = x, or with gated != 0 v = silu(a) b of rows (a, b) of 2 * channels (silu of a below -87.3 counts as 0)
  *   fgms_add_norm_int8: v = y of fgms_add_norm_fwd (before it is rounded to the type), without dropout
  * out_row: bytes, channels at least; what lies between the rows stays.  A row with an infinity or NaN has scale NaN and zeros, one
  * whose scale would be below 2^-126 scale 0 and zeros.
