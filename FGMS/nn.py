@@ -289,8 +289,9 @@ class Int8Linear(torch.nn.Module):
     def _apply(self, fn, recurse=True):
         scales = self.weight_scales
         super()._apply(fn, recurse)
-        # (scales stay fp32 whatever the layer is cast to; its results are of the type)
-        self.weight_scales = scales.to(self.weight.device)
+        # (weights stay in 8 bits and scales in fp32 whatever the layer is cast to; its results are of the type)
+        self.weight = self.weight.to(torch.int8)
+        self.weight_scales = torch.empty_like(scales, device=self.weight.device) if scales.is_meta else scales.to(self.weight.device)
         if self.weight.stride(0) % 16:      # (a copy's rows lie next to each other: on 16 bytes again, or every call would copy them)
             held = self.weight.new_zeros(self.out_features, (self.in_features + 15) // 16 * 16)
             held[:, :self.in_features] = self.weight
