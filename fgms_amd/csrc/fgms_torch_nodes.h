@@ -127,9 +127,9 @@ struct NoSecondDerivative final : public torch::autograd::Node {
   const char *op;
 
   explicit NoSecondDerivative(const char *op_) : op(op_) {}
-  variable_list apply(variable_list &&) override {
-    TORCH_CHECK_NOT_IMPLEMENTED(false, op, " has no second derivatives");
-    return {};
+  variable_list apply(variable_list &&grads) override {
+    TORCH_CHECK_NOT_IMPLEMENTED(!grads[0].defined(), op, " has no second derivatives");
+    return variable_list(num_outputs());      // (no gradient came)
   }
   std::string name() const override { return "NoSecondDerivative"; }
 };

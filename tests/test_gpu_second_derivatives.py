@@ -143,3 +143,26 @@ def test_sparse_conv_refuses():
     assert torch.equal(torch.autograd.grad(gx.sum() + (x ** 2).sum(), x, retain_graph=True)[0], 2 * x)
     gx, = torch.autograd.grad(nn.sparse_conv(x, w.detach(), kmap), x, g.detach(), create_graph=True)
     assert not gx.requires_grad
+
+
+class Takes(torch.autograd.Function):
+    """b, whatever a is: a's gradient is none."""
+
+    @staticmethod
+    def forward(ctx, a, b):
+        return b.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None, g
+
+
+def test_passes_that_bring_no_gradient():
+    """A gradient that a pass reaches and brings nothing to refuses nothing."""
+    from FGMS import nn
+    x, v, w = features(20, 64, 11).requires_grad_(), features(20, 64, 12).requires_grad_(), features(1, 64, 13)[0]
+    g, = torch.autograd.grad(nn.add_norm(x, None, w)[0], x, v, create_graph=True)
+    gx, gv, gg = torch.autograd.grad(Takes.apply(g, v * 2).sum(), (x, v, g), allow_unused=True, retain_graph=True)
+    assert gx is None and gg is None and torch.equal(gv, torch.full_like(v, 2))
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        torch.autograd.grad((Takes.apply(g, v) + g).sum(), x)
